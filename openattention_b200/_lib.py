@@ -44,6 +44,17 @@ SIGNATURES = {
     "oa_residual": (I32, [P, P, I64, I64, I64, I64, P, P, I64, P, I64, P, P, P, P, P, P, P, P, P]),
     "oa_residual_flash": (I32, [P, I64, P, P, I64, I64, I64, I64, P, P, I64, P, I64, P, P, P, P, P, P, P, P, P,
                                 I64, I32, F32, P, P]),
+    "oa_qk_norm_rope": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I32, I64, I64, I64,
+                              I64, P, P, I64, I64, P, I64, I32, I64, P, I64, I32, P, P, I32, F32, I32, I32, P]),
+    "oa_kv4_append": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64,
+                            I64, I64, I64, P, P, I64, I64, P, I64, I32, I64, P, I64, I32, P, P, I32, F32, I32, P]),
+    "oa_kv4_unpack": (I32, [P, I64, I64, I64, P, I64, I32, I64, P, I64, I32, P, I64, I64, I64, P, I64, I64, I64, I32, I64,
+                            I64, I64, I32, I32, P]),
+    "oa_kv4_attention_workspace_bytes": (SZ, [I64, I64, I64, I64, I64]),
+    "oa_kv4_attention": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I32, I64, P, I64, I64, I64, I32, I64, I64, I64,
+                               I64, F32, P, SZ, P]),
+    "oa_kv4_flash": (I32, [P, I64, P, I64, I64, P, I64, P, I64, P, P, I64, I64, I32, P, I64, P, I64, I32, I64, I64, I64,
+                           F32, P]),
     "oa_build_codes": (I32, [P, I64, I64, I64, P, P, P, P, P]),
     "oa_build_project_workspace_bytes": (SZ, [I64]),
     "oa_build_project": (I32, [P, I64, I64, I64, P, P, P, P, SZ, P]),
