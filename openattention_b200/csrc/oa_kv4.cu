@@ -5,7 +5,7 @@
 // kv4_attention: every position below the request's length; query token i of T (at position n - T + i) sees
 // positions <= n - T + i.  kv4_flash: index lists and cluster proxies (as OpenAttention.flash).  Rows with
 // nothing to attend give zeros.
-#include "oa_kv4.cuh"
+#include "oa_kv4_mma.cuh"
 
 #include "../../include/openattention_b200.h"
 
@@ -46,6 +46,14 @@ struct ListArgs {
   int G;
   float qk_scale;
 };
+
+__device__ __forceinline__ void store_out(const DenseArgs& a, int64_t b, int64_t h, int64_t t, int d, float v) {
+  const int64_t at = b * a.o.sb + h * a.o.sh + t * a.o.st + d;
+  if (a.out_f32)
+    static_cast<float*>(const_cast<void*>(a.o.p))[at] = v;
+  else
+    static_cast<__nv_bfloat16*>(const_cast<void*>(a.o.p))[at] = __float2bfloat16_rn(v);
+}
 
 // One half-warp's online softmax; lane hl holds dims 4hl..4hl+3 (i < 4) and 64 + 4hl.. (i >= 4).
 struct State {
@@ -110,23 +118,325 @@ __device__ __forceinline__ void merge_store(const State& s, int hw, int hl, void
     static_cast<__nv_bfloat16*>(out)[at + threadIdx.x] = __float2bfloat16_rn(o);
 }
 
-__global__ void __launch_bounds__(kThreads) dense_kernel(const DenseArgs a) {
-  const int lane = threadIdx.x & 31, hl = lane & 15, hw = threadIdx.x >> 4;
-  const unsigned hmask = 0xffffu << (lane & 16);
-  const int t = blockIdx.x % a.T;
-  const int h = (blockIdx.x / a.T) % a.HQ;
-  const int64_t b = blockIdx.x / a.T / a.HQ;
-  const int64_t n = min(per_request(a.n, b) + a.offset, a.Lmax) - a.T + 1 + t;
-  const unsigned char* base = a.cache + b * a.c_sb + (int64_t)(h / (a.HQ / a.HKV)) * a.c_sh;
-  State s;
-  s.init(static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + h * a.q.sh + t * a.q.st, hl);
-  for (int64_t j = hw; j < n; j += kHalfWarps) {
-    float k[8], v[8];
-    record_side(base + j * kRec, 0, hl, k);
-    record_side(base + j * kRec, 1, hl, v);
-    s.add(k, v, a.qk_scale, 0.f, hmask);
+// ---------------------------------------------------------------- dense
+// Work: a row is (request, KV head, block of up to 8 query columns); its tiles of 32 records are spread over
+// CTAs of 8 warps, each warp with its own ring of kStages tiles filled by asynchronous copies (the 4608 bytes
+// of a tile are contiguous).  Lengths live on the device, so each CTA finds its share itself:
+//  - each row its own CTAs, grid / rows of them (no more than one per 8 tiles), where that balances;
+//  - else the tiles of all rows in one line, cut into equal parts; a CTA then ends one row and begins the next.
+// A row that one CTA covers is written by it.  Otherwise each part leaves (m, l, O) in the workspace and the
+// last CTA to arrive (atomic ticket, no waiting) merges the parts in CTA order, so the result does not depend
+// on which CTA is last.
+constexpr int kWarps = 8;
+constexpr int kDenseThreads = 32 * kWarps;
+constexpr int kStages = 3;
+constexpr int kCols = 8;
+constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
+constexpr int kRingBytes = kWarps * kStages * kTileBytes;
+
+struct DensePlan {
+  int blocks;    // column blocks of a KV head: ceil(G T / 8)
+  int64_t rows;  // B * HKV * blocks
+  int grid;
+};
+
+DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax) {
+  DensePlan p;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) {
+    sms = 148;
+    (void)cudaGetLastError();  // a host without a GPU sizes for a B200
   }
-  merge_store(s, hw, hl, const_cast<void*>(a.o.p), b * a.o.sb + h * a.o.sh + t * a.o.st, a.out_f32);
+  p.blocks = (int)((HQ / HKV * T + kCols - 1) / kCols);
+  p.rows = B * HKV * p.blocks;
+  const int64_t tiles = (Lmax + kTile - 1) / kTile;
+  const int64_t parts = std::max<int64_t>(1, (tiles + kWarps - 1) / kWarps);
+  // two CTAs per SM (their rings fill its shared memory); no more than one per row and 8 tiles
+  p.grid = p.rows > 2 * sms ? 2 * sms : (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, p.rows * parts));
+  return p;
+}
+
+struct DenseWork {
+  int blocks;
+  int64_t rows;
+  float* parts;       // 2 per CTA: [0] of a row that began in an earlier CTA, [1] of one that begins here
+  unsigned* tickets;  // one per row, zero between calls
+};
+
+__device__ __forceinline__ int64_t dense_len(const DenseArgs& a, int64_t b) {
+  const int64_t n = min(per_request(a.n, b) + a.offset, a.Lmax);
+  return n < 0 ? 0 : n;
+}
+// a row without records still has its zeros to write: one (empty) tile
+__device__ __forceinline__ int64_t dense_tiles(int64_t n) { return n <= kTile ? 1 : (n + kTile - 1) / kTile; }
+
+// The parts of one row, part v at src (v = 0) or src + (2 v - 1) kPartFloats: weights 2^(m_v - M) in shared
+// memory first, then every thread sums four dims of one column over its share of the parts, eight loads in
+// flight; the shares are added in a fixed order.
+__device__ void merge_parts(const DenseArgs& a, const float* src, int parts, int ncol, float* sh, int64_t b, int64_t h0,
+                            int col0) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float* s_l = sh;                        // per column
+  float* s_f = sh + kCols;                // [part][column]
+  float* s_a = s_f + kCols * parts;       // [share][column][128]
+  for (int i = tid; i < parts * ncol; i += kDenseThreads) {
+    const int v = i / ncol, col = i - v * ncol;
+    s_f[v * kCols + col] = __ldcg(src + (v ? 2 * v - 1 : 0) * kPartFloats + kCols * kD + 2 * col);
+  }
+  __syncthreads();
+  if (warp < ncol) {  // one warp per column
+    float M = -INFINITY, L = 0.f;
+    for (int v = lane; v < parts; v += 32) M = fmaxf(M, s_f[v * kCols + warp]);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    M = biased(M);
+    for (int v = lane; v < parts; v += 32) {
+      const float f = ex2(s_f[v * kCols + warp] - M);
+      L = fmaf(f, __ldcg(src + (v ? 2 * v - 1 : 0) * kPartFloats + kCols * kD + 2 * warp + 1), L);
+      s_f[v * kCols + warp] = f;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) s_l[warp] = L;
+  }
+  __syncthreads();
+  const int quads = ncol * (kD / 4), shares = kDenseThreads / quads;  // ncol <= 8: at least one share
+  const int share = tid / quads, qd = tid - share * quads, col = qd / (kD / 4);
+  if (share < shares) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int v = share; v < parts; v += shares) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (v ? 2 * v - 1 : 0) * kPartFloats) + qd);
+      const float f = s_f[v * kCols + col];
+      acc.x = fmaf(f, x.x, acc.x);
+      acc.y = fmaf(f, x.y, acc.y);
+      acc.z = fmaf(f, x.z, acc.z);
+      acc.w = fmaf(f, x.w, acc.w);
+    }
+    reinterpret_cast<float4*>(s_a)[share * quads + qd] = acc;
+  }
+  __syncthreads();
+  for (int i = tid; i < ncol * kD; i += kDenseThreads) {
+    const int c = i / kD, d = i - c * kD, cc = col0 + c, hh = cc / a.T, tt = cc - hh * a.T;
+    float A = 0.f;
+    for (int v = 0; v < shares; ++v) A += s_a[v * ncol * kD + i];
+    const float L = s_l[c];
+    store_out(a, b, h0 + hh, tt, d, L == 0.f ? 0.f : A / L);
+  }
+}
+
+__global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
+  extern __shared__ __align__(16) unsigned char s_ring[];
+  __shared__ int64_t s_pre[kDenseThreads + 1];
+  __shared__ int64_t s_warp[kWarps], s_max[kWarps];
+  __shared__ unsigned s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int G = a.HQ / a.HKV, cols = G * a.T;
+  const int64_t per_req = (int64_t)a.HKV * w.blocks;
+  const int64_t grid = gridDim.x, cta = blockIdx.x;
+
+  // ---- this CTA's share: tiles of each request summed (thread i sums requests [i c, i c + c))
+  const int64_t c = (a.B + kDenseThreads - 1) / kDenseThreads;
+  int64_t sum = 0, most = 0;
+  for (int64_t b = tid * c; b < min((tid + 1) * c, (int64_t)a.B); ++b) {
+    const int64_t k = dense_tiles(dense_len(a, b));
+    sum += k;
+    most = max(most, k);
+  }
+  int64_t inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  if (lane == 0) s_max[warp] = most;
+  __syncthreads();
+  int64_t before = 0, req_tiles = 0;
+  most = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += s_warp[i];
+    req_tiles += s_warp[i];
+    most = max(most, s_max[i]);
+  }
+  s_pre[tid] = before + inc - sum;
+  if (tid == 0) s_pre[kDenseThreads] = req_tiles;
+  __syncthreads();
+  const int64_t total = req_tiles * per_req;
+  const int64_t cpr = grid / w.rows;  // CTAs a row can have to itself
+  const int64_t even = (total + grid - 1) / grid;
+  const bool aligned = cpr >= 1 && (most + cpr - 1) / cpr <= max((int64_t)kWarps, even + even / 8);
+  const int64_t active = min(grid, (total + kWarps - 1) / kWarps);  // of the line: at least 8 tiles each
+
+  int64_t b, r, tile, tiles, end;  // request, row within it, next tile, the row's tiles, end of the share (line)
+  int64_t n, share;                // length; tiles of this row that are this CTA's
+  int64_t parts;                   // CTAs that share the row
+  if (aligned) {
+    const int64_t row = cta / cpr, j = cta - row * cpr;
+    if (row >= w.rows) return;
+    b = row / per_req;
+    r = row - b * per_req;
+    n = dense_len(a, b);
+    tiles = dense_tiles(n);
+    parts = min(cpr, (tiles + kWarps - 1) / kWarps);
+    if (j >= parts) return;
+    tile = tiles * j / parts;
+    share = tiles * (j + 1) / parts - tile;
+    end = 0;
+  } else {
+    if (cta >= active) return;
+    const int64_t u = total * cta / active;
+    end = total * (cta + 1) / active;
+    if (u >= end) return;
+    const int64_t v = u / per_req;  // in units of one row of each request
+    int lo = 0, hi = kDenseThreads;  // the last thread whose requests begin at or before v
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_pre[mid] <= v) lo = mid; else hi = mid;
+    }
+    b = lo * c;
+    int64_t p = s_pre[lo];
+    n = dense_len(a, b);
+    tiles = dense_tiles(n);
+    while (p + tiles <= v) {
+      p += tiles;
+      n = dense_len(a, ++b);
+      tiles = dense_tiles(n);
+    }
+    const int64_t rem = u - p * per_req;
+    r = rem / tiles;
+    tile = rem - r * tiles;
+    end -= u;  // tiles left
+    share = min(tiles - tile, end);
+    parts = 0;
+  }
+
+  unsigned char* ring = s_ring + warp * (kStages * kTileBytes);
+  float* s_part = reinterpret_cast<float*>(s_ring);  // reused once a row's tiles are done
+  int64_t line = aligned ? 0 : total * cta / active;
+
+  for (;;) {
+    const int64_t kvh = r / w.blocks;
+    const int col0 = (int)(r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
+    const unsigned char* base = a.cache + b * a.c_sb + kvh * a.c_sh;
+    const int64_t t0 = tile + warp, t1 = tile + share;  // this warp: t0, t0 + 8, ...
+
+    auto fetch = [&](int64_t k, int slot) {
+      const unsigned char* src = base + k * kTileBytes;
+      const int64_t bytes = min((int64_t)kTileBytes, (n - k * kTile) * kRec);
+      unsigned char* dst = ring + slot * kTileBytes;
+#pragma unroll
+      for (int i = 0; i < kTileBytes / 512; ++i) {
+        const int at = 16 * (lane + 32 * i);
+        if (at < bytes) cp_async16(dst + at, src + at);
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+      if (t0 + s * kWarps < t1) fetch(t0 + s * kWarps, s);
+      cp_async_commit();
+    }
+    WarpAttention at;
+    {
+      const int col = col0 + g, hh = col / a.T, tt = col - hh * a.T;
+      const __nv_bfloat16* qp = nullptr;
+      if (g < ncol)
+        qp = static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + (kvh * G + hh) * a.q.sh + tt * a.q.st;
+      at.load_q(qp, a.qk_scale);
+    }
+    at.reset();
+    int64_t lim[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) lim[j] = n - a.T + 1 + (col0 + 2 * t + j) % a.T;
+    const int64_t whole = min(n, n - a.T + 1);  // tokens that every column sees
+    int slot = 0;
+    for (int64_t k = t0; k < t1; k += kWarps) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      const int64_t first = k * kTile;
+      if (first + kTile <= whole) {
+        const int none[2] = {kTile, kTile};
+        at.tile<false>(ring + slot * kTileBytes, 0, none);
+      } else {
+        const int l2[2] = {(int)max((int64_t)0, min((int64_t)kTile, lim[0] - first)),
+                           (int)max((int64_t)0, min((int64_t)kTile, lim[1] - first))};
+        at.tile<true>(ring + slot * kTileBytes, 0, l2);
+      }
+      __syncwarp();
+      const int64_t next = k + (kStages - 1) * kWarps;
+      if (next < t1) fetch(next, slot == 0 ? kStages - 1 : slot - 1);
+      cp_async_commit();
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+    }
+    cp_async_wait<0>();
+
+    // ---- merge the 8 warps
+    const bool begins = tile == 0, ends = tile + share == tiles;
+    __syncthreads();  // every warp is done with its ring
+    at.finish(s_part + warp * kPartFloats, s_part + warp * kPartFloats + kCols * kD, ncol);
+    __syncthreads();
+    float* part = w.parts + (2 * cta + (begins ? 1 : 0)) * (int64_t)kPartFloats;
+    for (int i = tid; i < ncol * kD; i += kDenseThreads) {
+      const int col = i / kD, d = i - col * kD;
+      float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) M = fmaxf(M, s_part[v * kPartFloats + kCols * kD + 2 * col]);
+      const float base_m = biased(M);
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const float* sp = s_part + v * kPartFloats;
+        const float f = ex2(sp[kCols * kD + 2 * col] - base_m);
+        L = fmaf(f, sp[kCols * kD + 2 * col + 1], L);
+        A = fmaf(f, sp[i], A);
+      }
+      if (begins && ends) {
+        const int cc = col0 + col, hh = cc / a.T, tt = cc - hh * a.T;
+        store_out(a, b, kvh * G + hh, tt, d, L == 0.f ? 0.f : A / L);
+      } else {
+        part[i] = A;
+        if (d == 0) {
+          part[kCols * kD + 2 * col] = M;
+          part[kCols * kD + 2 * col + 1] = L;
+        }
+      }
+    }
+    if (!(begins && ends)) {
+      // who shares this row: `parts` CTAs from `first` on; the first of them keeps its part in slot 1
+      int64_t first = cta;
+      if (aligned) {
+        first = ((b * per_req + r) * cpr);
+      } else {
+        const int64_t u0 = line - tile, u1 = u0 + tiles - 1;  // the row's first and last tile on the line
+        first = ((u0 + 1) * active + total - 1) / total - 1;
+        parts = ((u1 + 1) * active + total - 1) / total - first;
+      }
+      unsigned* ticket = w.tickets + b * per_req + r;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(ticket, 1u) == (unsigned)(parts - 1) ? 1u : 0u;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        merge_parts(a, w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part, b, kvh * G, col0);
+        if (tid == 0) *ticket = 0u;
+      }
+    }
+    if (aligned) return;
+    line += share;
+    end -= share;
+    if (end <= 0) return;
+    __syncthreads();  // s_part is the ring again
+    tile = 0;
+    if (++r == per_req) {
+      r = 0;
+      n = dense_len(a, ++b);
+      tiles = dense_tiles(n);
+    }
+    share = min(tiles, end);
+  }
 }
 
 __global__ void __launch_bounds__(kThreads) list_kernel(const ListArgs a) {
@@ -161,6 +471,8 @@ __global__ void __launch_bounds__(kThreads) list_kernel(const ListArgs a) {
   merge_store(s, hw, hl, a.out, r * a.out_stride, a.out_f32);
 }
 
+size_t ticket_bytes(int64_t rows) { return ((size_t)rows * sizeof(unsigned) + 255) & ~size_t(255); }
+
 bool rows_ok(const Rows& r, int esize) {
   const int64_t q = 16 / esize;
   return oa_aligned16(r.p) && r.sb % q == 0 && r.sh % q == 0 && r.st % q == 0;
@@ -170,7 +482,9 @@ bool rows_ok(const Rows& r, int esize) {
 }  // namespace oa
 
 extern "C" size_t oa_kv4_attention_workspace_bytes(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax) {
-  return 0;
+  if (B <= 0 || T <= 0 || HKV <= 0 || HQ < HKV || Lmax < 0) return 0;
+  const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
+  return oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
 }
 
 extern "C" int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* cache,
@@ -202,7 +516,18 @@ extern "C" int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64
   a.out_f32 = out_dtype == OA_F32;
   a.B = (int)B; a.HQ = (int)HQ; a.HKV = (int)HKV; a.T = (int)T;
   a.qk_scale = sm_scale * oa::kLog2e;
-  oa::dense_kernel<<<(unsigned)(B * HQ * T), oa::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
+  const size_t need = oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
+  OA_REQUIRE(workspace && workspace_bytes >= need && oa_aligned16(workspace),
+             "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, workspace_bytes);
+  oa::DenseWork w;
+  w.blocks = p.blocks;
+  w.rows = p.rows;
+  w.tickets = static_cast<unsigned*>(workspace);
+  w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + oa::ticket_bytes(p.rows));
+  const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(&oa::dense_kernel), oa::kRingBytes, fn, true);
+  if (rc != OA_OK) return rc;
+  oa::dense_kernel<<<(unsigned)p.grid, oa::kDenseThreads, oa::kRingBytes, static_cast<cudaStream_t>(stream)>>>(a, w);
   return oa_check_launch(fn);
 }
 
