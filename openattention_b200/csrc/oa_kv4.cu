@@ -131,6 +131,7 @@ constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kCols = 8;
+constexpr int kRowUnits = 12;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
 constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
 constexpr int kRingBytes = kWarps * kStages * kTileBytes;
 
@@ -164,12 +165,12 @@ struct DenseWork {
   unsigned* tickets;  // one per row, zero between calls
 };
 
-__device__ __forceinline__ int64_t dense_len(const DenseArgs& a, int64_t b) {
+__device__ __forceinline__ int dense_len(const DenseArgs& a, int64_t b) {
   const int64_t n = min(per_request(a.n, b) + a.offset, a.Lmax);
-  return n < 0 ? 0 : n;
+  return n < 0 ? 0 : (int)n;
 }
 // a row without records still has its zeros to write: one (empty) tile
-__device__ __forceinline__ int64_t dense_tiles(int64_t n) { return n <= kTile ? 1 : (n + kTile - 1) / kTile; }
+__device__ __forceinline__ int dense_tiles(int n) { return n <= kTile ? 1 : (int)(((unsigned)n + kTile - 1) / kTile); }
 
 // The parts of one row, part v at src (v = 0) or src + (2 v - 1) kPartFloats: weights 2^(m_v - M) in shared
 // memory first, then every thread sums four dims of one column over its share of the parts, eight loads in
@@ -226,155 +227,208 @@ __device__ void merge_parts(const DenseArgs& a, const float* src, int parts, int
   }
 }
 
-__global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
-  extern __shared__ __align__(16) unsigned char s_ring[];
-  __shared__ int64_t s_pre[kDenseThreads + 1];
-  __shared__ int64_t s_warp[kWarps], s_max[kWarps];
-  __shared__ unsigned s_last;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int G = a.HQ / a.HKV, cols = G * a.T;
-  const int64_t per_req = (int64_t)a.HKV * w.blocks;
-  const int64_t grid = gridDim.x, cta = blockIdx.x;
+// A CTA's way along the line of rows: the row it is at and its tiles of that row.
+struct DenseShare {
+  int64_t b, r;     // request, row within it
+  int n, tiles;     // the request's length, a row's tiles
+  int tile, share;  // first tile and number of tiles of this CTA's part
+  int64_t line;     // where the part begins on the line (units); -1: the row's CTAs are its own
+  int64_t left;     // units of this CTA's share from there on
+  int64_t total, active;
+  int parts;        // CTAs that share the row, from `first` on (line: found when needed)
+  int64_t first;
+};
 
-  // ---- this CTA's share: tiles of each request summed (thread i sums requests [i c, i c + c))
-  const int64_t c = (a.B + kDenseThreads - 1) / kDenseThreads;
-  int64_t sum = 0, most = 0;
-  for (int64_t b = tid * c; b < min((tid + 1) * c, (int64_t)a.B); ++b) {
-    const int64_t k = dense_tiles(dense_len(a, b));
-    sum += k;
-    most = max(most, k);
-  }
-  int64_t inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  }
-  if (lane == 31) s_warp[warp] = inc;
-  if (lane == 0) s_max[warp] = most;
-  __syncthreads();
-  int64_t before = 0, req_tiles = 0;
-  most = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += s_warp[i];
-    req_tiles += s_warp[i];
-    most = max(most, s_max[i]);
-  }
-  s_pre[tid] = before + inc - sum;
-  if (tid == 0) s_pre[kDenseThreads] = req_tiles;
-  __syncthreads();
-  const int64_t total = req_tiles * per_req;
-  const int64_t cpr = grid / w.rows;  // CTAs a row can have to itself
-  const int64_t even = (total + grid - 1) / grid;
-  const bool aligned = cpr >= 1 && (most + cpr - 1) / cpr <= max((int64_t)kWarps, even + even / 8);
-  const int64_t active = min(grid, (total + kWarps - 1) / kWarps);  // of the line: at least 8 tiles each
-
-  int64_t b, r, tile, tiles, end;  // request, row within it, next tile, the row's tiles, end of the share (line)
-  int64_t n, share;                // length; tiles of this row that are this CTA's
-  int64_t parts;                   // CTAs that share the row
-  if (aligned) {
-    const int64_t row = cta / cpr, j = cta - row * cpr;
-    if (row >= w.rows) return;
-    b = row / per_req;
-    r = row - b * per_req;
-    n = dense_len(a, b);
-    tiles = dense_tiles(n);
-    parts = min(cpr, (tiles + kWarps - 1) / kWarps);
-    if (j >= parts) return;
-    tile = tiles * j / parts;
-    share = tiles * (j + 1) / parts - tile;
-    end = 0;
+// False: nothing for this CTA.  Every thread of the CTA finds the same.
+__device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
+  __shared__ int64_t s_pre[kDenseThreads + 1];  // units of a row of each request before thread i's requests
+  __shared__ int64_t s_sum[kWarps];
+  __shared__ int s_most[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t per_req = (int64_t)a.HKV * w.blocks, grid = gridDim.x, cta = blockIdx.x;
+  const int64_t c = (a.B + kDenseThreads - 1) / kDenseThreads;  // requests a thread sums
+  const bool same = a.n.stride == 0;
+  int64_t units;
+  int most;
+  if (same) {
+    s.n = dense_len(a, 0);
+    most = dense_tiles(s.n);
+    units = a.B * (int64_t)(most + kRowUnits);
   } else {
-    if (cta >= active) return;
-    const int64_t u = total * cta / active;
-    end = total * (cta + 1) / active;
-    if (u >= end) return;
-    const int64_t v = u / per_req;  // in units of one row of each request
+    int64_t sum = 0;
+    most = 0;
+    for (int64_t b = tid * c; b < min((tid + 1) * c, (int64_t)a.B); ++b) {
+      const int k = dense_tiles(dense_len(a, b));
+      sum += k + kRowUnits;
+      most = max(most, k);
+    }
+    int64_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    if (lane == 0) s_most[warp] = most;
+    __syncthreads();
+    int64_t before = 0;
+    units = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += s_sum[i];
+      units += s_sum[i];
+      most = max(most, s_most[i]);
+    }
+    s_pre[tid] = before + inc - sum;
+    __syncthreads();
+  }
+  s.total = units * per_req;
+  const int64_t cpr = grid / w.rows;  // CTAs a row can have to itself
+  const int64_t even = (s.total + grid - 1) / grid;
+  if (cpr >= 1 && kRowUnits + (most + cpr - 1) / cpr <= max((int64_t)(kRowUnits + kWarps), even + even / 8)) {
+    const int64_t row = cta / cpr, j = cta - row * cpr;
+    if (row >= w.rows) return false;
+    s.b = row / per_req;
+    s.r = row - s.b * per_req;
+    if (!same) s.n = dense_len(a, s.b);
+    s.tiles = dense_tiles(s.n);
+    s.parts = (int)min(cpr, (int64_t)(s.tiles + kWarps - 1) / kWarps);
+    if (j >= s.parts) return false;
+    s.tile = (int)((int64_t)s.tiles * j / s.parts);
+    s.share = (int)((int64_t)s.tiles * (j + 1) / s.parts) - s.tile;
+    s.first = cta - j;
+    s.line = -1;
+    s.left = 0;
+    return true;
+  }
+  s.active = min(grid, (s.total + kRowUnits + kWarps - 1) / (kRowUnits + kWarps));
+  if (cta >= s.active) return false;
+  s.line = s.total * cta / s.active;
+  s.left = s.total * (cta + 1) / s.active - s.line;
+  const int64_t v = s.line / per_req;
+  int64_t p;
+  if (same) {
+    s.tiles = most;
+    s.b = v / (most + kRowUnits);
+    p = s.b * (most + kRowUnits);
+  } else {
     int lo = 0, hi = kDenseThreads;  // the last thread whose requests begin at or before v
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_pre[mid] <= v) lo = mid; else hi = mid;
     }
-    b = lo * c;
-    int64_t p = s_pre[lo];
-    n = dense_len(a, b);
-    tiles = dense_tiles(n);
-    while (p + tiles <= v) {
-      p += tiles;
-      n = dense_len(a, ++b);
-      tiles = dense_tiles(n);
+    s.b = lo * c;
+    p = s_pre[lo];
+    s.n = dense_len(a, s.b);
+    s.tiles = dense_tiles(s.n);
+    while (p + s.tiles + kRowUnits <= v) {
+      p += s.tiles + kRowUnits;
+      s.n = dense_len(a, ++s.b);
+      s.tiles = dense_tiles(s.n);
     }
-    const int64_t rem = u - p * per_req;
-    r = rem / tiles;
-    tile = rem - r * tiles;
-    end -= u;  // tiles left
-    share = min(tiles - tile, end);
-    parts = 0;
   }
+  const int64_t rem = s.line - p * per_req;
+  s.r = rem / (s.tiles + kRowUnits);
+  const int off = (int)(rem - s.r * (s.tiles + kRowUnits));
+  s.tile = max(0, off - kRowUnits);
+  s.share = (int)min((int64_t)s.tiles, off + s.left - kRowUnits) - s.tile;
+  s.parts = off;  // units of the row before this part, until dense_next
+  return true;
+}
 
-  unsigned char* ring = s_ring + warp * (kStages * kTileBytes);
+// The next row on the line, if any of its units are left to this CTA.
+__device__ __forceinline__ bool dense_next(const DenseArgs& a, int64_t per_req, DenseShare& s) {
+  if (s.line < 0) return false;
+  const int64_t step = s.tiles + kRowUnits - s.parts;
+  s.line += step;
+  s.left -= step;
+  if (s.left <= kRowUnits) return false;  // not one tile
+  if (++s.r == per_req) {
+    s.r = 0;
+    ++s.b;
+    if (a.n.stride) {
+      s.n = dense_len(a, s.b);
+      s.tiles = dense_tiles(s.n);
+    }
+  }
+  s.tile = 0;
+  s.parts = 0;
+  s.share = (int)min((int64_t)s.tiles, s.left - kRowUnits);
+  return true;
+}
+
+__global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
+  extern __shared__ __align__(16) unsigned char s_ring[];
+  __shared__ unsigned s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = a.HQ / a.HKV, cols = G * a.T;
+  const int64_t per_req = (int64_t)a.HKV * w.blocks, cta = blockIdx.x;
+  DenseShare s;
+  if (!dense_share(a, w, s)) return;
+
+  const uint32_t ring = smem_u32(s_ring) + warp * (kStages * kTileBytes);
   float* s_part = reinterpret_cast<float*>(s_ring);  // reused once a row's tiles are done
-  int64_t line = aligned ? 0 : total * cta / active;
+  WarpAttention at;
+  at.lane_addresses();
 
-  for (;;) {
-    const int64_t kvh = r / w.blocks;
-    const int col0 = (int)(r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
-    const unsigned char* base = a.cache + b * a.c_sb + kvh * a.c_sh;
-    const int64_t t0 = tile + warp, t1 = tile + share;  // this warp: t0, t0 + 8, ...
+  do {
+    if (s.share <= 0) continue;  // the share ends before the row's first tile
+    const int kvh = (int)(s.r / w.blocks);
+    const int col0 = (int)(s.r - (int64_t)kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
+    const int t0 = s.tile + warp, t1 = s.tile + s.share;  // this warp: t0, t0 + 8, ...
+    const unsigned char* src = a.cache + s.b * a.c_sb + kvh * a.c_sh + (int64_t)t0 * kTileBytes + 16 * lane;
 
-    auto fetch = [&](int64_t k, int slot) {
-      const unsigned char* src = base + k * kTileBytes;
-      const int64_t bytes = min((int64_t)kTileBytes, (n - k * kTile) * kRec);
-      unsigned char* dst = ring + slot * kTileBytes;
+    auto fetch = [&](int k, uint32_t slot) {  // tile k, `src` at it
+      const uint32_t dst = ring + slot * kTileBytes + 16 * lane;
+      const int records = s.n - k * kTile;
+      if (records >= kTile) {
 #pragma unroll
-      for (int i = 0; i < kTileBytes / 512; ++i) {
-        const int at = 16 * (lane + 32 * i);
-        if (at < bytes) cp_async16(dst + at, src + at);
+        for (int i = 0; i < kTileBytes / 512; ++i) cp_async16(dst + 512 * i, src + 512 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTileBytes / 512; ++i)
+          if (16 * lane + 512 * i < records * kRec) cp_async16(dst + 512 * i, src + 512 * i);
       }
+      src += (int64_t)kWarps * kTileBytes;
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      if (t0 + s * kWarps < t1) fetch(t0 + s * kWarps, s);
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (t0 + i * kWarps < t1) fetch(t0 + i * kWarps, i);
       cp_async_commit();
     }
-    WarpAttention at;
     {
-      const int col = col0 + g, hh = col / a.T, tt = col - hh * a.T;
+      const int g = lane >> 2, col = col0 + g, hh = col / a.T, tt = col - hh * a.T;
       const __nv_bfloat16* qp = nullptr;
       if (g < ncol)
-        qp = static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + (kvh * G + hh) * a.q.sh + tt * a.q.st;
+        qp = static_cast<const __nv_bfloat16*>(a.q.p) + s.b * a.q.sb + (int64_t)(kvh * G + hh) * a.q.sh + tt * a.q.st;
       at.load_q(qp, a.qk_scale);
     }
     at.reset();
-    int64_t lim[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) lim[j] = n - a.T + 1 + (col0 + 2 * t + j) % a.T;
-    const int64_t whole = min(n, n - a.T + 1);  // tokens that every column sees
-    int slot = 0;
-    for (int64_t k = t0; k < t1; k += kWarps) {
+    const int whole = s.n - a.T + 1;  // tokens that every column sees
+    uint32_t slot = 0;
+    for (int k = t0; k < t1; k += kWarps) {
       cp_async_wait<kStages - 2>();
       __syncwarp();
-      const int64_t first = k * kTile;
-      if (first + kTile <= whole) {
+      if ((k + 1) * kTile <= whole) {
         const int none[2] = {kTile, kTile};
-        at.tile<false>(ring + slot * kTileBytes, 0, none);
+        at.tile<false>(ring + slot * kTileBytes, none);
       } else {
-        const int l2[2] = {(int)max((int64_t)0, min((int64_t)kTile, lim[0] - first)),
-                           (int)max((int64_t)0, min((int64_t)kTile, lim[1] - first))};
-        at.tile<true>(ring + slot * kTileBytes, 0, l2);
+        int lim[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          lim[j] = max(0, min(kTile, whole + (col0 + 2 * (lane & 3) + j) % a.T - k * kTile));
+        at.tile<true>(ring + slot * kTileBytes, lim);
       }
       __syncwarp();
-      const int64_t next = k + (kStages - 1) * kWarps;
-      if (next < t1) fetch(next, slot == 0 ? kStages - 1 : slot - 1);
+      if (k + (kStages - 1) * kWarps < t1) fetch(k + (kStages - 1) * kWarps, slot == 0 ? kStages - 1 : slot - 1);
       cp_async_commit();
       slot = slot + 1 == kStages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
 
     // ---- merge the 8 warps
-    const bool begins = tile == 0, ends = tile + share == tiles;
+    const bool begins = s.tile == 0, alone = begins && s.share == s.tiles;
     __syncthreads();  // every warp is done with its ring
     at.finish(s_part + warp * kPartFloats, s_part + warp * kPartFloats + kCols * kD, ncol);
     __syncthreads();
@@ -392,9 +446,9 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
         L = fmaf(f, sp[kCols * kD + 2 * col + 1], L);
         A = fmaf(f, sp[i], A);
       }
-      if (begins && ends) {
+      if (alone) {
         const int cc = col0 + col, hh = cc / a.T, tt = cc - hh * a.T;
-        store_out(a, b, kvh * G + hh, tt, d, L == 0.f ? 0.f : A / L);
+        store_out(a, s.b, kvh * G + hh, tt, d, L == 0.f ? 0.f : A / L);
       } else {
         part[i] = A;
         if (d == 0) {
@@ -403,40 +457,27 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
         }
       }
     }
-    if (!(begins && ends)) {
-      // who shares this row: `parts` CTAs from `first` on; the first of them keeps its part in slot 1
-      int64_t first = cta;
-      if (aligned) {
-        first = ((b * per_req + r) * cpr);
-      } else {
-        const int64_t u0 = line - tile, u1 = u0 + tiles - 1;  // the row's first and last tile on the line
-        first = ((u0 + 1) * active + total - 1) / total - 1;
-        parts = ((u1 + 1) * active + total - 1) / total - first;
+    if (!alone) {
+      int64_t first = s.first;
+      int parts = s.parts;
+      if (s.line >= 0) {  // the CTAs of the row's first and last tile
+        const int64_t u0 = s.line - s.parts + kRowUnits, u1 = u0 + s.tiles - 1;
+        first = ((u0 + 1) * s.active + s.total - 1) / s.total - 1;
+        parts = (int)(((u1 + 1) * s.active + s.total - 1) / s.total - first);
       }
-      unsigned* ticket = w.tickets + b * per_req + r;
+      unsigned* ticket = w.tickets + s.b * per_req + s.r;
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicAdd(ticket, 1u) == (unsigned)(parts - 1) ? 1u : 0u;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        merge_parts(a, w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part, b, kvh * G, col0);
+        merge_parts(a, w.parts + (2 * first + 1) * (int64_t)kPartFloats, parts, ncol, s_part, s.b, kvh * G, col0);
         if (tid == 0) *ticket = 0u;
       }
     }
-    if (aligned) return;
-    line += share;
-    end -= share;
-    if (end <= 0) return;
     __syncthreads();  // s_part is the ring again
-    tile = 0;
-    if (++r == per_req) {
-      r = 0;
-      n = dense_len(a, ++b);
-      tiles = dense_tiles(n);
-    }
-    share = min(tiles, end);
-  }
+  } while (dense_next(a, per_req, s));
 }
 
 __global__ void __launch_bounds__(kThreads) list_kernel(const ListArgs a) {
@@ -496,7 +537,7 @@ extern "C" int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64
   OA_REQUIRE(B >= 0 && T >= 0 && HKV >= 1 && HQ >= HKV && HQ % HKV == 0,
              "%s: need B, T >= 0 and HQ a multiple of HKV (B=%lld T=%lld HQ=%lld HKV=%lld)", fn, (long long)B,
              (long long)T, (long long)HQ, (long long)HKV);
-  OA_REQUIRE(B * HQ * T <= 0x7fffffff, "%s: too many rows", fn);
+  OA_REQUIRE(B <= 0x7fffffff && T <= 0x7fffffff && HQ <= 0x7fffffff && HQ * T <= 0x7fffffff / std::max<int64_t>(B, 1) && Lmax <= 0x7fffffff - 64, "%s: too many rows or positions", fn);
   OA_REQUIRE(out_dtype == OA_BF16 || out_dtype == OA_F32, "%s: out_dtype must be OA_BF16 or OA_F32", fn);
   OA_REQUIRE((cache || Lmax == 0) && oa_aligned16(cache) && c_sb % 16 == 0 && c_sh % 16 == 0 && Lmax >= 0,
              "%s: the cache and its strides must be multiples of 16 bytes", fn);

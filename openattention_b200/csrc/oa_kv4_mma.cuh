@@ -54,6 +54,19 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, results under 2^-126 ar
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ float biased(float m) { return m == -INFINITY ? 0.f : m; }
 
+// shared-space loads
+__device__ __forceinline__ uint4 lds128(uint32_t at, int imm) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at + imm));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at, int imm) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at + imm));
+  return v;
+}
+__device__ __forceinline__ uint32_t shr8(uint32_t x) { return x >> 8; }
+
 // Token (0..15 of a 16-token block) of MMA row r (0..7); row r + 8 holds the next token.
 __device__ __forceinline__ int row_token(int r) { return (r & 1) ? 8 + ((r + 3) & 7) : r; }
 
@@ -62,7 +75,7 @@ struct WarpAttention {
   float scale[2];            // per column (2t, 2t + 1): sm_scale log2(e) 2^(24 - exponent of q)
   float q0[2], q1[2];        // sm_scale log2(e) times the sum of q over each half
   float acc[8][4];           // O^T: half h, tile i -> acc[4 h + i]
-  float m[2], l[2];          // running maximum (log2 units), this lane's share of the sum
+  float m[2], bm[2], l[2];   // running maximum (log2 units; bm: 0 while it is -inf), this lane's share of the sum
   float z0[2], z1[2];        // this lane's share of sum p z, per half
   float r0, r1, cap0, cap1;  // power-of-two factors of p s per half, and the largest scale they hold
 
@@ -118,7 +131,7 @@ struct WarpAttention {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       m[j] = -INFINITY;
-      l[j] = z0[j] = z1[j] = 0.f;
+      bm[j] = l[j] = z0[j] = z1[j] = 0.f;
     }
     r0 = r1 = pow2i(126);
     cap0 = cap1 = pow2i(15 - 126);
@@ -142,49 +155,63 @@ struct WarpAttention {
     cap = pow2i(15) / next;
   }
 
-  // One tile of 32 records in shared memory; the first is token `base`.  MASK: column 2t + j sees only the
-  // tokens below lim[j]; what masked records hold (stale bytes, NaN scales) does not enter.
+  // This lane's addresses in a tile (shared-space bytes from the tile's start).
+  uint32_t at_k, at_m, at_v0, at_v1;
+  __device__ __forceinline__ void lane_addresses() {
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t tok = row_token(g);
+    at_k = tok * kRec + 16 * t;                                // K codes of MMA row g; row g + 8 is the next record
+    at_m = tok * kRec + kRecMeta;
+    at_v0 = 2 * t * kRec + kRecV + 8 * g;                      // V dims 8g .. 8g + 7 (and + 64) of MMA row 2t
+    at_v1 = (8 + ((2 * t + 4) & 7)) * kRec + kRecV + 8 * g;    // and of row 2t + 1
+  }
+
+  // One tile of 32 records at shared address `sm`.  MASK: column 2t + j sees only the tokens below lim[j] of the
+  // tile; what masked records hold (stale bytes, NaN scales) does not enter.
   template <bool MASK>
-  __device__ __forceinline__ void tile(const unsigned char* sm, int base, const int (&lim)[2]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int tok = row_token(g);
+  __device__ __forceinline__ void tile(uint32_t sm, const int (&lim)[2]) {
+    const int tok = MASK ? row_token((threadIdx.x & 31) >> 2) : 0;
     float x[2][4];
     uint2 vm[2][2];  // value scales and offsets of this lane's four tokens
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const unsigned char* pa = sm + (16 * b + tok) * kRec;
-      const unsigned char* pb = pa + kRec;
-      const uint4 ka = *reinterpret_cast<const uint4*>(pa + 16 * t);
-      const uint4 kb = *reinterpret_cast<const uint4*>(pb + 16 * t);
-      const uint4 ma = *reinterpret_cast<const uint4*>(pa + kRecMeta);
-      const uint4 mb = *reinterpret_cast<const uint4*>(pb + kRecMeta);
+      const uint4 ka = lds128(sm + at_k, 16 * b * kRec), kb = lds128(sm + at_k, (16 * b + 1) * kRec);
+      const uint4 ma = lds128(sm + at_m, 16 * b * kRec), mb = lds128(sm + at_m, (16 * b + 1) * kRec);
       float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a = wa[i], c = wb[i], a8 = a >> 8, c8 = c >> 8;
+        const uint32_t a = wa[i], c = wb[i], a8 = shr8(a), c8 = shr8(c);
         mma_f16(c0, a & kLoMask, c & kLoMask, a8 & kLoMask, c8 & kLoMask, qf[2 * i], qf[2 * i + 1]);
         mma_f16(c1, a & kHiMask, c & kHiMask, a8 & kHiMask, c8 & kHiMask, qf[8 + 2 * i], qf[8 + 2 * i + 1]);
       }
       vm[b][0] = make_uint2(ma.z, ma.w);
       vm[b][1] = make_uint2(mb.z, mb.w);
+      const float sa0 = bf_lo(ma.x), za0 = bf_hi(ma.x), sa1 = bf_lo(ma.y), za1 = bf_hi(ma.y);
+      const float sb0 = bf_lo(mb.x), zb0 = bf_hi(mb.x), sb1 = bf_lo(mb.y), zb1 = bf_hi(mb.y);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float ya = fmaf(bf_lo(ma.y), c1[j], bf_lo(ma.x) * c0[j]);
-        const float yb = fmaf(bf_lo(mb.y), c1[2 + j], bf_lo(mb.x) * c0[2 + j]);
-        x[b][j] = fmaf(ya, scale[j], fmaf(bf_hi(ma.y), q1[j], bf_hi(ma.x) * q0[j]));
-        x[b][2 + j] = fmaf(yb, scale[j], fmaf(bf_hi(mb.y), q1[j], bf_hi(mb.x) * q0[j]));
+        x[b][j] = fmaf(fmaf(sa1, c1[j], sa0 * c0[j]), scale[j], fmaf(za1, q1[j], za0 * q0[j]));
+        x[b][2 + j] = fmaf(fmaf(sb1, c1[2 + j], sb0 * c0[2 + j]), scale[j], fmaf(zb1, q1[j], zb0 * q0[j]));
         if (MASK) {
-          if (base + 16 * b + tok >= lim[j]) x[b][j] = -INFINITY;
-          if (base + 16 * b + tok + 1 >= lim[j]) x[b][2 + j] = -INFINITY;
+          if (16 * b + tok >= lim[j]) x[b][j] = -INFINITY;
+          if (16 * b + tok + 1 >= lim[j]) x[b][2 + j] = -INFINITY;
         }
       }
     }
-    // m is the same in all lanes of a column, so nothing moves until some lane sees a larger score
-    float mx[2];
+    // m is the same in all lanes of a column, so nothing moves until some lane sees a larger score (or scale)
+    float mx[2], s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; ++j) mx[j] = fmaxf(fmaxf(x[0][j], x[0][2 + j]), fmaxf(x[1][j], x[1][2 + j]));
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const bool in = !MASK || 16 * b + tok + k < max(lim[0], lim[1]);
+        s0 = fmaxf(s0, in ? bf_lo(vm[b][k].x) : 0.f);
+        s1 = fmaxf(s1, in ? bf_lo(vm[b][k].y) : 0.f);
+      }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || s0 > cap0 || s1 > cap1)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -192,6 +219,7 @@ struct WarpAttention {
         const float nm = fmaxf(m[j], mx[j]);
         const float al = ex2(m[j] - biased(nm));
         m[j] = nm;
+        bm[j] = biased(nm);
         l[j] *= al;
         z0[j] *= al;
         z1[j] *= al;
@@ -201,34 +229,22 @@ struct WarpAttention {
           acc[i][2 + j] *= al;
         }
       }
-    }
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const bool in = !MASK || base + 16 * b + tok + k < max(lim[0], lim[1]);
-        s0 = fmaxf(s0, in ? bf_lo(vm[b][k].x) : 0.f);
-        s1 = fmaxf(s1, in ? bf_lo(vm[b][k].y) : 0.f);
-      }
-    if (__any_sync(0xffffffffu, s0 > cap0 || s1 > cap1)) {
       raise_cap(s0, r0, cap0, 0);
       raise_cap(s1, r1, cap1, 1);
     }
-    const float b0m = biased(m[0]), b1m = biased(m[1]);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       uint32_t pl[2], ph[2];  // weights of the two halves, turned: tokens of rows 0..7, of rows 8..15
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float p0 = ex2(x[b][2 * k] - b0m), p1 = ex2(x[b][2 * k + 1] - b1m);
+        const float p0 = ex2(x[b][2 * k] - bm[0]), p1 = ex2(x[b][2 * k + 1] - bm[1]);
         l[0] += p0;
         l[1] += p1;
         const float sa = bf_lo(vm[b][k].x) * r0, za = bf_hi(vm[b][k].x);
         const float sb = bf_lo(vm[b][k].y) * r1, zb = bf_hi(vm[b][k].y);
         float wa0 = p0 * sa, wa1 = p1 * sa, wb0 = p0 * sb, wb1 = p1 * sb;
         if (MASK) {
-          const int tk = base + 16 * b + tok + k;
+          const int tk = 16 * b + tok + k;
           const bool in0 = tk < lim[0], in1 = tk < lim[1];
           wa0 = in0 ? wa0 : 0.f;
           wb0 = in0 ? wb0 : 0.f;
@@ -247,17 +263,14 @@ struct WarpAttention {
         pl[k] = transpose8x8(pack_half2(wa0, wa1));
         ph[k] = transpose8x8(pack_half2(wb0, wb1));
       }
-      // the tokens of MMA rows 2t, 2t + 1 (and the next ones, rows 2t + 8, 2t + 9), dims 8g .. 8g + 7 and + 64
-      const unsigned char* v0 = sm + (16 * b + 2 * t) * kRec + kRecV + 8 * g;
-      const unsigned char* v1 = sm + (16 * b + 8 + ((2 * t + 4) & 7)) * kRec + kRecV + 8 * g;
-      const uint2 a0 = *reinterpret_cast<const uint2*>(v0), a1 = *reinterpret_cast<const uint2*>(v1);
-      const uint2 n0 = *reinterpret_cast<const uint2*>(v0 + kRec), n1 = *reinterpret_cast<const uint2*>(v1 + kRec);
+      const uint2 a0 = lds64(sm + at_v0, 16 * b * kRec), a1 = lds64(sm + at_v1, 16 * b * kRec);
+      const uint2 n0 = lds64(sm + at_v0, (16 * b + 1) * kRec), n1 = lds64(sm + at_v1, (16 * b + 1) * kRec);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
         const uint32_t u = __byte_perm(i < 2 ? a0.x : a0.y, i < 2 ? a1.x : a1.y, sel);
         const uint32_t w = __byte_perm(i < 2 ? n0.x : n0.y, i < 2 ? n1.x : n1.y, sel);
-        const uint32_t u8 = u >> 8, w8 = w >> 8;
+        const uint32_t u8 = shr8(u), w8 = shr8(w);
         mma_f16(acc[i], u & kLoMask, u8 & kLoMask, w & kLoMask, w8 & kLoMask, pl[0], pl[1]);
         mma_f16(acc[4 + i], u & kHiMask, u8 & kHiMask, w & kHiMask, w8 & kHiMask, ph[0], ph[1]);
       }
