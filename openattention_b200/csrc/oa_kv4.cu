@@ -47,14 +47,6 @@ struct ListArgs {
   float qk_scale;
 };
 
-__device__ __forceinline__ void store_out(const DenseArgs& a, int64_t b, int64_t h, int64_t t, int d, float v) {
-  const int64_t at = b * a.o.sb + h * a.o.sh + t * a.o.st + d;
-  if (a.out_f32)
-    static_cast<float*>(const_cast<void*>(a.o.p))[at] = v;
-  else
-    static_cast<__nv_bfloat16*>(const_cast<void*>(a.o.p))[at] = __float2bfloat16_rn(v);
-}
-
 // One half-warp's online softmax; lane hl holds dims 4hl..4hl+3 (i < 4) and 64 + 4hl.. (i >= 4).
 struct State {
   float q[8], acc[8], m, l;
@@ -159,10 +151,10 @@ DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax
 }
 
 struct DenseWork {
-  int blocks;
-  int64_t rows;
-  float* parts;       // 2 per CTA: [0] of a row that began in an earlier CTA, [1] of one that begins here
-  unsigned* tickets;  // one per row, zero between calls
+  unsigned blocks, per_req, rows;  // column blocks of a KV head; rows of a request; rows
+  unsigned cpr;                    // CTAs a row can have to itself: grid / rows
+  float* parts;                    // 2 per CTA: [0] of a row that began in an earlier CTA, [1] of one that begins here
+  unsigned* tickets;               // one per row, zero between calls
 };
 
 __device__ __forceinline__ int dense_len(const DenseArgs& a, int64_t b) {
@@ -172,29 +164,59 @@ __device__ __forceinline__ int dense_len(const DenseArgs& a, int64_t b) {
 // a row without records still has its zeros to write: one (empty) tile
 __device__ __forceinline__ int dense_tiles(int n) { return n <= kTile ? 1 : (int)(((unsigned)n + kTile - 1) / kTile); }
 
-// The parts of one row, part v at src (v = 0) or src + (2 v - 1) kPartFloats: weights 2^(m_v - M) in shared
-// memory first, then every thread sums four dims of one column over its share of the parts, eight loads in
-// flight; the shares are added in a fixed order.
-__device__ void merge_parts(const DenseArgs& a, const float* src, int parts, int ncol, float* sh, int64_t b, int64_t h0,
-                            int col0) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  float* s_l = sh;                        // per column
-  float* s_f = sh + kCols;                // [part][column]
-  float* s_a = s_f + kCols * parts;       // [share][column][128]
-  for (int i = tid; i < parts * ncol; i += kDenseThreads) {
-    const int v = i / ncol, col = i - v * ncol;
-    s_f[v * kCols + col] = __ldcg(src + (v ? 2 * v - 1 : 0) * kPartFloats + kCols * kD + 2 * col);
+__device__ __forceinline__ void axpy(float4& y, float f, const float4& x) {
+  y.x = fmaf(f, x.x, y.x);
+  y.y = fmaf(f, x.y, y.y);
+  y.z = fmaf(f, x.z, y.z);
+  y.w = fmaf(f, x.w, y.w);
+}
+// dims 4 lane .. 4 lane + 3 of the output row at element `at`
+__device__ __forceinline__ void store_out4(void* out, int out_f32, int64_t at, int lane, const float4& A, float L) {
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float4 o = L == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+  if (out_f32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at + 4 * lane) = o;
+  } else {
+    uint2 w;
+    w.x = (uint32_t)f2bf_bits(o.x) | ((uint32_t)f2bf_bits(o.y) << 16);
+    w.y = (uint32_t)f2bf_bits(o.z) | ((uint32_t)f2bf_bits(o.w) << 16);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + at + 4 * lane) = w;
   }
-  __syncthreads();
-  if (warp < ncol) {  // one warp per column
+}
+
+// The parts of one row, part v at src (v = 0) or src + (2 v - 1) kPartFloats.  Every thread sums four dims of one
+// column over its share of the parts, kAhead loads in flight; the first ones are issued before the weights
+// 2^(m_v - M) are known.  The shares are added in a fixed order.  o_at: the output row of column `warp`.
+// Inlined, and kAhead no larger: a call, or more loads held, spills the caller's main loop.
+template <int kAhead>
+__device__ __forceinline__ void merge_parts(const float* src, int parts, int ncol, float* sh, void* out, int out_f32,
+                                         int64_t o_at) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float* s_l = sh;                   // per column
+  float* s_f = sh + kCols;           // [part][column]
+  float* s_a = s_f + kCols * parts;  // [share][column][128]
+  const int quads = ncol * (kD / 4), shares = kDenseThreads / quads;  // ncol <= 8: at least one share
+  const int share = tid / quads, qd = tid - share * quads, col = qd / (kD / 4);
+  auto at = [&](int v) { return src + (v ? 2 * v - 1 : 0) * (int64_t)kPartFloats; };
+  float4 x[kAhead];
+  if (share < shares) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (share + i * shares < parts) x[i] = __ldcg(reinterpret_cast<const float4*>(at(share + i * shares)) + qd);
+  }
+  if (warp < ncol) {  // the weights of column `warp`
     float M = -INFINITY, L = 0.f;
-    for (int v = lane; v < parts; v += 32) M = fmaxf(M, s_f[v * kCols + warp]);
+    for (int v = lane; v < parts; v += 32) {
+      const float m = __ldcg(at(v) + kCols * kD + 2 * warp);
+      s_f[v * kCols + warp] = m;
+      M = fmaxf(M, m);
+    }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     M = biased(M);
     for (int v = lane; v < parts; v += 32) {
       const float f = ex2(s_f[v * kCols + warp] - M);
-      L = fmaf(f, __ldcg(src + (v ? 2 * v - 1 : 0) * kPartFloats + kCols * kD + 2 * warp + 1), L);
+      L = fmaf(f, __ldcg(at(v) + kCols * kD + 2 * warp + 1), L);
       s_f[v * kCols + warp] = f;
     }
 #pragma unroll
@@ -202,80 +224,84 @@ __device__ void merge_parts(const DenseArgs& a, const float* src, int parts, int
     if (lane == 0) s_l[warp] = L;
   }
   __syncthreads();
-  const int quads = ncol * (kD / 4), shares = kDenseThreads / quads;  // ncol <= 8: at least one share
-  const int share = tid / quads, qd = tid - share * quads, col = qd / (kD / 4);
   if (share < shares) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int v = share; v < parts; v += shares) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (v ? 2 * v - 1 : 0) * kPartFloats) + qd);
-      const float f = s_f[v * kCols + col];
-      acc.x = fmaf(f, x.x, acc.x);
-      acc.y = fmaf(f, x.y, acc.y);
-      acc.z = fmaf(f, x.z, acc.z);
-      acc.w = fmaf(f, x.w, acc.w);
+    for (int v = share; v < parts;) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i, v += shares)
+        if (v < parts) axpy(acc, s_f[v * kCols + col], x[i]);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i * shares < parts) x[i] = __ldcg(reinterpret_cast<const float4*>(at(v + i * shares)) + qd);
     }
     reinterpret_cast<float4*>(s_a)[share * quads + qd] = acc;
   }
   __syncthreads();
-  for (int i = tid; i < ncol * kD; i += kDenseThreads) {
-    const int c = i / kD, d = i - c * kD, cc = col0 + c, hh = cc / a.T, tt = cc - hh * a.T;
-    float A = 0.f;
-    for (int v = 0; v < shares; ++v) A += s_a[v * ncol * kD + i];
-    const float L = s_l[c];
-    store_out(a, b, h0 + hh, tt, d, L == 0.f ? 0.f : A / L);
+  if (warp < ncol) {
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int v = 0; v < shares; ++v) axpy(A, 1.f, reinterpret_cast<const float4*>(s_a)[v * quads + 32 * warp + lane]);
+    store_out4(out, out_f32, o_at, lane, A, s_l[warp]);
   }
 }
 
-// A CTA's way along the line of rows: the row it is at and its tiles of that row.
+// A CTA's way along the line of rows: the row it is at and its tiles of that row.  Counts of units fit 31 bits
+// (checked by the host).
 struct DenseShare {
-  int64_t b, r;     // request, row within it
-  int n, tiles;     // the request's length, a row's tiles
-  int tile, share;  // first tile and number of tiles of this CTA's part
-  int64_t line;     // where the part begins on the line (units); -1: the row's CTAs are its own
-  int64_t left;     // units of this CTA's share from there on
-  int64_t total, active;
-  int parts;        // CTAs that share the row, from `first` on (line: found when needed)
-  int64_t first;
+  unsigned b, r;          // request, row within it
+  int n, tiles;           // the request's length, a row's tiles
+  int tile, share;        // first tile and number of tiles of this CTA's part
+  bool own;               // the row's CTAs serve no other row
+  unsigned line;          // where the part begins on the line (units)
+  int left, off;          // units of this CTA's share from there on; units of the row before the part
+  unsigned each, extra;   // the line's cut: `extra` CTAs take each + 1 units, the others `each`
+  unsigned first, parts;  // own: the row's CTAs
 };
+// the CTA that unit u belongs to, and where a CTA's units begin
+__device__ __forceinline__ unsigned cta_of(const DenseShare& s, unsigned u) {
+  const unsigned big = s.extra * (s.each + 1);
+  return u < big ? u / (s.each + 1) : s.extra + (u - big) / s.each;
+}
+__device__ __forceinline__ unsigned cta_begin(const DenseShare& s, unsigned cta) {
+  return cta * s.each + min(cta, s.extra);
+}
 
 // False: nothing for this CTA.  Every thread of the CTA finds the same.
 __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
-  __shared__ int64_t s_pre[kDenseThreads + 1];  // units of a row of each request before thread i's requests
-  __shared__ int64_t s_sum[kWarps];
+  __shared__ unsigned s_pre[kDenseThreads];  // units of a row of each request before thread i's requests
+  __shared__ unsigned s_sum[kWarps];
   __shared__ int s_most[kWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t per_req = (int64_t)a.HKV * w.blocks, grid = gridDim.x, cta = blockIdx.x;
-  const int64_t c = (a.B + kDenseThreads - 1) / kDenseThreads;  // requests a thread sums
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned grid = gridDim.x, cta = blockIdx.x;
+  const unsigned c = ((unsigned)a.B + kDenseThreads - 1) / kDenseThreads;  // requests a thread sums
   const bool same = a.n.stride == 0;
-  int64_t units;
+  unsigned units;
   int most;
   if (same) {
     s.n = dense_len(a, 0);
     most = dense_tiles(s.n);
-    units = a.B * (int64_t)(most + kRowUnits);
+    units = a.B * (unsigned)(most + kRowUnits);
   } else {
-    int64_t sum = 0;
+    unsigned sum = 0;
     most = 0;
-    for (int64_t b = tid * c; b < min((tid + 1) * c, (int64_t)a.B); ++b) {
+    for (unsigned b = tid * c; b < min((tid + 1) * c, (unsigned)a.B); ++b) {
       const int k = dense_tiles(dense_len(a, b));
       sum += k + kRowUnits;
       most = max(most, k);
     }
-    int64_t inc = sum;
+    unsigned inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
+    most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 31) s_sum[warp] = inc;
     if (lane == 0) s_most[warp] = most;
     __syncthreads();
-    int64_t before = 0;
+    unsigned before = 0;
     units = 0;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
+    for (unsigned i = 0; i < kWarps; ++i) {
       if (i < warp) before += s_sum[i];
       units += s_sum[i];
       most = max(most, s_most[i]);
@@ -283,39 +309,39 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
     s_pre[tid] = before + inc - sum;
     __syncthreads();
   }
-  s.total = units * per_req;
-  const int64_t cpr = grid / w.rows;  // CTAs a row can have to itself
-  const int64_t even = (s.total + grid - 1) / grid;
-  if (cpr >= 1 && kRowUnits + (most + cpr - 1) / cpr <= max((int64_t)(kRowUnits + kWarps), even + even / 8)) {
-    const int64_t row = cta / cpr, j = cta - row * cpr;
+  const unsigned total = units * w.per_req;
+  s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * (8u * grid) <= max((kRowUnits + kWarps) * 8u * grid, 9u * total);
+  if (s.own) {
+    const unsigned row = cta / w.cpr, j = cta - row * w.cpr;
     if (row >= w.rows) return false;
-    s.b = row / per_req;
-    s.r = row - s.b * per_req;
+    s.b = row / w.per_req;
+    s.r = row - s.b * w.per_req;
     if (!same) s.n = dense_len(a, s.b);
     s.tiles = dense_tiles(s.n);
-    s.parts = (int)min(cpr, (int64_t)(s.tiles + kWarps - 1) / kWarps);
+    s.parts = min(w.cpr, (unsigned)(s.tiles + kWarps - 1) / kWarps);
     if (j >= s.parts) return false;
-    s.tile = (int)((int64_t)s.tiles * j / s.parts);
-    s.share = (int)((int64_t)s.tiles * (j + 1) / s.parts) - s.tile;
+    const unsigned each = s.tiles / s.parts, extra = s.tiles - each * s.parts;
+    s.tile = j * each + min(j, extra);
+    s.share = each + (j < extra ? 1 : 0);
     s.first = cta - j;
-    s.line = -1;
-    s.left = 0;
     return true;
   }
-  s.active = min(grid, (s.total + kRowUnits + kWarps - 1) / (kRowUnits + kWarps));
-  if (cta >= s.active) return false;
-  s.line = s.total * cta / s.active;
-  s.left = s.total * (cta + 1) / s.active - s.line;
-  const int64_t v = s.line / per_req;
-  int64_t p;
+  const unsigned active = min(grid, (total + kRowUnits + kWarps - 1) / (kRowUnits + kWarps));
+  if (cta >= active) return false;
+  s.each = total / active;
+  s.extra = total - s.each * active;
+  s.line = cta_begin(s, cta);
+  s.left = s.each + (cta < s.extra ? 1 : 0);
+  const unsigned v = s.line / w.per_req;
+  unsigned p;
   if (same) {
     s.tiles = most;
     s.b = v / (most + kRowUnits);
     p = s.b * (most + kRowUnits);
   } else {
-    int lo = 0, hi = kDenseThreads;  // the last thread whose requests begin at or before v
+    unsigned lo = 0, hi = kDenseThreads;  // the last thread whose requests begin at or before v
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
+      const unsigned mid = (lo + hi) >> 1;
       if (s_pre[mid] <= v) lo = mid; else hi = mid;
     }
     s.b = lo * c;
@@ -328,23 +354,21 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
       s.tiles = dense_tiles(s.n);
     }
   }
-  const int64_t rem = s.line - p * per_req;
+  const unsigned rem = s.line - p * w.per_req;
   s.r = rem / (s.tiles + kRowUnits);
-  const int off = (int)(rem - s.r * (s.tiles + kRowUnits));
-  s.tile = max(0, off - kRowUnits);
-  s.share = (int)min((int64_t)s.tiles, off + s.left - kRowUnits) - s.tile;
-  s.parts = off;  // units of the row before this part, until dense_next
+  s.off = rem - s.r * (s.tiles + kRowUnits);
+  s.tile = max(0, s.off - kRowUnits);
+  s.share = min(s.tiles, s.off + s.left - kRowUnits) - s.tile;
   return true;
 }
 
-// The next row on the line, if any of its units are left to this CTA.
-__device__ __forceinline__ bool dense_next(const DenseArgs& a, int64_t per_req, DenseShare& s) {
-  if (s.line < 0) return false;
-  const int64_t step = s.tiles + kRowUnits - s.parts;
+// The next row on the line, if any of its tiles are this CTA's.
+__device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
+  const int step = s.tiles + kRowUnits - s.off;
   s.line += step;
   s.left -= step;
-  if (s.left <= kRowUnits) return false;  // not one tile
-  if (++s.r == per_req) {
+  if (s.left <= kRowUnits) return false;
+  if (++s.r == w.per_req) {
     s.r = 0;
     ++s.b;
     if (a.n.stride) {
@@ -353,35 +377,51 @@ __device__ __forceinline__ bool dense_next(const DenseArgs& a, int64_t per_req, 
     }
   }
   s.tile = 0;
-  s.parts = 0;
-  s.share = (int)min((int64_t)s.tiles, s.left - kRowUnits);
+  s.off = 0;
+  s.share = min(s.tiles, s.left - kRowUnits);
   return true;
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
   extern __shared__ __align__(16) unsigned char s_ring[];
   __shared__ unsigned s_last;
+  __shared__ DenseShare s;  // the same for all threads: kept here, out of the loop's registers
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.HQ / a.HKV, cols = G * a.T;
-  const int64_t per_req = (int64_t)a.HKV * w.blocks, cta = blockIdx.x;
-  DenseShare s;
-  if (!dense_share(a, w, s)) return;
+  const unsigned cta = blockIdx.x;
+  {
+    DenseShare mine;
+    if (!dense_share(a, w, mine)) return;
+    if (tid == 0) s = mine;
+  }
+  __syncthreads();
 
   const uint32_t ring = smem_u32(s_ring) + warp * (kStages * kTileBytes);
   float* s_part = reinterpret_cast<float*>(s_ring);  // reused once a row's tiles are done
-  WarpAttention at;
+  WarpAttention<PAIR> at;
   at.lane_addresses();
 
-  do {
-    if (s.share <= 0) continue;  // the share ends before the row's first tile
-    const int kvh = (int)(s.r / w.blocks);
-    const int col0 = (int)(s.r - (int64_t)kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
-    const int t0 = s.tile + warp, t1 = s.tile + s.share;  // this warp: t0, t0 + 8, ...
+  for (;;) {
+    if (s.share <= 0) return;  // the share ends before the row's first tile
+    const int kvh = s.r / w.blocks;
+    const int col0 = (s.r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
+    // the query row of column c: head h0 + (col0 + c) / T, query token (col0 + c) % T
+    const int64_t q_at = s.b * a.q.sb + (int64_t)(kvh * G) * a.q.sh;
+    auto split = [&](int c, int& hh, int& tt) {
+      hh = a.T == 1 ? col0 + c : (col0 + c) / a.T;
+      tt = col0 + c - hh * a.T;
+    };
+    {
+      int hh, tt;
+      split(at.op_col(), hh, tt);
+      at.load_q(at.op_col() < ncol ? static_cast<const __nv_bfloat16*>(a.q.p) + q_at + hh * a.q.sh + tt * a.q.st : nullptr);
+    }
+    const int t0 = s.tile + warp, t1 = s.tile + s.share, n = s.n;  // this warp: t0, t0 + 8, ...
     const unsigned char* src = a.cache + s.b * a.c_sb + kvh * a.c_sh + (int64_t)t0 * kTileBytes + 16 * lane;
-
     auto fetch = [&](int k, uint32_t slot) {  // tile k, `src` at it
       const uint32_t dst = ring + slot * kTileBytes + 16 * lane;
-      const int records = s.n - k * kTile;
+      const int records = n - k * kTile;
       if (records >= kTile) {
 #pragma unroll
         for (int i = 0; i < kTileBytes / 512; ++i) cp_async16(dst + 512 * i, src + 512 * i);
@@ -397,28 +437,25 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
       if (t0 + i * kWarps < t1) fetch(t0 + i * kWarps, i);
       cp_async_commit();
     }
-    {
-      const int g = lane >> 2, col = col0 + g, hh = col / a.T, tt = col - hh * a.T;
-      const __nv_bfloat16* qp = nullptr;
-      if (g < ncol)
-        qp = static_cast<const __nv_bfloat16*>(a.q.p) + s.b * a.q.sb + (int64_t)(kvh * G + hh) * a.q.sh + tt * a.q.st;
-      at.load_q(qp, a.qk_scale);
+    at.begin(a.qk_scale);
+    const int whole = n - a.T + 1;  // tokens that every column sees
+    int sees[2];                      // tokens that the lane's columns see
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      int hh, tt;
+      split(at.acc_col(j), hh, tt);
+      sees[j] = whole + tt;
     }
-    at.reset();
-    const int whole = s.n - a.T + 1;  // tokens that every column sees
     uint32_t slot = 0;
     for (int k = t0; k < t1; k += kWarps) {
       cp_async_wait<kStages - 2>();
       __syncwarp();
       if ((k + 1) * kTile <= whole) {
         const int none[2] = {kTile, kTile};
-        at.tile<false>(ring + slot * kTileBytes, none);
+        at.template tile<false>(ring + slot * kTileBytes, none);
       } else {
-        int lim[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          lim[j] = max(0, min(kTile, whole + (col0 + 2 * (lane & 3) + j) % a.T - k * kTile));
-        at.tile<true>(ring + slot * kTileBytes, lim);
+        const int lim[2] = {max(0, min(kTile, sees[0] - k * kTile)), max(0, min(kTile, sees[1] - k * kTile))};
+        at.template tile<true>(ring + slot * kTileBytes, lim);
       }
       __syncwarp();
       if (k + (kStages - 1) * kWarps < t1) fetch(k + (kStages - 1) * kWarps, slot == 0 ? kStages - 1 : slot - 1);
@@ -427,57 +464,62 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
     }
     cp_async_wait<0>();
 
-    // ---- merge the 8 warps
+    // ---- merge the 8 warps: warp c takes column c, a lane four dims
     const bool begins = s.tile == 0, alone = begins && s.share == s.tiles;
     __syncthreads();  // every warp is done with its ring
     at.finish(s_part + warp * kPartFloats, s_part + warp * kPartFloats + kCols * kD, ncol);
     __syncthreads();
-    float* part = w.parts + (2 * cta + (begins ? 1 : 0)) * (int64_t)kPartFloats;
-    for (int i = tid; i < ncol * kD; i += kDenseThreads) {
-      const int col = i / kD, d = i - col * kD;
-      float M = -INFINITY, L = 0.f, A = 0.f;
-#pragma unroll
-      for (int v = 0; v < kWarps; ++v) M = fmaxf(M, s_part[v * kPartFloats + kCols * kD + 2 * col]);
-      const float base_m = biased(M);
+    int hh, tt;
+    split(warp, hh, tt);
+    const int64_t o_at = s.b * a.o.sb + (int64_t)(kvh * G + hh) * a.o.sh + tt * a.o.st;
+    if (warp < ncol) {
+      float f[kWarps], M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) {
-        const float* sp = s_part + v * kPartFloats;
-        const float f = ex2(sp[kCols * kD + 2 * col] - base_m);
-        L = fmaf(f, sp[kCols * kD + 2 * col + 1], L);
-        A = fmaf(f, sp[i], A);
+        f[v] = s_part[v * kPartFloats + kCols * kD + 2 * warp];
+        M = fmaxf(M, f[v]);
+      }
+      const float base_m = biased(M);
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const float e = ex2(f[v] - base_m);
+        L = fmaf(e, s_part[v * kPartFloats + kCols * kD + 2 * warp + 1], L);
+        axpy(A, e, reinterpret_cast<const float4*>(s_part + v * kPartFloats)[32 * warp + lane]);
       }
       if (alone) {
-        const int cc = col0 + col, hh = cc / a.T, tt = cc - hh * a.T;
-        store_out(a, s.b, kvh * G + hh, tt, d, L == 0.f ? 0.f : A / L);
+        store_out4(const_cast<void*>(a.o.p), a.out_f32, o_at, lane, A, L);
       } else {
-        part[i] = A;
-        if (d == 0) {
-          part[kCols * kD + 2 * col] = M;
-          part[kCols * kD + 2 * col + 1] = L;
-        }
+        float* part = w.parts + (2 * cta + (begins ? 1 : 0)) * (int64_t)kPartFloats;
+        reinterpret_cast<float4*>(part)[32 * warp + lane] = A;
+        if (lane == 0) *reinterpret_cast<float2*>(part + kCols * kD + 2 * warp) = make_float2(M, L);
       }
     }
     if (!alone) {
-      int64_t first = s.first;
-      int parts = s.parts;
-      if (s.line >= 0) {  // the CTAs of the row's first and last tile
-        const int64_t u0 = s.line - s.parts + kRowUnits, u1 = u0 + s.tiles - 1;
-        first = ((u0 + 1) * s.active + s.total - 1) / s.total - 1;
-        parts = (int)(((u1 + 1) * s.active + s.total - 1) / s.total - first);
+      unsigned first = s.first, parts = s.parts;
+      if (!s.own) {  // the CTAs of the row's first and last tile
+        const unsigned u = s.line - s.off + kRowUnits;
+        first = cta_of(s, u);
+        parts = cta_of(s, u + s.tiles - 1) - first + 1;
       }
-      unsigned* ticket = w.tickets + s.b * per_req + s.r;
+      unsigned* ticket = w.tickets + s.b * w.per_req + s.r;
       __threadfence();
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(ticket, 1u) == (unsigned)(parts - 1) ? 1u : 0u;
+      if (tid == 0) s_last = atomicAdd(ticket, 1u) == parts - 1 ? 1u : 0u;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        merge_parts(a, w.parts + (2 * first + 1) * (int64_t)kPartFloats, parts, ncol, s_part, s.b, kvh * G, col0);
+        merge_parts<PAIR ? 6 : 4>(w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part,
+                                  const_cast<void*>(a.o.p), a.out_f32, o_at);
         if (tid == 0) *ticket = 0u;
       }
     }
+    if (s.own) return;
+    __syncthreads();
+    if (tid == 0) s_last = dense_next(a, w, s) ? 1u : 0u;
     __syncthreads();  // s_part is the ring again
-  } while (dense_next(a, per_req, s));
+    if (!s_last) return;
+  }
 }
 
 __global__ void __launch_bounds__(kThreads) list_kernel(const ListArgs a) {
@@ -558,17 +600,24 @@ extern "C" int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64
   a.B = (int)B; a.HQ = (int)HQ; a.HKV = (int)HKV; a.T = (int)T;
   a.qk_scale = sm_scale * oa::kLog2e;
   const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
+  // units on the line (and 9 of them per row of the grid's widest product) are counted in 32 bits
+  const int64_t most_units = p.rows * ((Lmax + oa::kTile - 1) / oa::kTile + 1 + oa::kRowUnits);
+  OA_REQUIRE(most_units <= 0xffffffffll / 9 && most_units / std::max<int64_t>(p.rows, 1) * 8 * p.grid <= 0xffffffffll,
+             "%s: too many records (B * HKV * Lmax) for one call", fn);
   const size_t need = oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
   OA_REQUIRE(workspace && workspace_bytes >= need && oa_aligned16(workspace),
              "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, workspace_bytes);
   oa::DenseWork w;
   w.blocks = p.blocks;
-  w.rows = p.rows;
+  w.per_req = (unsigned)(HKV * p.blocks);
+  w.rows = (unsigned)p.rows;
+  w.cpr = (unsigned)(p.grid / p.rows);
   w.tickets = static_cast<unsigned*>(workspace);
   w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + oa::ticket_bytes(p.rows));
-  const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(&oa::dense_kernel), oa::kRingBytes, fn, true);
+  const auto kernel = HQ / HKV * T <= 4 ? &oa::dense_kernel<true> : &oa::dense_kernel<false>;
+  const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(kernel), oa::kRingBytes, fn, true);
   if (rc != OA_OK) return rc;
-  oa::dense_kernel<<<(unsigned)p.grid, oa::kDenseThreads, oa::kRingBytes, static_cast<cudaStream_t>(stream)>>>(a, w);
+  kernel<<<(unsigned)p.grid, oa::kDenseThreads, oa::kRingBytes, static_cast<cudaStream_t>(stream)>>>(a, w);
   return oa_check_launch(fn);
 }
 
