@@ -10,8 +10,9 @@
 // Codes cost one AND each pair: a nibble left in place in a 16-bit word is an fp16 subnormal, code * 2^-24 (low
 // nibble) or 16 * code * 2^-24 (high nibble), exact.  Low and high nibbles are the two halves, so the factor 16
 // belongs to a whole half.  q is scaled by a power of two per column (largest element in [2^13, 2^14)), exact
-// unless an element is 2^-37 of the largest; p s by a power of two per half, raised so that the largest scale
-// seen gives [2^14, 2^15): p s is rounded to fp16 (11 bits) over 28 octaves below the largest.
+// unless an element is 2^-37 of the largest; p s by a power of two per half, chosen so that the largest scale
+// seen gives [2^6, 2^7): p s is rounded to fp16 (11 bits) over 20 octaves below the largest, beneath them it is
+// off by 2^-32 of the largest.
 //
 // Layout.  Scores are computed transposed, S^T = codes (16 tokens) x q (8 columns), so that columns lie along
 // the accumulator's lanes the same way as in O^T = V^T (16 dims) x P (8 columns): running maxima and sums need
@@ -27,6 +28,8 @@ namespace oa {
 
 constexpr int kTile = 32;                   // records per tile
 constexpr int kTileBytes = kTile * kRec;
+constexpr float kSlack = 8.f;  // log2
+constexpr int kTop = 7;        // scales times r stay at most 2^kTop, weights at most 2^(kTop + kSlack) < fp16's 65504
 constexpr uint32_t kLoMask = 0x000f000fu, kHiMask = 0x00f000f0u;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -175,7 +178,7 @@ struct WarpAttention {
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       r[h] = pow2i(126);
-      cap[h] = pow2i(15 - 126);
+      cap[h] = pow2i(kTop - 126);
     }
   }
 
@@ -184,8 +187,8 @@ struct WarpAttention {
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
     if (!(s > cap[h])) return;
-    const int es = max(-112, (__float_as_int(s) >> 23) - 127);
-    const float next = pow2i(14 - es);
+    const int es = max(kTop - 127, (__float_as_int(s) >> 23) - 127);
+    const float next = pow2i(kTop - 1 - es);
     // next / r as a power of two; one under 2^-126 drops what is there, which is that much smaller
     const int d = (__float_as_int(next) >> 23) - (__float_as_int(r[h]) >> 23);
     const float f = d < -126 ? 0.f : pow2i(d);
@@ -194,7 +197,7 @@ struct WarpAttention {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[4 * h + i][j] *= f;
     r[h] = next;
-    cap[h] = pow2i(15) / next;
+    cap[h] = pow2i(kTop) / next;
   }
 
   // One tile of 32 records at shared address `sm`.  MASK: the lane's accumulator column j sees only the tokens
@@ -251,7 +254,8 @@ struct WarpAttention {
           x[b][2 * k + j] = v;
         }
     }
-    // m is the same in all lanes of a column, so nothing moves until some lane sees a larger score (or scale)
+    // m is the same in all lanes of a column and nothing moves until some lane sees a score kSlack above it (or
+    // a scale above the cap): weights up to 2^kSlack are as good as weights up to 1, and new maxima are common
     float mx[2], s[kHalves];
 #pragma unroll
     for (int j = 0; j < 2; ++j) mx[j] = fmaxf(fmaxf(x[0][j], x[0][2 + j]), fmaxf(x[1][j], x[1][2 + j]));
@@ -264,7 +268,7 @@ struct WarpAttention {
         s[h] = fmaxf(s[h], in ? bf_lo(vm[i >> 1][i & 1][h]) : 0.f);
       }
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || s[0] > cap[0] || s[kHalves - 1] > cap[kHalves - 1])) {
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack || s[0] > cap[0] || s[kHalves - 1] > cap[kHalves - 1])) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
