@@ -285,73 +285,109 @@ int oa_cluster_sums(const void* K, const void* V, int64_t hkv, int64_t Lmax, int
 /* ------------------------------------------------------------------------------------------------
  * Rows on their way into attention, and the 4-bit K/V cache.  No counterpart in the reference.
  *
- * Rows: (B, heads, T, 128), strides (_sb request, _sh head, _st token) in elements, contiguous last dim, base
- * and strides on 16-byte boundaries.  Row i of request b stands at position p = start[b] + offset + i.
- * Per-request arrays (start, lens, n): device int32 (or int64 where the _i64 flag is 1), element b * stride
- * (stride 0: one number for all).  lens (may be NULL: T rows each): rows i >= lens[b] are padding.
+ * These entries take their arguments in one block of 8-byte fields (a decode loop that crosses a foreign-function
+ * boundary per call pays for each argument there).  An oa_tensor is an address with sizes and strides in elements;
+ * the entries check sizes against each other, that last dims are contiguous and that rows start on 16-byte
+ * boundaries (base and strides; the stride of a dim of one element is ignored).
  *
- * Cache: (B, HKV, Lmax, 144) bytes, c_sb / c_sh the request and head strides in bytes (multiples of 16).  A
- * record of 144 bytes holds one token of one KV head:
+ * Row i of request b stands at position p = start[b] + offset + i.  Per-request numbers (oa_index: start, lens, n)
+ * are device int32 or int64, one for each request or one for all.  lens (p NULL: all T rows): rows i >= lens[b] are
+ * padding.
+ *
+ * Cache: (B, HKV, Lmax, 144) bytes, records contiguous.  A record of 144 bytes holds one token of one KV head:
  *   bytes   0.. 63  K codes: byte j = code of dim j | code of dim j + 64 << 4;  bytes 64..127  V codes
  *   bytes 128..143  bf16 scale, offset of K dims 0..63, of K dims 64..127, of V dims 0..63, of V dims 64..127
  * value = scale * code + offset; offset = the group's minimum, scale = bf16((max - min) / 15), code =
  * min(rint((x - offset) / scale), 15) (0 where the scale is 0); a group with an infinity or a NaN, or a range
  * past fp32's, gets scale NaN.
  * ----------------------------------------------------------------------------------------------*/
+typedef struct {
+  const void* p;
+  int64_t size[4], stride[4];
+} oa_tensor4;
+typedef struct {
+  const void* p;
+  int64_t size[3], stride[3];
+} oa_tensor3;
+typedef struct {
+  const void* p;
+  int64_t size[2], stride[2];
+} oa_tensor2;
+typedef struct {
+  const void* p;                     /* NULL: absent */
+  int64_t size, stride, is_int64;
+} oa_index;
 
-/* Optional per-head RMS norm of q (HQ heads) and k (HKV heads), then the position rotation, in one pass:
+/* Optional per-head RMS norm of q (B, HQ, T, 128) and k (B, HKV, T, 128), then the position rotation, in one pass:
  *   y = x * rsqrt(mean(x^2) + eps) * w   (fp32; where q_weight / k_weight (128,) is not NULL; type w_dtype)
  *   out[d] = y[d] * cos[p, d] + rot(y)[d] * sin[p, d] for d < R (products and sum rounded apart in fp32), y[d] for
  *   d >= R; rot(y) = [-y[R/2 .. R), y[0 .. R/2)]; rounded once to the rows' dtype (OA_BF16 or OA_F32).
  * cos, sin (P, R) fp32 contiguous, R a multiple of 16 up to 128.  Positions outside [0, P) are padding.  Padding
  * rows of an output become zero where zero_q / zero_k is 1 and keep their contents where it is 0.  An output may
  * be its input. */
-int oa_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb,
-                    int64_t k_sh, int64_t k_st, void* q_out, int64_t qo_sb, int64_t qo_sh, int64_t qo_st, void* k_out,
-                    int64_t ko_sb, int64_t ko_sh, int64_t ko_st, int dtype, int64_t B, int64_t T, int64_t HQ,
-                    int64_t HKV, const float* cos, const float* sin, int64_t P, int64_t R, const void* start,
-                    int64_t start_stride, int start_i64, int64_t offset, const void* lens, int64_t lens_stride,
-                    int lens_i64, const void* q_weight, const void* k_weight, int w_dtype, float eps, int zero_q,
-                    int zero_k, void* stream);
+typedef struct {
+  oa_tensor4 q, k, q_out, k_out;
+  const float *cos, *sin;
+  int64_t P, R;
+  oa_index start, lens;
+  const void *q_weight, *k_weight;
+  int64_t offset, dtype, w_dtype, zero_q, zero_k;
+  double eps;
+} oa_qk_norm_rope_args;
+int oa_qk_norm_rope(const oa_qk_norm_rope_args* args, void* stream);
 
-/* Writes k, v (bf16 rows) into the cache at their positions; positions outside [0, Lmax) and padding rows write
- * nothing.  With cos / sin (else HQ = 0 and both NULL), q and k first go through oa_qk_norm_rope's arithmetic
- * (k rounded to bf16 before it is quantised) and q is written to q_out, in the same launch. */
-int oa_kv4_append(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb, int64_t k_sh,
-                  int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st, void* q_out, int64_t qo_sb,
-                  int64_t qo_sh, int64_t qo_st, void* cache, int64_t c_sb, int64_t c_sh, int64_t Lmax, int64_t B,
-                  int64_t T, int64_t HQ, int64_t HKV, const float* cos, const float* sin, int64_t P, int64_t R,
-                  const void* start, int64_t start_stride, int start_i64, int64_t offset, const void* lens,
-                  int64_t lens_stride, int lens_i64, const void* q_weight, const void* k_weight, int w_dtype, float eps,
-                  int zero_q, void* stream);
+/* Writes k, v (B, HKV, T, 128) bf16 into the cache at their positions; positions outside [0, Lmax) and padding rows
+ * write nothing.  With cos and sin, q and k first go through oa_qk_norm_rope's arithmetic (k rounded to bf16 before
+ * it is quantised) and q is written to q_out, in the same launch; without them (NULL) q and q_out are absent. */
+typedef struct {
+  oa_tensor4 q, k, v, q_out, cache;
+  const float *cos, *sin;
+  int64_t P, R;
+  oa_index start, lens;
+  const void *q_weight, *k_weight;
+  int64_t offset, w_dtype, zero_q;
+  double eps;
+} oa_kv4_append_args;
+int oa_kv4_append(const oa_kv4_append_args* args, void* stream);
 
-/* The values of records back as rows (dtype OA_BF16 or OA_F32); padding rows and positions outside [0, Lmax)
- * become zero where zero_k / zero_v is 1 and keep their contents where it is 0. */
-int oa_kv4_unpack(const void* cache, int64_t c_sb, int64_t c_sh, int64_t Lmax, const void* start,
-                  int64_t start_stride, int start_i64, int64_t offset, const void* lens, int64_t lens_stride,
-                  int lens_i64, void* k_out, int64_t ko_sb, int64_t ko_sh, int64_t ko_st, void* v_out, int64_t vo_sb,
-                  int64_t vo_sh, int64_t vo_st, int dtype, int64_t B, int64_t T, int64_t HKV, int zero_k, int zero_v,
-                  void* stream);
+/* The values of records back as rows k_out, v_out (B, HKV, T, 128) (dtype OA_BF16 or OA_F32); padding rows and
+ * positions outside [0, Lmax) become zero where zero_k / zero_v is 1 and keep their contents where it is 0. */
+typedef struct {
+  oa_tensor4 cache, k_out, v_out;
+  oa_index start, lens;
+  int64_t offset, dtype, zero_k, zero_v;
+} oa_kv4_unpack_args;
+int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream);
 
 /* Dense attention over the cache: q (B, HQ, T, 128) bf16 rows, out the same shape in bf16 or fp32 (out_dtype).
  * Request b has min(n[b] + offset, Lmax) positions, its T query tokens are the last T of them and token i sees
  * positions <= length - T + i; one that sees none gives zeros.  Query head h reads KV head h / (HQ / HKV).
  * workspace: oa_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, zero before its first use; every call
  * leaves it ready for the next call of the same sizes.  Calls that share one must not overlap on the GPU. */
+typedef struct {
+  oa_tensor4 q, cache, out;
+  oa_index n;
+  void* workspace;
+  int64_t workspace_bytes, offset, out_dtype;
+  double sm_scale;
+} oa_kv4_attention_args;
 size_t oa_kv4_attention_workspace_bytes(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax);
-int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* cache, int64_t c_sb,
-                     int64_t c_sh, int64_t Lmax, const void* n, int64_t n_stride, int n_i64, int64_t offset, void* out,
-                     int64_t o_sb, int64_t o_sh, int64_t o_st, int out_dtype, int64_t B, int64_t HQ, int64_t HKV,
-                     int64_t T, float sm_scale, void* workspace, size_t workspace_bytes, void* stream);
+int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream);
 
-/* OpenAttention.flash over the cache (BH, Lmax, 144): q (BQ, 128) bf16, lists, proxies and out as in
- * oa_flash_kvhead_proxies (per_qhead 0: kbar, vbar (BH, NB, 128)) or oa_flash_qhead_proxies (per_qhead 1:
- * (BQ, NB, 128)). */
-int oa_kv4_flash(const void* q, int64_t q_stride, const void* cache, int64_t c_sh, int64_t Lmax, const int32_t* sel,
-                 int64_t n_sel, const int32_t* exp_idx, int64_t n_exp, const void* kbar, const void* vbar,
-                 int64_t kbar_stride_h, int64_t kbar_stride_b, int per_qhead, const float* log_n, int64_t log_n_stride,
-                 void* out, int64_t out_stride, int out_dtype, int64_t BQ, int64_t BH, int64_t NB, float sm_scale,
-                 void* stream);
+/* OpenAttention.flash over the cache (BH, Lmax, 144): q (BQ, 128) bf16, sel and exp_idx (BQ, n) int32 contiguous,
+ * proxies kbar, vbar (BQ, >= NB, 128) (for each query row) or (BH, >= NB, 128) (for each KV row) bf16, log_n
+ * (BQ, >= NB) fp32, out (BQ, 128) in out_dtype; semantics of oa_flash_qhead_proxies / oa_flash_kvhead_proxies.
+ * NB = 0 disables the proxies. */
+typedef struct {
+  oa_tensor2 q;
+  oa_tensor3 cache;
+  oa_tensor2 sel, exp_idx;
+  oa_tensor3 kbar, vbar;
+  oa_tensor2 log_n, out;
+  int64_t out_dtype, NB;
+  double sm_scale;
+} oa_kv4_flash_args;
+int oa_kv4_flash(const oa_kv4_flash_args* args, void* stream);
 
 #ifdef __cplusplus
 }

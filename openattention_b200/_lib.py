@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -18,6 +19,7 @@ I64 = ctypes.c_int64
 I32 = ctypes.c_int
 F32 = ctypes.c_float
 SZ = ctypes.c_size_t
+BLOCK = ctypes.c_char_p  # a packed argument block (see BLOCKS)
 
 # name -> (restype, argtypes); every compute entry returns an int status.
 SIGNATURES = {
@@ -44,17 +46,12 @@ SIGNATURES = {
     "oa_residual": (I32, [P, P, I64, I64, I64, I64, P, P, I64, P, I64, P, P, P, P, P, P, P, P, P]),
     "oa_residual_flash": (I32, [P, I64, P, P, I64, I64, I64, I64, P, P, I64, P, I64, P, P, P, P, P, P, P, P, P,
                                 I64, I32, F32, P, P]),
-    "oa_qk_norm_rope": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I32, I64, I64, I64,
-                              I64, P, P, I64, I64, P, I64, I32, I64, P, I64, I32, P, P, I32, F32, I32, I32, P]),
-    "oa_kv4_append": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64,
-                            I64, I64, I64, P, P, I64, I64, P, I64, I32, I64, P, I64, I32, P, P, I32, F32, I32, P]),
-    "oa_kv4_unpack": (I32, [P, I64, I64, I64, P, I64, I32, I64, P, I64, I32, P, I64, I64, I64, P, I64, I64, I64, I32, I64,
-                            I64, I64, I32, I32, P]),
+    "oa_qk_norm_rope": (I32, [BLOCK, P]),
+    "oa_kv4_append": (I32, [BLOCK, P]),
+    "oa_kv4_unpack": (I32, [BLOCK, P]),
     "oa_kv4_attention_workspace_bytes": (SZ, [I64, I64, I64, I64, I64]),
-    "oa_kv4_attention": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I32, I64, P, I64, I64, I64, I32, I64, I64, I64,
-                               I64, F32, P, SZ, P]),
-    "oa_kv4_flash": (I32, [P, I64, P, I64, I64, P, I64, P, I64, P, P, I64, I64, I32, P, I64, P, I64, I32, I64, I64, I64,
-                           F32, P]),
+    "oa_kv4_attention": (I32, [BLOCK, P]),
+    "oa_kv4_flash": (I32, [BLOCK, P]),
     "oa_build_codes": (I32, [P, I64, I64, I64, P, P, P, P, P]),
     "oa_build_project_workspace_bytes": (SZ, [I64]),
     "oa_build_project": (I32, [P, I64, I64, I64, P, P, P, P, SZ, P]),
@@ -63,6 +60,18 @@ SIGNATURES = {
     "oa_csr_build": (I32, [P, I64, I64, I64, I64, P, I64, P, P, P, SZ, P]),
     "oa_kmeans_update": (I32, [P, I64, I64, I64, P, I64, P, P, P, P, P, P]),
     "oa_cluster_sums": (I32, [P, P, I64, I64, I64, P, I64, P, P, P, P, P, P]),
+}
+
+# Entries that take their arguments in a block of 8-byte fields: q whole numbers and addresses, d doubles, in the
+# order of the header's structs (ctypes converts each argument of a call by itself, which for forty of them costs
+# more than the launch; packing them takes a tenth).
+_T4, _T3, _T2, _IX = "9q", "7q", "5q", "4q"
+BLOCKS = {
+    "oa_qk_norm_rope": struct.Struct("=" + 4 * _T4 + "4q" + 2 * _IX + "2q" + "5q" + "d"),
+    "oa_kv4_append": struct.Struct("=" + 5 * _T4 + "4q" + 2 * _IX + "2q" + "3q" + "d"),
+    "oa_kv4_unpack": struct.Struct("=" + 3 * _T4 + 2 * _IX + "4q"),
+    "oa_kv4_attention": struct.Struct("=" + 3 * _T4 + _IX + "4q" + "d"),
+    "oa_kv4_flash": struct.Struct("=" + _T2 + _T3 + 2 * _T2 + 2 * _T3 + 2 * _T2 + "2q" + "d"),
 }
 
 _lock = threading.Lock()
@@ -90,11 +99,15 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise RuntimeError with the library's message on failure."""
-    lib = load()
-    status = getattr(lib, name)(*args)
+    status = getattr(_lib or load(), name)(*args)
     if status != 0:
-        msg = lib.oa_last_error_string().decode(errors="replace")
+        msg = load().oa_last_error_string().decode(errors="replace")
         raise RuntimeError(f"{name} failed (status {status}): {msg}")
+
+
+def call_block(name: str, stream: int, *fields) -> None:
+    """call() of an entry that takes its arguments in a block."""
+    call(name, BLOCKS[name].pack(*fields), stream)
 
 
 def ptr(t) -> int:

@@ -7,8 +7,6 @@
 // nothing to attend give zeros.
 #include "oa_kv4_mma.cuh"
 
-#include "../../include/openattention_b200.h"
-
 namespace oa {
 namespace {
 
@@ -374,7 +372,7 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
   constexpr uint32_t kStageBytes = kWarps * kTileBytes;
   // the merge's room is the last stage: free between a row's last tile and the next row's third
   float* s_part = reinterpret_cast<float*>(s_ring + (kStages - 1) * kStageBytes);
-  const unsigned char* src;  // the next tile this warp copies, at this lane's bytes
+  const unsigned char* src = nullptr;  // the next tile this warp copies, at this lane's bytes
   auto fetch = [&](int records, uint32_t stage) {  // `records` of the tile are the request's
     const uint32_t dst = ring + stage * kStageBytes + 16 * lane;
     if (records >= kTile) {
@@ -621,11 +619,6 @@ size_t part_bytes(const DensePlan& p) {
   return (size_t)p.grid * (p.most_units >= (int64_t)kLongShare * p.grid ? kLevels : 1) * 2 * kPartFloats * sizeof(float);
 }
 
-bool rows_ok(const Rows& r, int esize) {
-  const int64_t q = 16 / esize;
-  return oa_aligned16(r.p) && r.sb % q == 0 && r.sh % q == 0 && r.st % q == 0;
-}
-
 }  // namespace
 }  // namespace oa
 
@@ -635,35 +628,30 @@ extern "C" size_t oa_kv4_attention_workspace_bytes(int64_t B, int64_t HQ, int64_
   return oa::spread_bytes(p.rows) + oa::part_bytes(p);
 }
 
-extern "C" int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* cache,
-                                int64_t c_sb, int64_t c_sh, int64_t Lmax, const void* n, int64_t n_stride, int n_i64,
-                                int64_t offset, void* out, int64_t o_sb, int64_t o_sh, int64_t o_st, int out_dtype,
-                                int64_t B, int64_t HQ, int64_t HKV, int64_t T, float sm_scale, void* workspace,
-                                size_t workspace_bytes, void* stream) {
+extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream) {
   const char* fn = "oa_kv4_attention";
-  OA_REQUIRE(B >= 0 && T >= 0 && HKV >= 1 && HQ >= HKV && HQ % HKV == 0,
-             "%s: need B, T >= 0 and HQ a multiple of HKV (B=%lld T=%lld HQ=%lld HKV=%lld)", fn, (long long)B,
-             (long long)T, (long long)HQ, (long long)HKV);
-  OA_REQUIRE(B <= 0x7fffffff && T <= 0x7fffffff && HQ <= 0x7fffffff && HQ * T <= 0x7fffffff / std::max<int64_t>(B, 1) && Lmax <= 0x7fffffff - 64, "%s: too many rows or positions", fn);
-  OA_REQUIRE(out_dtype == OA_BF16 || out_dtype == OA_F32, "%s: out_dtype must be OA_BF16 or OA_F32", fn);
-  OA_REQUIRE((cache || Lmax == 0) && oa_aligned16(cache) && c_sb % 16 == 0 && c_sh % 16 == 0 && Lmax >= 0,
-             "%s: the cache and its strides must be multiples of 16 bytes", fn);
-  if (B == 0 || T == 0) return OA_OK;
-  OA_REQUIRE(q && out && n, "%s: null q/out/n", fn);
+  OA_REQUIRE(args != nullptr, "%s: null arguments", fn);
+  const oa_kv4_attention_args& g = *args;
+  OA_REQUIRE(g.out_dtype == OA_BF16 || g.out_dtype == OA_F32, "%s: out_dtype must be OA_BF16 or OA_F32", fn);
   oa::DenseArgs a;
-  a.q = oa::Rows{q, q_sb, q_sh, q_st};
-  a.o = oa::Rows{out, o_sb, o_sh, o_st};
-  OA_REQUIRE(oa::rows_ok(a.q, 2) && oa::rows_ok(a.o, out_dtype == OA_F32 ? 4 : 2),
-             "%s: q and out rows must start on 16-byte boundaries (base addresses and strides)", fn);
-  a.cache = static_cast<const unsigned char*>(cache);
-  a.c_sb = c_sb;
-  a.c_sh = c_sh;
+  const int64_t B = g.q.size[0], HQ = g.q.size[1], T = g.q.size[2], HKV = g.cache.size[1], Lmax = g.cache.size[2];
+  OA_TRY(oa_take_cache(fn, g.cache, false, &a.cache, &a.c_sb, &a.c_sh));
+  OA_REQUIRE(g.cache.size[0] == B && HKV >= 1 && HQ >= HKV && HQ % HKV == 0,
+             "%s: q holds %lld requests of %lld heads, the cache %lld of %lld: need the same requests and a multiple of the KV "
+             "heads",
+             fn, (long long)B, (long long)HQ, (long long)g.cache.size[0], (long long)HKV);
+  OA_TRY(oa_take_rows(fn, "q", g.q, 2, B, HQ, T, false, &a.q));
+  OA_TRY(oa_take_rows(fn, "out", g.out, g.out_dtype == OA_F32 ? 4 : 2, B, HQ, T, true, &a.o));
+  OA_TRY(oa_take_index(fn, "n", g.n, B, true, &a.n));
+  if (B == 0 || T == 0) return OA_OK;
+  OA_REQUIRE(HQ * T <= 0x7fffffff / B, "%s: too many rows", fn);
   a.Lmax = Lmax;
-  a.n = oa::PerRequest{n, n_stride, n_i64};
-  a.offset = offset;
-  a.out_f32 = out_dtype == OA_F32;
+  a.offset = g.offset;
+  a.out_f32 = g.out_dtype == OA_F32;
   a.B = (int)B; a.HQ = (int)HQ; a.HKV = (int)HKV; a.T = (int)T;
-  a.qk_scale = sm_scale * oa::kLog2e;
+  a.qk_scale = (float)(g.sm_scale * (double)oa::kLog2e);
+  void* const workspace = g.workspace;
+  const size_t workspace_bytes = (size_t)std::max<int64_t>(g.workspace_bytes, 0);
   const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
   // units on the line (and 9 of them per row of the grid's widest product) are counted in 32 bits
   OA_REQUIRE(p.most_units <= 0xffffffffll / 9 && p.most_units / p.rows * 8 * p.grid <= 0xffffffffll,
@@ -690,46 +678,67 @@ extern "C" int oa_kv4_attention(const void* q, int64_t q_sb, int64_t q_sh, int64
   return oa_check_launch(fn);
 }
 
-extern "C" int oa_kv4_flash(const void* q, int64_t q_stride, const void* cache, int64_t c_sh, int64_t Lmax,
-                            const int32_t* sel, int64_t n_sel, const int32_t* exp_idx, int64_t n_exp,
-                            const void* kbar, const void* vbar, int64_t kbar_stride_h, int64_t kbar_stride_b,
-                            int per_qhead, const float* log_n, int64_t log_n_stride, void* out, int64_t out_stride,
-                            int out_dtype, int64_t BQ, int64_t BH, int64_t NB, float sm_scale, void* stream) {
+extern "C" int oa_kv4_flash(const oa_kv4_flash_args* args, void* stream) {
   const char* fn = "oa_kv4_flash";
-  OA_REQUIRE(BQ >= 0 && BH >= 1 && BQ % BH == 0 && BQ <= 0x7fffffff, "%s: need BQ a multiple of BH (BQ=%lld BH=%lld)",
+  OA_REQUIRE(args != nullptr, "%s: null arguments", fn);
+  const oa_kv4_flash_args& g = *args;
+  const int64_t BQ = g.q.size[0], BH = g.cache.size[0], NB = g.NB;
+  OA_REQUIRE(g.out_dtype == OA_BF16 || g.out_dtype == OA_F32, "%s: out_dtype must be OA_BF16 or OA_F32", fn);
+  OA_REQUIRE(BQ >= 0 && BQ <= 0x7fffffff && BH >= 1 && BQ % BH == 0, "%s: q's %lld rows must be a multiple of the cache's %lld",
              fn, (long long)BQ, (long long)BH);
-  OA_REQUIRE(n_sel >= 0 && n_exp >= 0 && NB >= 0 && Lmax >= 0 && n_sel + n_exp + NB < (int64_t)1 << 30,
-             "%s: bad list sizes", fn);
-  OA_REQUIRE(out_dtype == OA_BF16 || out_dtype == OA_F32, "%s: out_dtype must be OA_BF16 or OA_F32", fn);
-  if (BQ == 0) return OA_OK;
-  OA_REQUIRE(q && (cache || Lmax == 0) && out, "%s: null q/cache/out", fn);
-  OA_REQUIRE((n_sel == 0 || sel) && (n_exp == 0 || exp_idx), "%s: null index list", fn);
-  OA_REQUIRE(NB == 0 || (kbar && vbar && log_n), "%s: null kbar/vbar/log_n with NB > 0", fn);
-  OA_REQUIRE(oa_aligned16(q) && oa_aligned16(cache) && q_stride % 8 == 0 && c_sh % 16 == 0,
-             "%s: q and the cache must start on 16-byte boundaries (base addresses and strides)", fn);
-  OA_REQUIRE(NB == 0 || (oa_aligned16(kbar) && oa_aligned16(vbar) && kbar_stride_h % 8 == 0 && kbar_stride_b % 8 == 0),
-             "%s: kbar/vbar rows must start on 16-byte boundaries", fn);
+  const oa_tensor4 c4 = {g.cache.p, {1, BH, g.cache.size[1], g.cache.size[2]}, {0, g.cache.stride[0], g.cache.stride[1], g.cache.stride[2]}};
   oa::ListArgs a;
-  a.q = static_cast<const __nv_bfloat16*>(q);
-  a.q_stride = q_stride;
-  a.cache = static_cast<const unsigned char*>(cache);
-  a.c_sh = c_sh;
-  a.Lmax = Lmax;
-  a.sel = sel;
-  a.exp = exp_idx;
+  int64_t none;
+  OA_TRY(oa_take_cache(fn, c4, false, &a.cache, &none, &a.c_sh));
+  OA_REQUIRE(g.q.size[1] == oa::kD && g.out.size[0] == BQ && g.out.size[1] == oa::kD, "%s: q and out must be (%lld, 128)", fn,
+             (long long)BQ);
+  OA_REQUIRE(g.sel.size[0] == BQ && g.exp_idx.size[0] == BQ, "%s: sel_idx and exp_idx must have %lld rows", fn, (long long)BQ);
+  const int64_t n_sel = g.sel.size[1], n_exp = g.exp_idx.size[1];
+  OA_REQUIRE(NB >= 0 && n_sel >= 0 && n_exp >= 0 && n_sel + n_exp + NB < (int64_t)1 << 30, "%s: bad list sizes", fn);
+  if (BQ == 0) return OA_OK;
+  OA_REQUIRE(g.q.p && g.out.p && g.q.stride[1] == 1 && g.out.stride[1] == 1, "%s: q and out must have a contiguous last dim", fn);
+  const int es = g.out_dtype == OA_F32 ? 4 : 2;
+  a.q_stride = BQ > 1 ? g.q.stride[0] : 0;
+  a.out_stride = BQ > 1 ? g.out.stride[0] : 0;
+  OA_REQUIRE(BQ <= 1 || a.out_stride >= oa::kD || a.out_stride <= -oa::kD, "%s: out's rows overlap", fn);
+  OA_REQUIRE(oa_aligned16(g.q.p) && oa_aligned16(g.out.p) && a.q_stride % 8 == 0 && a.out_stride * es % 16 == 0,
+             "%s: q and out rows must start on 16-byte boundaries (base addresses and strides)", fn);
+  OA_REQUIRE((n_sel == 0 || (g.sel.p && g.sel.stride[1] == 1 && (BQ == 1 || g.sel.stride[0] == n_sel))) &&
+                 (n_exp == 0 || (g.exp_idx.p && g.exp_idx.stride[1] == 1 && (BQ == 1 || g.exp_idx.stride[0] == n_exp))),
+             "%s: sel_idx and exp_idx must be contiguous", fn);
+  a.kbar = a.vbar = nullptr;
+  a.kb_sh = a.kb_sb = a.ln_stride = 0;
+  a.logn = nullptr;
+  a.per_qhead = 1;
+  if (NB > 0) {
+    bool same = true;
+    for (int i = 0; i < 3; ++i) same = same && g.kbar.size[i] == g.vbar.size[i] && g.kbar.stride[i] == g.vbar.stride[i];
+    OA_REQUIRE(same && (g.kbar.size[0] == BQ || g.kbar.size[0] == BH) && g.kbar.size[1] >= NB && g.kbar.size[2] == oa::kD &&
+                   g.kbar.stride[2] == 1,
+               "%s: kbar and vbar must be (%lld or %lld, >= %lld, 128) of one shape and strides with a contiguous last dim", fn,
+               (long long)BQ, (long long)BH, (long long)NB);
+    OA_REQUIRE(g.log_n.size[0] == BQ && g.log_n.size[1] >= NB && g.log_n.stride[1] == 1,
+               "%s: log_n must be (%lld, >= %lld) with a contiguous last dim", fn, (long long)BQ, (long long)NB);
+    OA_REQUIRE(g.kbar.p && g.vbar.p && g.log_n.p, "%s: null kbar/vbar/log_n with NB > 0", fn);
+    a.kb_sh = g.kbar.size[0] > 1 ? g.kbar.stride[0] : 0;
+    a.kb_sb = g.kbar.size[1] > 1 ? g.kbar.stride[1] : 0;
+    OA_REQUIRE(oa_aligned16(g.kbar.p) && oa_aligned16(g.vbar.p) && a.kb_sh % 8 == 0 && a.kb_sb % 8 == 0,
+               "%s: kbar/vbar rows must start on 16-byte boundaries", fn);
+    a.kbar = static_cast<const __nv_bfloat16*>(g.kbar.p);
+    a.vbar = static_cast<const __nv_bfloat16*>(g.vbar.p);
+    a.per_qhead = g.kbar.size[0] == BQ;
+    a.logn = static_cast<const float*>(g.log_n.p);
+    a.ln_stride = BQ > 1 ? g.log_n.stride[0] : 0;
+  }
+  a.q = static_cast<const __nv_bfloat16*>(g.q.p);
+  a.Lmax = g.cache.size[1];
+  a.sel = static_cast<const int32_t*>(g.sel.p);
+  a.exp = static_cast<const int32_t*>(g.exp_idx.p);
   a.n_sel = (int)n_sel; a.n_exp = (int)n_exp; a.NB = (int)NB;
-  a.kbar = static_cast<const __nv_bfloat16*>(kbar);
-  a.vbar = static_cast<const __nv_bfloat16*>(vbar);
-  a.kb_sh = kbar_stride_h;
-  a.kb_sb = kbar_stride_b;
-  a.per_qhead = per_qhead;
-  a.logn = log_n;
-  a.ln_stride = log_n_stride;
-  a.out = out;
-  a.out_stride = out_stride;
-  a.out_f32 = out_dtype == OA_F32;
+  a.out = const_cast<void*>(g.out.p);
+  a.out_f32 = g.out_dtype == OA_F32;
   a.G = (int)(BQ / BH);
-  a.qk_scale = sm_scale * oa::kLog2e;
+  a.qk_scale = (float)(g.sm_scale * (double)oa::kLog2e);
   oa::list_kernel<<<(unsigned)BQ, oa::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return oa_check_launch(fn);
 }

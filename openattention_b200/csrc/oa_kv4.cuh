@@ -14,6 +14,7 @@
 // groups (low nibbles against high nibbles), and 72 bytes per row and side = 4.5 bits per value.
 #pragma once
 #include "oa_common.cuh"
+#include "../../include/openattention_b200.h"
 
 namespace oa {
 
@@ -38,3 +39,67 @@ struct Rows {
 };
 
 }  // namespace oa
+
+// ---------------------------------------------------------------- host: checks of the argument blocks
+#define OA_TRY(e)                 \
+  do {                            \
+    const int rc_ = (e);          \
+    if (rc_ != OA_OK) return rc_; \
+  } while (0)
+
+// Rows (B, H, T, 128) of element size `esize` into out (strides of single-element dims cleared: any number may
+// stand there); H, T < 0: any.  Empty rows have no address.  `writes`: rows must not share memory.
+static inline int oa_take_rows(const char* fn, const char* name, const oa_tensor4& t, int esize, int64_t B, int64_t H,
+                               int64_t T, bool writes, oa::Rows* out) {
+  OA_REQUIRE(t.size[0] == B && (H < 0 || t.size[1] == H) && (T < 0 || t.size[2] == T) && t.size[3] == oa::kD,
+             "%s: %s must be (%lld, %lld, %lld, 128) rows, got (%lld, %lld, %lld, %lld)", fn, name, (long long)B,
+             (long long)(H < 0 ? t.size[1] : H), (long long)(T < 0 ? t.size[2] : T), (long long)t.size[0],
+             (long long)t.size[1], (long long)t.size[2], (long long)t.size[3]);
+  OA_REQUIRE(t.size[0] >= 0 && t.size[1] >= 0 && t.size[2] >= 0 && t.size[0] <= 0x7fffffff && t.size[1] <= 0xfffff &&
+                 t.size[2] <= 0x7fffffff,
+             "%s: %s: bad sizes (%lld, %lld, %lld, 128)", fn, name, (long long)t.size[0], (long long)t.size[1],
+             (long long)t.size[2]);
+  const bool empty = t.size[0] == 0 || t.size[1] == 0 || t.size[2] == 0;
+  OA_REQUIRE(t.p != nullptr || empty, "%s: null %s", fn, name);
+  OA_REQUIRE(t.stride[3] == 1 || empty, "%s: %s must have a contiguous last dim", fn, name);
+  int64_t st[3];
+  for (int i = 0; i < 3; ++i) {
+    st[i] = t.size[i] > 1 ? t.stride[i] : 0;
+    OA_REQUIRE(!writes || empty || t.size[i] <= 1 || st[i] != 0, "%s: %s must not be an expanded tensor", fn, name);
+    OA_REQUIRE(st[i] * esize % 16 == 0 || empty, "%s: %s rows must start on 16-byte boundaries (strides)", fn, name);
+  }
+  OA_REQUIRE(oa_aligned16(t.p), "%s: %s rows must start on 16-byte boundaries (base address)", fn, name);
+  *out = oa::Rows{t.p, st[0], st[1], st[2]};
+  return OA_OK;
+}
+
+static inline int oa_take_index(const char* fn, const char* name, const oa_index& x, int64_t B, bool required,
+                                oa::PerRequest* out) {
+  OA_REQUIRE(x.p != nullptr || !required || B == 0, "%s: %s must be given", fn, name);
+  OA_REQUIRE(x.p == nullptr || x.size == 1 || x.size == B, "%s: %s must hold %lld numbers or one, got %lld", fn, name,
+             (long long)B, (long long)x.size);
+  *out = oa::PerRequest{x.p, x.size == 1 ? 0 : x.stride, (int)x.is_int64};
+  return OA_OK;
+}
+
+// A cache (B, HKV, Lmax, 144): its strides in bytes (0 for dims of one element).
+static inline int oa_take_cache(const char* fn, const oa_tensor4& t, bool writes, const unsigned char** p, int64_t* sb,
+                                int64_t* sh) {
+  OA_REQUIRE(t.size[3] == oa::kRec && t.stride[3] == 1 && (t.size[2] <= 1 || t.stride[2] == oa::kRec),
+             "%s: the cache must be (B, hkv, Lmax, 144) bytes with contiguous records, got (%lld, %lld, %lld, %lld) with strides "
+             "(%lld, %lld, %lld, %lld)",
+             fn, (long long)t.size[0], (long long)t.size[1], (long long)t.size[2], (long long)t.size[3],
+             (long long)t.stride[0], (long long)t.stride[1], (long long)t.stride[2], (long long)t.stride[3]);
+  OA_REQUIRE(t.size[0] >= 0 && t.size[1] >= 0 && t.size[2] >= 0 && t.size[2] <= 0x7fffffff - 64,
+             "%s: the cache has bad sizes (%lld, %lld, %lld, 144)", fn, (long long)t.size[0], (long long)t.size[1],
+             (long long)t.size[2]);
+  const bool empty = t.size[0] == 0 || t.size[1] == 0 || t.size[2] == 0;
+  OA_REQUIRE((t.p != nullptr || empty) && oa_aligned16(t.p), "%s: the cache must start on a 16-byte boundary", fn);
+  *p = static_cast<const unsigned char*>(t.p);
+  *sb = t.size[0] > 1 ? t.stride[0] : 0;
+  *sh = t.size[1] > 1 ? t.stride[1] : 0;
+  OA_REQUIRE(empty || (*sb % 16 == 0 && *sh % 16 == 0), "%s: cache strides must be multiples of 16 bytes", fn);
+  OA_REQUIRE(!writes || empty || ((t.size[0] <= 1 || *sb != 0) && (t.size[1] <= 1 || *sh != 0)),
+             "%s: the cache must not be an expanded tensor: its requests would share records", fn);
+  return OA_OK;
+}

@@ -12,8 +12,6 @@
 // rotation's partner dims are R/16 lanes away and a quantisation group is eight lanes.
 #include "oa_kv4.cuh"
 
-#include "../../include/openattention_b200.h"
-
 namespace oa {
 namespace {
 
@@ -249,11 +247,6 @@ __global__ void __launch_bounds__(kRowThreads) unpack_kernel(const UnpackArgs a)
 }
 
 // ---------------------------------------------------------------- host side
-bool rows_ok(const Rows& r, int esize) {
-  const int64_t q = 16 / esize;
-  return oa_aligned16(r.p) && r.sb % q == 0 && r.sh % q == 0 && r.st % q == 0;
-}
-
 template <typename E, bool CACHE>
 int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
   if (a.B == 0 || a.T == 0 || a.heads == 0) return OA_OK;
@@ -269,153 +262,104 @@ int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
   return oa_check_launch(fn);
 }
 
-int check_common(const char* fn, int64_t B, int64_t T, int64_t HQ, int64_t HKV, const void* start) {
-  OA_REQUIRE(B >= 0 && T >= 0 && HQ >= 0 && HKV >= 1 && HQ <= (1 << 20) && HKV <= (1 << 20), "%s: bad sizes (B=%lld T=%lld HQ=%lld HKV=%lld)", fn,
-             (long long)B, (long long)T, (long long)HQ, (long long)HKV);
-  OA_REQUIRE(B <= 0x7fffffff && T <= 0x7fffffff, "%s: B and T must fit 31 bits", fn);
-  OA_REQUIRE(start != nullptr, "%s: null start", fn);
+// The parts of a block that oa_qk_norm_rope and oa_kv4_append share.
+template <typename Args>
+int take_rope(const char* fn, const Args& g, RowArgs& a) {
+  OA_REQUIRE(g.cos && g.sin && oa_aligned16(g.cos) && oa_aligned16(g.sin), "%s: cos/sin must be 16-byte aligned", fn);
+  OA_REQUIRE(g.P >= 0 && g.R >= 16 && g.R <= kD && g.R % 16 == 0,
+             "%s: the rotated width must be a multiple of 16 in 16..128 (got %lld)", fn, (long long)g.R);
+  OA_REQUIRE(g.w_dtype == OA_BF16 || g.w_dtype == OA_F32, "%s: w_dtype must be OA_BF16 or OA_F32", fn);
+  OA_REQUIRE(oa_aligned16(g.q_weight) && oa_aligned16(g.k_weight), "%s: weights must be 16-byte aligned", fn);
+  a.cos = g.cos;
+  a.sin = g.sin;
+  a.P = g.P;
+  a.R = (int)g.R;
+  a.wq = g.q_weight;
+  a.wk = g.k_weight;
+  a.w_f32 = g.w_dtype == OA_F32;
+  a.eps = (float)g.eps;
+  a.zero_q = g.zero_q != 0;
   return OA_OK;
 }
-int check_table(const char* fn, const float* cos, const float* sin, int64_t P, int64_t R) {
-  OA_REQUIRE(cos && sin && oa_aligned16(cos) && oa_aligned16(sin), "%s: cos/sin must be 16-byte aligned", fn);
-  OA_REQUIRE(P >= 0 && R >= 16 && R <= kD && R % 16 == 0, "%s: the rotated width must be a multiple of 16 in 16..128 (got %lld)",
-             fn, (long long)R);
-  return OA_OK;
-}
-int check_cache(const char* fn, const void* cache, int64_t sb, int64_t sh, int64_t Lmax) {
-  OA_REQUIRE((cache || Lmax == 0) && oa_aligned16(cache), "%s: the cache must be 16-byte aligned", fn);
-  OA_REQUIRE(sb % 16 == 0 && sh % 16 == 0, "%s: cache strides must be multiples of 16 bytes", fn);
-  OA_REQUIRE(Lmax >= 0, "%s: negative cache length", fn);
-  return OA_OK;
-}
-#define OA_TRY(e)              \
-  do {                         \
-    const int rc_ = (e);       \
-    if (rc_ != OA_OK) return rc_; \
-  } while (0)
 
 }  // namespace
 }  // namespace oa
 
-using oa::Rows;
-using oa::PerRequest;
-
-extern "C" int oa_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb,
-                               int64_t k_sh, int64_t k_st, void* q_out, int64_t qo_sb, int64_t qo_sh, int64_t qo_st,
-                               void* k_out, int64_t ko_sb, int64_t ko_sh, int64_t ko_st, int dtype, int64_t B,
-                               int64_t T, int64_t HQ, int64_t HKV, const float* cos, const float* sin, int64_t P,
-                               int64_t R, const void* start, int64_t start_stride, int start_i64, int64_t offset,
-                               const void* lens, int64_t lens_stride, int lens_i64, const void* q_weight,
-                               const void* k_weight, int w_dtype, float eps, int zero_q, int zero_k, void* stream) {
+extern "C" int oa_qk_norm_rope(const oa_qk_norm_rope_args* args, void* stream) {
   const char* fn = "oa_qk_norm_rope";
-  OA_TRY(oa::check_common(fn, B, T, HQ, HKV, start));
-  OA_TRY(oa::check_table(fn, cos, sin, P, R));
-  OA_REQUIRE(dtype == OA_BF16 || dtype == OA_F32, "%s: dtype must be OA_BF16 or OA_F32", fn);
-  OA_REQUIRE(w_dtype == OA_BF16 || w_dtype == OA_F32, "%s: w_dtype must be OA_BF16 or OA_F32", fn);
-  OA_REQUIRE(oa_aligned16(q_weight) && oa_aligned16(k_weight), "%s: weights must be 16-byte aligned", fn);
+  OA_REQUIRE(args != nullptr, "%s: null arguments", fn);
+  const oa_qk_norm_rope_args& g = *args;
+  OA_REQUIRE(g.dtype == OA_BF16 || g.dtype == OA_F32, "%s: dtype must be OA_BF16 or OA_F32", fn);
   oa::RowArgs a{};
-  a.q = Rows{q, q_sb, q_sh, q_st};
-  a.k = Rows{k, k_sb, k_sh, k_st};
-  a.qo = Rows{q_out, qo_sb, qo_sh, qo_st};
-  a.ko = Rows{k_out, ko_sb, ko_sh, ko_st};
-  const int es = dtype == OA_F32 ? 4 : 2;
-  OA_REQUIRE(B * T == 0 || (k && k_out && (HQ == 0 || (q && q_out))), "%s: null rows", fn);
-  OA_REQUIRE(oa::rows_ok(a.q, es) && oa::rows_ok(a.k, es) && oa::rows_ok(a.qo, es) && oa::rows_ok(a.ko, es),
-             "%s: rows must start on 16-byte boundaries (base addresses and strides)", fn);
-  a.cos = cos;
-  a.sin = sin;
-  a.P = P;
-  a.R = (int)R;
-  a.start = PerRequest{start, start_stride, start_i64};
-  a.lens = PerRequest{lens, lens_stride, lens_i64};
-  a.offset = offset;
-  a.wq = q_weight;
-  a.wk = k_weight;
-  a.w_f32 = w_dtype == OA_F32;
-  a.eps = eps;
-  a.zero_q = zero_q;
-  a.zero_k = zero_k;
+  const int es = g.dtype == OA_F32 ? 4 : 2;
+  const int64_t B = g.q.size[0], HQ = g.q.size[1], T = g.q.size[2], HKV = g.k.size[1];
+  OA_TRY(oa_take_rows(fn, "q", g.q, es, B, -1, T, false, &a.q));
+  OA_TRY(oa_take_rows(fn, "k", g.k, es, B, -1, T, false, &a.k));
+  OA_TRY(oa_take_rows(fn, "q_out", g.q_out, es, B, HQ, T, true, &a.qo));
+  OA_TRY(oa_take_rows(fn, "k_out", g.k_out, es, B, HKV, T, true, &a.ko));
+  OA_TRY(oa::take_rope(fn, g, a));
+  OA_TRY(oa_take_index(fn, "start", g.start, B, true, &a.start));
+  OA_TRY(oa_take_index(fn, "lens", g.lens, B, false, &a.lens));
+  a.zero_k = g.zero_k != 0;
+  a.offset = g.offset;
   a.B = (int)B; a.T = (int)T; a.HQ = (int)HQ; a.HKV = (int)HKV;
   a.heads = (int)(HQ + HKV);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == OA_F32 ? oa::launch_rows<float, false>(a, fn, st) : oa::launch_rows<__nv_bfloat16, false>(a, fn, st);
+  return g.dtype == OA_F32 ? oa::launch_rows<float, false>(a, fn, st) : oa::launch_rows<__nv_bfloat16, false>(a, fn, st);
 }
 
-extern "C" int oa_kv4_append(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st, const void* k, int64_t k_sb,
-                             int64_t k_sh, int64_t k_st, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_st,
-                             void* q_out, int64_t qo_sb, int64_t qo_sh, int64_t qo_st, void* cache, int64_t c_sb,
-                             int64_t c_sh, int64_t Lmax, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
-                             const float* cos, const float* sin, int64_t P, int64_t R, const void* start,
-                             int64_t start_stride, int start_i64, int64_t offset, const void* lens,
-                             int64_t lens_stride, int lens_i64, const void* q_weight, const void* k_weight,
-                             int w_dtype, float eps, int zero_q, void* stream) {
+extern "C" int oa_kv4_append(const oa_kv4_append_args* args, void* stream) {
   const char* fn = "oa_kv4_append";
-  OA_TRY(oa::check_common(fn, B, T, HQ, HKV, start));
-  OA_TRY(oa::check_cache(fn, cache, c_sb, c_sh, Lmax));
-  if (cos || sin) OA_TRY(oa::check_table(fn, cos, sin, P, R));
-  OA_REQUIRE(cos || (HQ == 0 && !q_weight && !k_weight), "%s: queries and norm weights need the cos/sin tables", fn);
-  OA_REQUIRE(w_dtype == OA_BF16 || w_dtype == OA_F32, "%s: w_dtype must be OA_BF16 or OA_F32", fn);
-  OA_REQUIRE(oa_aligned16(q_weight) && oa_aligned16(k_weight), "%s: weights must be 16-byte aligned", fn);
+  OA_REQUIRE(args != nullptr, "%s: null arguments", fn);
+  const oa_kv4_append_args& g = *args;
   oa::RowArgs a{};
-  a.q = Rows{q, q_sb, q_sh, q_st};
-  a.k = Rows{k, k_sb, k_sh, k_st};
-  a.v = Rows{v, v_sb, v_sh, v_st};
-  a.qo = Rows{q_out, qo_sb, qo_sh, qo_st};
-  OA_REQUIRE(B * T == 0 || (k && v && (HQ == 0 || (q && q_out))), "%s: null rows", fn);
-  OA_REQUIRE(oa::rows_ok(a.q, 2) && oa::rows_ok(a.k, 2) && oa::rows_ok(a.v, 2) && oa::rows_ok(a.qo, 2),
-             "%s: rows must start on 16-byte boundaries (base addresses and strides)", fn);
-  a.cache = static_cast<unsigned char*>(cache);
-  a.c_sb = c_sb;
-  a.c_sh = c_sh;
-  a.Lmax = Lmax;
-  a.cos = cos;
-  a.sin = sin;
-  a.P = P;
-  a.R = (int)R;
-  a.start = PerRequest{start, start_stride, start_i64};
-  a.lens = PerRequest{lens, lens_stride, lens_i64};
-  a.offset = offset;
-  a.wq = q_weight;
-  a.wk = k_weight;
-  a.w_f32 = w_dtype == OA_F32;
-  a.eps = eps;
-  a.zero_q = zero_q;
+  const unsigned char* cache;
+  OA_TRY(oa_take_cache(fn, g.cache, true, &cache, &a.c_sb, &a.c_sh));
+  a.cache = const_cast<unsigned char*>(cache);
+  a.Lmax = g.cache.size[2];
+  const int64_t B = g.cache.size[0], HKV = g.cache.size[1], T = g.k.size[2];
+  OA_TRY(oa_take_rows(fn, "k", g.k, 2, B, HKV, T, false, &a.k));
+  OA_TRY(oa_take_rows(fn, "v", g.v, 2, B, HKV, T, false, &a.v));
+  int64_t HQ = 0;
+  if (g.cos || g.sin || g.q.p || g.q_out.p) {
+    HQ = g.q.size[1];
+    OA_TRY(oa_take_rows(fn, "q", g.q, 2, B, -1, T, false, &a.q));
+    OA_TRY(oa_take_rows(fn, "q_out", g.q_out, 2, B, HQ, T, true, &a.qo));
+    OA_TRY(oa::take_rope(fn, g, a));
+  } else {
+    OA_REQUIRE(!g.q_weight && !g.k_weight, "%s: norm weights need the cos/sin tables", fn);
+  }
+  OA_TRY(oa_take_index(fn, "start", g.start, B, true, &a.start));
+  OA_TRY(oa_take_index(fn, "lens", g.lens, B, false, &a.lens));
+  a.offset = g.offset;
   a.B = (int)B; a.T = (int)T; a.HQ = (int)HQ; a.HKV = (int)HKV;
   a.heads = (int)(HQ + 2 * HKV);
   return oa::launch_rows<__nv_bfloat16, true>(a, fn, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int oa_kv4_unpack(const void* cache, int64_t c_sb, int64_t c_sh, int64_t Lmax, const void* start,
-                             int64_t start_stride, int start_i64, int64_t offset, const void* lens,
-                             int64_t lens_stride, int lens_i64, void* k_out, int64_t ko_sb, int64_t ko_sh,
-                             int64_t ko_st, void* v_out, int64_t vo_sb, int64_t vo_sh, int64_t vo_st, int dtype,
-                             int64_t B, int64_t T, int64_t HKV, int zero_k, int zero_v, void* stream) {
+extern "C" int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream) {
   const char* fn = "oa_kv4_unpack";
-  OA_TRY(oa::check_common(fn, B, T, 0, HKV, start));
-  OA_TRY(oa::check_cache(fn, cache, c_sb, c_sh, Lmax));
-  OA_REQUIRE(dtype == OA_BF16 || dtype == OA_F32, "%s: dtype must be OA_BF16 or OA_F32", fn);
+  OA_REQUIRE(args != nullptr, "%s: null arguments", fn);
+  const oa_kv4_unpack_args& g = *args;
+  OA_REQUIRE(g.dtype == OA_BF16 || g.dtype == OA_F32, "%s: dtype must be OA_BF16 or OA_F32", fn);
   oa::UnpackArgs a{};
-  a.cache = static_cast<const unsigned char*>(cache);
-  a.c_sb = c_sb;
-  a.c_sh = c_sh;
-  a.Lmax = Lmax;
-  a.start = PerRequest{start, start_stride, start_i64};
-  a.lens = PerRequest{lens, lens_stride, lens_i64};
-  a.offset = offset;
-  a.ko = Rows{k_out, ko_sb, ko_sh, ko_st};
-  a.vo = Rows{v_out, vo_sb, vo_sh, vo_st};
-  a.zero_k = zero_k;
-  a.zero_v = zero_v;
+  OA_TRY(oa_take_cache(fn, g.cache, false, &a.cache, &a.c_sb, &a.c_sh));
+  a.Lmax = g.cache.size[2];
+  const int64_t B = g.cache.size[0], HKV = g.cache.size[1], T = g.k_out.size[2];
+  const int es = g.dtype == OA_F32 ? 4 : 2;
+  OA_TRY(oa_take_rows(fn, "k_out", g.k_out, es, B, HKV, T, true, &a.ko));
+  OA_TRY(oa_take_rows(fn, "v_out", g.v_out, es, B, HKV, T, true, &a.vo));
+  OA_TRY(oa_take_index(fn, "start", g.start, B, true, &a.start));
+  OA_TRY(oa_take_index(fn, "lens", g.lens, B, false, &a.lens));
+  a.offset = g.offset;
+  a.zero_k = g.zero_k != 0;
+  a.zero_v = g.zero_v != 0;
   a.B = (int)B; a.T = (int)T; a.HKV = (int)HKV;
-  if (B * T == 0) return OA_OK;
-  OA_REQUIRE(k_out && v_out, "%s: null rows", fn);
-  const int es = dtype == OA_F32 ? 4 : 2;
-  OA_REQUIRE(oa::rows_ok(a.ko, es) && oa::rows_ok(a.vo, es),
-             "%s: rows must start on 16-byte boundaries (base addresses and strides)", fn);
+  if (B == 0 || T == 0 || HKV == 0) return OA_OK;
   const int64_t grid = (B * T * HKV * 16 + oa::kRowThreads - 1) / oa::kRowThreads;
   OA_REQUIRE(grid <= 0x7fffffff, "%s: too many rows", fn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == OA_F32)
+  if (g.dtype == OA_F32)
     oa::unpack_kernel<float><<<(unsigned)grid, oa::kRowThreads, 0, st>>>(a);
   else
     oa::unpack_kernel<__nv_bfloat16><<<(unsigned)grid, oa::kRowThreads, 0, st>>>(a);

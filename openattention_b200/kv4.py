@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .geometry import D, HKV
-from .rotary import _call, _CODE, _out, _per_request, _rows, _same_device, _strides, _table, _weights
+from .rotary import _call, _CODE, _current_stream, _index, _like, _rows, _same_device, _table, _weights
 
 REC = 144
 
@@ -32,51 +32,28 @@ def new_cache(B, Lmax, dev, hkv=HKV):
     return torch.zeros(B, hkv, Lmax, REC, dtype=torch.uint8, device=dev)
 
 
-def _cache(cache, ndim=4, write=False):
-    if not isinstance(cache, torch.Tensor) or not cache.is_cuda:
-        raise RuntimeError("cache must be a CUDA tensor")
-    if cache.dtype != torch.uint8 or cache.dim() != ndim or cache.shape[-1] != REC or cache.stride(-1) != 1 or \
-            (cache.shape[-2] > 1 and cache.stride(-2) != REC):
-        raise RuntimeError(f"cache must be {'(B, hkv, Lmax, 144)' if ndim == 4 else '(B * hkv, Lmax, 144)'} uint8 with "
-                           f"contiguous records, got {tuple(cache.shape)} {cache.dtype} strides {cache.stride()}")
-    if write and any(s == 0 and n > 1 for n, s in zip(cache.shape, cache.stride())):
-        raise RuntimeError("cache must not be an expanded tensor: its requests would share records")
+def _cache(cache, ndim=4):
+    """The block's fields of a cache; sizes and strides are checked by the entry."""
+    if not isinstance(cache, torch.Tensor) or not cache.is_cuda or cache.dtype is not torch.uint8 or cache.dim() != ndim:
+        if not isinstance(cache, torch.Tensor) or not cache.is_cuda:
+            raise RuntimeError("cache must be a CUDA tensor")
+        raise RuntimeError(f"cache must be {'(B, hkv, Lmax, 144)' if ndim == 4 else '(B * hkv, Lmax, 144)'} uint8, got "
+                           f"{tuple(cache.shape)} {cache.dtype}")
+    return cache.data_ptr(), *cache.shape, *cache.stride()
 
 
-def _hstrides(cache):
-    return tuple(0 if n == 1 else s for n, s in zip(cache.shape[:-2], cache.stride()[:-2]))
-
-
-def _append(cache, q, k, v, cos, sin, start, offset, lens, q_weight, k_weight, eps, q_out):
-    _cache(cache, write=True)
-    dev, (B, hkv, Lmax, _) = cache.device, cache.shape
-    _rows("k", k, torch.bfloat16, (B, hkv, k.shape[2], D) if isinstance(k, torch.Tensor) and k.dim() == 4 else None)
-    T = k.shape[2]
-    _rows("v", v, torch.bfloat16, k.shape)
-    _same_device(dev, k=k, v=v, q=q, q_out=q_out)
-    st, ln = _per_request("start", start, B, dev), _per_request("lens", lens, B, dev)
-    tab, wts, HQ, zq = (0, 0, 0, 0), (0, 0, _lib.OA_F32), 0, False
-    if start is None:
-        raise RuntimeError("start must be given: the position of each request's first row")
-    if q is not None:
-        _rows("q", q, torch.bfloat16, (B, q.shape[1], T, D) if q.dim() == 4 else None)
-        HQ = q.shape[1]
-        tab, wts, zq = _table(cos, sin, dev), _weights(q_weight, k_weight, torch.bfloat16, dev), q_out is None
-        if zq:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        else:
-            _out("q_out", q_out, q.dtype, q.shape)
-    p = _lib.ptr
-    _call(dev, "oa_kv4_append", p(q), *_strides(q), p(k), *_strides(k), p(v), *_strides(v), p(q_out), *_strides(q_out),
-          p(cache), *_hstrides(cache), Lmax, B, T, HQ, hkv, *tab, *st, int(offset), *ln, *wts, float(eps), int(zq))
-    return q_out
+_NO_ROWS = (0,) * 9
 
 
 def append(cache, k, v, start, *, offset=0, lens=None):
     """Writes k, v (B, hkv, T, 128) bf16 into the cache (B, hkv, Lmax, 144): row i of request b at position
     start[b] + offset + i.  Rows i >= lens[b] (default T) and positions outside [0, Lmax) write nothing.
     Calls that write the same positions must be ordered (one stream, or events)."""
-    _append(cache, None, k, v, None, None, start, offset, lens, None, None, 0.0, None)
+    fc, dev = _cache(cache), cache.get_device()
+    fk, fv = _rows("k", k, torch.bfloat16), _rows("v", v, torch.bfloat16)
+    _same_device(dev, k=k, v=v)
+    _call(dev, "oa_kv4_append", *_NO_ROWS, *fk, *fv, *_NO_ROWS, *fc, 0, 0, 0, 0, *_index("start", start, dev),
+          *_index("lens", lens, dev), 0, 0, offset, _lib.OA_F32, 0, 0.0)
 
 
 def rope_append(cache, q, k, v, cos, sin, start, *, offset=0, lens=None, q_weight=None, k_weight=None, eps=1e-5,
@@ -85,36 +62,38 @@ def rope_append(cache, q, k, v, cos, sin, start, *, offset=0, lens=None, q_weigh
     writes the normalised, rotated k (rounded to bf16) and v into the cache.  Arguments as in those two; rows
     whose position is outside the tables or behind lens are padding (no record; q as in qk_norm_rope), rows at
     positions past the cache rotate q and write no record."""
-    if not isinstance(q, torch.Tensor):
-        raise RuntimeError("q must be a CUDA tensor")
-    return _append(cache, q, k, v, cos, sin, start, offset, lens, q_weight, k_weight, eps, q_out)
+    fc, dev, bf = _cache(cache), cache.get_device(), torch.bfloat16
+    fq, fk, fv = _rows("q", q, bf), _rows("k", k, bf), _rows("v", v, bf)
+    zero = q_out is None
+    if zero:
+        q_out = _like(q)
+    _same_device(dev, q=q, k=k, v=v, q_out=q_out)
+    qp, kp, wd = _weights(q_weight, k_weight, bf, dev)
+    _call(dev, "oa_kv4_append", *fq, *fk, *fv, *_rows("q_out", q_out, bf), *fc, *_table(cos, sin, dev),
+          *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, wd, zero, eps)
+    return q_out
 
 
 def unpack(cache, start, T, *, offset=0, lens=None, out_dtype=torch.bfloat16, k_out=None, v_out=None):
     """The values (k, v), each (B, hkv, T, 128) bf16 or fp32, of the records at positions start[b] + offset + i,
     i < T.  Rows i >= lens[b] and positions outside the cache are zero in outputs that this call allocates and
     left as they were in k_out / v_out."""
-    _cache(cache)
-    dev, (B, hkv, Lmax, _) = cache.device, cache.shape
-    if start is None:
-        raise RuntimeError("start must be given: the position of each request's first row")
+    fc, dev = _cache(cache), cache.get_device()
+    shape = (cache.shape[0], cache.shape[1], T, D)
+    _same_device(dev, k_out=k_out, v_out=v_out)
+    if k_out is not None or v_out is not None:
+        out_dtype = (v_out if k_out is None else k_out).dtype
     if T < 0 or out_dtype not in _CODE:
-        raise RuntimeError(f"T must be >= 0 and out_dtype bf16 or fp32, got {T}, {out_dtype}")
-    st, ln = _per_request("start", start, B, dev), _per_request("lens", lens, B, dev)
+        raise RuntimeError(f"T must be >= 0 and the outputs bf16 or fp32, got {T}, {out_dtype}")
     zk, zv = k_out is None, v_out is None
-    shape = torch.Size((B, hkv, T, D))
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is not None:
-            _same_device(dev, **{name: t})
-            out_dtype = t.dtype if t.dtype in _CODE else out_dtype
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is not None:
-            _out(name, t, out_dtype, shape)
-    k_out = torch.empty(shape, dtype=out_dtype, device=dev) if zk else k_out
-    v_out = torch.empty(shape, dtype=out_dtype, device=dev) if zv else v_out
-    p = _lib.ptr
-    _call(dev, "oa_kv4_unpack", p(cache), *_hstrides(cache), Lmax, *st, int(offset), *ln, p(k_out), *_strides(k_out),
-          p(v_out), *_strides(v_out), _CODE[out_dtype], B, T, hkv, int(zk), int(zv))
+    if zk:
+        k_out = torch.empty(shape, dtype=out_dtype, device=cache.device)
+    if zv:
+        v_out = torch.empty(shape, dtype=out_dtype, device=cache.device)
+    if k_out.shape != shape:
+        raise RuntimeError(f"k_out must be {shape}, got {tuple(k_out.shape)}")
+    _call(dev, "oa_kv4_unpack", *fc, *_rows("k_out", k_out, out_dtype), *_rows("v_out", v_out, out_dtype),
+          *_index("start", start, dev), *_index("lens", lens, dev), offset, _CODE[out_dtype], zk, zv)
     return k_out, v_out
 
 
@@ -126,6 +105,21 @@ def attention_workspace(B, HQ, T, cache_len, dev, hkv=HKV):
     can overlap on the GPU must not share one."""
     need = _lib.load().oa_kv4_attention_workspace_bytes(B, HQ, hkv, T, cache_len)
     return torch.zeros(need, dtype=torch.uint8, device=dev) if need else None
+
+
+def _workspace(dev, *sizes):
+    """The kept workspace of these sizes, one for each GPU and stream: calls on one stream run in order and may share
+    it.  A call that is being captured gets its own from the graph's pool, where its zero-fill is replayed too."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    key = (dev, _current_stream(dev), *sizes)
+    ws = None if capturing else _ws_cache.get(key)
+    if ws is None:
+        with torch.cuda.device(dev):
+            need = _lib.load().oa_kv4_attention_workspace_bytes(*sizes)
+        ws = torch.zeros(max(need, 16), dtype=torch.uint8, device=f"cuda:{dev}")
+        if not capturing:
+            _ws_cache[key] = ws
+    return ws
 
 
 def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, out=None, workspace=None):
@@ -140,40 +134,23 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
     workspace: attention_workspace(...) of the same sizes.  By default one is kept for each device, stream and
     size; a call that is being captured allocates its own from the graph's pool (graphs may then be replayed
     side by side), so a decode loop that captures many layers passes one."""
-    _rows("q", q, torch.bfloat16)
-    _cache(cache)
-    dev, (B, HQ, T, _) = q.device, q.shape
-    hkv, Lmax = cache.shape[1], cache.shape[2]
-    if cache.shape[0] != B or hkv < 1 or HQ < 1 or HQ % hkv:
-        raise RuntimeError(f"q holds {B} requests of {HQ} heads, the cache {cache.shape[0]} of {hkv}: need the same "
-                           "requests and a multiple of the KV heads")
-    _same_device(dev, cache=cache, out=out, workspace=workspace)
-    if n is None:
-        raise RuntimeError("n must be given: the length of each request")
-    ln = _per_request("n", n, B, dev)
-    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
-        raise RuntimeError("workspace must be a contiguous uint8 tensor")
+    fq, fc, dev = _rows("q", q, torch.bfloat16), _cache(cache), q.get_device()
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
-    elif out_dtype is not None and out_dtype != out.dtype:
-        raise RuntimeError(f"out is {out.dtype}, out_dtype {out_dtype}")
-    if out.dtype not in _CODE:
-        raise RuntimeError(f"the output must be bf16 or fp32, got {out.dtype}")
-    _out("out", out, out.dtype, q.shape)
-    need = _lib.load().oa_kv4_attention_workspace_bytes(B, HQ, hkv, T, Lmax)
-    if workspace is None and need:
-        if torch.cuda.is_current_stream_capturing():
-            workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
-        else:
-            key = (dev.index, torch.cuda.current_stream(dev).cuda_stream, B, HQ, hkv, T, Lmax)
-            workspace = _ws_cache.get(key)
-            if workspace is None:
-                workspace = _ws_cache[key] = torch.zeros(need, dtype=torch.uint8, device=dev)
-    p = _lib.ptr
-    _call(dev, "oa_kv4_attention", p(q), *_strides(q), p(cache), *_hstrides(cache), Lmax, *ln, int(offset), p(out),
-          *_strides(out), _CODE[out.dtype], B, HQ, hkv, T, float(D ** -0.5 if sm_scale is None else sm_scale),
-          p(workspace), 0 if workspace is None else workspace.numel())
+        out = _like(q) if out_dtype is None else torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    _same_device(dev, cache=cache, out=out, workspace=workspace)
+    dt = out.dtype
+    if dt not in _CODE or (out_dtype is not None and out_dtype != dt):
+        raise RuntimeError(f"the output must be bf16 or fp32 and out of type out_dtype, got {dt}, out_dtype {out_dtype}")
+    if workspace is None:
+        workspace = _workspace(dev, *fq[1:3], fc[2], fq[3], fc[3])
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise RuntimeError("workspace must be a contiguous uint8 tensor")
+    _call(dev, "oa_kv4_attention", *fq, *fc, *_rows("out", out, dt), *_index("n", n, dev), workspace.data_ptr(),
+          workspace.numel(), offset, _CODE[dt], D ** -0.5 if sm_scale is None else sm_scale)
     return out
+
+
+_NO_PROXIES, _NO_LOG = (0,) * 14, (0,) * 5
 
 
 def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, sm_scale=None, out_dtype=None,
@@ -185,44 +162,30 @@ def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, s
     is padding) and nb cluster proxies with logits q . kbar * sm_scale + log_n (log_n = -inf skips one).
     kbar, vbar bf16 (BQ, NB, 128) (for each query row) or (BH, NB, 128) (for each KV row), log_n (BQ, NB) fp32;
     nb = 0 disables the proxies.  A row with nothing to attend gives zeros."""
-    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype != torch.bfloat16 or q.dim() != 2 or \
-            q.shape[1] != D or q.stride(1) != 1:
-        raise RuntimeError("q must be a (rows, 128) bf16 CUDA tensor with a contiguous last dim")
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype is not torch.bfloat16 or q.dim() != 2:
+        raise RuntimeError("q must be a (rows, 128) bf16 CUDA tensor")
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("q requires a gradient: this operator has no backward pass (use torch.no_grad())")
-    _cache(cache, ndim=3)
-    dev, BQ = q.device, q.shape[0]
-    BH, Lmax, _ = cache.shape
-    if BH < 1 or BQ % BH:
-        raise RuntimeError(f"q's {BQ} rows must be a multiple of the cache's {BH}")
+    fc, dev = _cache(cache, ndim=3), q.get_device()
     _same_device(dev, cache=cache, sel_idx=sel_idx, exp_idx=exp_idx, out=out)
-    for name, t in (("sel_idx", sel_idx), ("exp_idx", exp_idx)):
-        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != BQ or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be a contiguous ({BQ}, n) int32 tensor, got {tuple(t.shape)} {t.dtype}")
+    if sel_idx.dtype is not torch.int32 or sel_idx.dim() != 2 or exp_idx.dtype is not torch.int32 or exp_idx.dim() != 2:
+        raise RuntimeError(f"sel_idx and exp_idx must be (rows, n) int32 tensors, got {tuple(sel_idx.shape)} {sel_idx.dtype} "
+                           f"and {tuple(exp_idx.shape)} {exp_idx.dtype}")
     NB = (0 if kbar is None else kbar.shape[1]) if nb is None else int(nb)
-    if NB < 0:
-        raise RuntimeError(f"nb must not be negative, got {NB}")
-    per_qhead, strides = 1, (0, 0)
+    fb, fl = _NO_PROXIES, _NO_LOG
     if NB > 0:
         _same_device(dev, kbar=kbar, vbar=vbar, log_n=log_n)
-        for name, t in (("kbar", kbar), ("vbar", vbar)):
-            if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[0] not in (BQ, BH) or t.shape[1] < NB or \
-                    t.shape[2] != D or t.stride(2) != 1 or t.shape != kbar.shape or t.stride() != kbar.stride():
-                raise RuntimeError(f"{name} must be ({BQ} or {BH}, >= {NB}, 128) bf16 with a contiguous last dim, kbar and "
-                                   f"vbar of one shape and strides; got {tuple(t.shape)} {t.dtype}")
-        if log_n.dtype != torch.float32 or log_n.dim() != 2 or log_n.shape[0] != BQ or log_n.shape[1] < NB or \
-                log_n.stride(1) != 1:
-            raise RuntimeError(f"log_n must be ({BQ}, >= {NB}) fp32 with a contiguous last dim, got {tuple(log_n.shape)}")
-        per_qhead = 1 if kbar.shape[0] == BQ else 0
-        strides = tuple(0 if m == 1 else s for m, s in zip(kbar.shape[:2], kbar.stride()[:2]))
+        if kbar is None or vbar is None or log_n is None or kbar.dtype is not torch.bfloat16 or kbar.dim() != 3 or \
+                vbar.dtype is not torch.bfloat16 or vbar.dim() != 3 or log_n.dtype is not torch.float32 or log_n.dim() != 2:
+            raise RuntimeError("kbar and vbar must be (rows, NB, 128) bf16 and log_n (rows, NB) fp32")
+        fb = (kbar.data_ptr(), *kbar.shape, *kbar.stride(), vbar.data_ptr(), *vbar.shape, *vbar.stride())
+        fl = (log_n.data_ptr(), *log_n.shape, *log_n.stride())
     if out is None:
-        out = torch.empty(BQ, D, dtype=out_dtype or q.dtype, device=dev)
-    if out.dtype not in _CODE or out.shape != (BQ, D) or out.stride(1) != 1 or (BQ > 1 and out.stride(0) < D) or \
-            (out_dtype is not None and out_dtype != out.dtype):
-        raise RuntimeError(f"out must be ({BQ}, 128) bf16 or fp32 rows, got {tuple(out.shape)} {out.dtype}")
-    p = _lib.ptr
-    _call(dev, "oa_kv4_flash", p(q), q.stride(0) if BQ > 1 else 0, p(cache), *_hstrides(cache), Lmax, p(sel_idx),
-          sel_idx.shape[1], p(exp_idx), exp_idx.shape[1], p(kbar) if NB else 0, p(vbar) if NB else 0, *strides, per_qhead,
-          p(log_n) if NB else 0, log_n.stride(0) if NB else 0, p(out), out.stride(0) if BQ > 1 else 0, _CODE[out.dtype],
-          BQ, BH, NB, float(D ** -0.5 if sm_scale is None else sm_scale))
+        out = _like(q) if out_dtype is None else torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    dt = out.dtype
+    if dt not in _CODE or out.dim() != 2 or (out_dtype is not None and out_dtype != dt):
+        raise RuntimeError(f"out must be (rows, 128) bf16 or fp32 of type out_dtype, got {tuple(out.shape)} {dt}")
+    _call(dev, "oa_kv4_flash", q.data_ptr(), *q.shape, *q.stride(), *fc, sel_idx.data_ptr(), *sel_idx.shape,
+          *sel_idx.stride(), exp_idx.data_ptr(), *exp_idx.shape, *exp_idx.stride(), *fb, *fl, out.data_ptr(), *out.shape,
+          *out.stride(), _CODE[dt], NB, D ** -0.5 if sm_scale is None else sm_scale)
     return out

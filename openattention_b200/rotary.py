@@ -14,77 +14,78 @@ from .geometry import D
 _CODE = {torch.bfloat16: _lib.OA_BF16, torch.float32: _lib.OA_F32}
 
 
-def _rows(name, t, dtype, shape=None):
-    """(B, heads, T, 128) rows whose last dim is contiguous, on CUDA; any other strides."""
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _bad_rows(name, t, dtype):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 4 or t.shape[3] != D or t.stride(3) != 1 or (shape is not None and t.shape != shape):
-        want = "(B, heads, T, 128)" if shape is None else tuple(shape)
-        raise RuntimeError(f"{name} must be {want} with a contiguous last dim, got {tuple(t.shape)}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (use torch.no_grad())")
+    if t.dim() != 4:
+        raise RuntimeError(f"{name} must be (B, heads, T, 128), got {tuple(t.shape)}")
+    raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (use torch.no_grad())")
+
+
+def _rows(name, t, dtype):
+    """The block's fields of (B, heads, T, 128) rows; sizes, strides and alignment are checked by the entry."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not dtype or t.dim() != 4 or \
+            (t.requires_grad and torch.is_grad_enabled()):
+        _bad_rows(name, t, dtype)
+    return t.data_ptr(), *t.shape, *t.stride()
 
 
 def _same_device(dev, **tensors):
     for name, t in tensors.items():
-        if t is not None and (not isinstance(t, torch.Tensor) or t.device != dev):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != dev):
             where = t.device if isinstance(t, torch.Tensor) else type(t).__name__
-            raise RuntimeError(f"{name} must be a tensor on {dev}, got {where}")
+            raise RuntimeError(f"{name} must be a tensor on cuda:{dev}, got {where}")
 
 
-def _strides(t):
-    """Strides of the first three dims; a dim of one element has none."""
+def _index(name, t, dev):
+    """The block's fields of one whole number for each request, or one for all."""
     if t is None:
-        return 0, 0, 0
-    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
-
-
-def _out(name, t, dtype, shape):
-    """An output's rows must not overlap each other (an expanded tensor would be written by several rows)."""
-    _rows(name, t, dtype, shape)
-    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
-        raise RuntimeError(f"{name} must not be an expanded tensor")
-
-
-def _per_request(name, t, B, dev):
-    """(pointer, stride, is_int64) of one whole number for each request, or one for all."""
-    if t is None:
-        return 0, 0, 0
-    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in (torch.int32, torch.int64) or t.dim() != 1 \
-            or t.shape[0] not in (1, B):
+        return 0, 0, 0, 0
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dim() != 1 or \
+            (t.dtype is not torch.int32 and t.dtype is not torch.int64):
         got = f"{tuple(t.shape)} {t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise RuntimeError(f"{name} must be ({B},) or (1,) int32 or int64 on {dev}, got {got}")
-    return t.data_ptr(), 0 if t.shape[0] == 1 else t.stride(0), 1 if t.dtype == torch.int64 else 0
+        raise RuntimeError(f"{name} must be (B,) or (1,) int32 or int64 on cuda:{dev}, got {got}")
+    return t.data_ptr(), t.shape[0], t.stride(0), t.dtype is torch.int64
 
 
 def _table(cos, sin, dev):
     for name, t in (("cos", cos), ("sin", sin)):
-        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.float32 or t.dim() != 2 or \
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype is not torch.float32 or t.dim() != 2 or \
                 not t.is_contiguous() or t.shape != cos.shape:
-            raise RuntimeError(f"{name} must be a contiguous fp32 (positions, rotated dims) table on {dev}, the same "
-                               "shape for both")
-    return cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.shape[1]
+            raise RuntimeError(f"{name} must be a contiguous fp32 (positions, rotated dims) table on cuda:{dev}, the "
+                               "same shape for both")
+    return cos.data_ptr(), sin.data_ptr(), *cos.shape
 
 
 def _weights(q_weight, k_weight, dtype, dev):
     """(q pointer, k pointer, dtype code) of the norm weights: both in the rows' type or both fp32."""
     given = [w for w in (q_weight, k_weight) if w is not None]
+    if not given:
+        return 0, 0, _lib.OA_F32
     for w in given:
-        if not isinstance(w, torch.Tensor) or w.device != dev or w.shape != (D,) or not w.is_contiguous() or \
+        if not isinstance(w, torch.Tensor) or w.get_device() != dev or w.shape != (D,) or not w.is_contiguous() or \
                 w.dtype not in (dtype, torch.float32) or w.dtype != given[0].dtype:
-            raise RuntimeError(f"norm weights must be contiguous ({D},) tensors on {dev}, both {dtype} or both fp32")
-    return _lib.ptr(q_weight), _lib.ptr(k_weight), _CODE[given[0].dtype] if given else _lib.OA_F32
+            raise RuntimeError(f"norm weights must be contiguous ({D},) tensors on cuda:{dev}, both {dtype} or both fp32")
+    return _lib.ptr(q_weight), _lib.ptr(k_weight), _CODE[given[0].dtype]
 
 
-def _call(dev, name, *args):
-    """_lib.call on the current stream of `dev` (a launch needs its stream's device to be current)."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _call(dev, name, *fields):
+    """_lib.call_block on the current stream of GPU `dev` (a launch needs its stream's device to be current)."""
+    if dev == _current_device():
+        _lib.call_block(name, _current_stream(dev), *fields)
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+            _lib.call_block(name, _current_stream(dev), *fields)
 
 
 def qk_norm_rope(q, k, cos, sin, start, *, offset=0, lens=None, q_weight=None, k_weight=None, eps=1e-5, q_out=None,
@@ -101,24 +102,14 @@ def qk_norm_rope(q, k, cos, sin, start, *, offset=0, lens=None, q_weight=None, k
     lens[b] (default T) rows of request b are real.  Rows behind them, and rows whose position is outside
     the table, are padding: they are zero in outputs that this call allocates and left as they were in
     q_out / k_out.  q_out may be q and k_out may be k (in place); otherwise outputs must not overlap inputs."""
-    _rows("q", q, q.dtype if getattr(q, "dtype", None) in _CODE else torch.bfloat16)
-    dev, (B, HQ, T, _) = q.device, q.shape
-    _rows("k", k, q.dtype, (B, k.shape[1], T, D) if isinstance(k, torch.Tensor) and k.dim() == 4 else None)
+    dt = torch.float32 if getattr(q, "dtype", None) is torch.float32 else torch.bfloat16
+    fq, fk = _rows("q", q, dt), _rows("k", k, dt)
+    dev, given = q.get_device(), (q_out is not None, k_out is not None)
+    q_out = q_out if given[0] else _like(q)
+    k_out = k_out if given[1] else _like(k)
     _same_device(dev, k=k, q_out=q_out, k_out=k_out)
-    tab = _table(cos, sin, dev)
-    st, ln = _per_request("start", start, B, dev), _per_request("lens", lens, B, dev)
-    wts = _weights(q_weight, k_weight, q.dtype, dev)
-    zq, zk = q_out is None, k_out is None
-    if zq:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    else:
-        _out("q_out", q_out, q.dtype, q.shape)
-    if zk:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-    else:
-        _out("k_out", k_out, k.dtype, k.shape)
-    p = _lib.ptr
-    _call(dev, "oa_qk_norm_rope", p(q), *_strides(q), p(k), *_strides(k), p(q_out), *_strides(q_out), p(k_out),
-          *_strides(k_out), _CODE[q.dtype], B, T, HQ, k.shape[1], *tab, *st, int(offset), *ln, *wts, float(eps),
-          int(zq), int(zk))
+    qp, kp, wd = _weights(q_weight, k_weight, dt, dev)
+    _call(dev, "oa_qk_norm_rope", *fq, *fk, *_rows("q_out", q_out, dt), *_rows("k_out", k_out, dt), *_table(cos, sin, dev),
+          *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, _CODE[dt], wd, not given[0],
+          not given[1], eps)
     return q_out, k_out

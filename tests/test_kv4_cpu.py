@@ -1,6 +1,7 @@
 """What the 4-bit cache operators and the rotation refuse, before any launch; and the definitions the GPU tests
 compare with, checked on the CPU."""
-import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -26,161 +27,158 @@ def test_wrappers_refuse_host_tensors():
 
 
 class _Fake(torch.Tensor):
-    """A host tensor that says it is on a GPU: the checks behind the device's own are reached without one."""
+    """A host tensor that says it is on a GPU."""
     is_cuda = True
 
 
 def _fake(t):
-    return t.as_subclass(_Fake)
+    return t.as_subclass(_Fake) if isinstance(t, torch.Tensor) else t
 
 
-@pytest.mark.parametrize("change,match", [
-    (dict(q=torch.zeros(1, 4, 2, D, dtype=torch.float16)), "q must be torch.bfloat16"),
-    (dict(q=torch.zeros(4, 2, D, dtype=BF)), "q must be"),
-    (dict(q=torch.zeros(1, 4, 2, 64, dtype=BF)), "q must be"),
-    (dict(q=torch.zeros(1, 4, D, 2, dtype=BF).transpose(2, 3)), "contiguous last dim"),
-    (dict(k=torch.zeros(1, 2, 3, D, dtype=BF)), "k must be"),
-    (dict(k=torch.zeros(1, 2, 2, D)), "k must be torch.bfloat16"),
-    (dict(start=torch.zeros(3, dtype=torch.int32)), "start must be"),
+@pytest.fixture
+def entry(monkeypatch):
+    """Lets wrappers reach the library with host tensors, which every call here must be refused before using: not
+    where a GPU could be given their addresses."""
+    if torch.cuda.is_available():
+        pytest.skip("host addresses are not passed on where there is a GPU")
+    for m in (rotary, kv4):
+        monkeypatch.setattr(m, "_current_stream", lambda dev: 0)
+    monkeypatch.setattr(rotary, "_current_device", lambda: -1)
+
+
+def _refused(call, base, change, match):
+    a = {**base, **change}
+    with pytest.raises(RuntimeError, match=match):
+        call(**{n: _fake(t) for n, t in a.items()})
+
+
+def _i(n=1, dtype=torch.int32):
+    return torch.zeros(n, dtype=dtype)
+
+
+def _r(*shape, dtype=BF):
+    return torch.zeros(*shape, D, dtype=dtype)
+
+
+def _c(*shape):
+    return torch.zeros(*shape, REC, dtype=torch.uint8)
+
+
+ROPE = [
+    (dict(q=_r(1, 4, 2, dtype=torch.float16)), "q must be torch.bfloat16"),
+    (dict(q=_r(4, 2)), "q must be"),
+    (dict(q=torch.zeros(1, 4, 2, 64, dtype=BF)), "q must be .* 128"),
+    (dict(q=torch.zeros(1, 4, D, D, dtype=BF).transpose(2, 3), k=_r(1, 2, D)), "contiguous last dim"),
+    (dict(q=torch.zeros(1 + 4 * 2 * 132, dtype=BF)[1:].view(1, 4, 2, 132)[..., :D]), "16-byte"),
+    (dict(k=_r(1, 2, 3)), "k must be"),
+    (dict(k=_r(2, 2, 2)), "k must be"),
+    (dict(k=_r(1, 2, 2, dtype=torch.float32)), "k must be torch.bfloat16"),
+    (dict(start=_i(3)), "start must hold 1"),
     (dict(start=torch.zeros(1)), "start must be"),
+    (dict(start=None), "start must be given"),
     (dict(start=0), "start must be"),
-    (dict(lens=torch.zeros(1, 1, dtype=torch.int32)), "lens must be"),
+    (dict(lens=_i(1).view(1, 1)), "lens must be"),
+    (dict(lens=_i(2)), "lens must hold"),
     (dict(cos=torch.zeros(8, 64)), "must be a contiguous fp32"),
+    (dict(cos=torch.zeros(8, 24), sin=torch.zeros(8, 24)), "multiple of 16"),
+    (dict(cos=torch.zeros(8, 144), sin=torch.zeros(8, 144)), "multiple of 16"),
     (dict(q_weight=torch.zeros(64)), "norm weights"),
     (dict(q_weight=torch.zeros(D), k_weight=torch.zeros(D, dtype=BF)), "norm weights"),
-    (dict(q_out=torch.zeros(1, 4, 2, D)), "q_out must be torch.bfloat16"),
-    (dict(q_out=torch.zeros(1, 1, 2, D, dtype=BF).expand(1, 4, 2, D)), "expanded"),
-])
-def test_rope_refusals(change, match):
-    a = dict(q=torch.zeros(1, 4, 2, D, dtype=BF), k=torch.zeros(1, 2, 2, D, dtype=BF), start=torch.zeros(1, dtype=torch.int32))
-    a["cos"], a["sin"] = P.table(8, 128)
-    a.update(change)
-    with pytest.raises(RuntimeError, match=match):
-        rotary.qk_norm_rope(**{n: _fake(t) if isinstance(t, torch.Tensor) else t for n, t in a.items()})
+    (dict(q_out=_r(1, 4, 2, dtype=torch.float32)), "q_out must be torch.bfloat16"),
+    (dict(q_out=_r(1, 4, 3)), "q_out must be"),
+    (dict(q_out=_r(1, 1, 2).expand(1, 4, 2, D)), "expanded"),
+    (dict(q=_r(1, 4, 2).requires_grad_()), "no backward pass"),
+]
 
 
-def test_gradients_are_refused():
-    q = _fake(torch.zeros(1, 4, 2, D, dtype=BF)).requires_grad_()
-    k = _fake(torch.zeros(1, 2, 2, D, dtype=BF))
+@pytest.mark.parametrize("change,match", ROPE)
+def test_rope_refusals(entry, change, match):
     cos, sin = P.table(8, 128)
-    with pytest.raises(RuntimeError, match="no backward pass"):
-        rotary.qk_norm_rope(q, k, cos, sin, torch.zeros(1, dtype=torch.int32))
-
-
-@pytest.mark.parametrize("cache,match", [
-    (torch.zeros(1, 2, 8, REC), "uint8"), (torch.zeros(1, 2, 8, 160, dtype=torch.uint8)[..., :REC], "contiguous records"),
-    (torch.zeros(2, 8, REC, dtype=torch.uint8), "cache must be"), (torch.zeros(1, 2, 8, 128, dtype=torch.uint8), "cache must be"),
-    (torch.zeros(1, 1, 8, REC, dtype=torch.uint8).expand(1, 2, 8, REC), "expanded")])
-def test_append_refuses_caches(cache, match):
-    k = _fake(torch.zeros(1, 2, 2, D, dtype=BF))
-    with pytest.raises(RuntimeError, match=match):
-        kv4.append(_fake(cache), k, k, _fake(torch.zeros(1, dtype=torch.int32)))
+    _refused(rotary.qk_norm_rope, dict(q=_r(1, 4, 2), k=_r(1, 2, 2), cos=cos, sin=sin, start=_i()), change, match)
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(cache=torch.zeros(2, 2, 8, REC, dtype=torch.uint8)), "same requests"),
-    (dict(cache=torch.zeros(1, 3, 8, REC, dtype=torch.uint8)), "multiple of the KV heads"),
-    (dict(n=None), "n must be given"), (dict(n=torch.zeros(2, dtype=torch.int32)), "n must be"),
-    (dict(out_dtype=torch.float16), "bf16 or fp32"), (dict(out=torch.zeros(1, 4, 1, D, dtype=BF)), "out must be"),
-    (dict(out=torch.zeros(1, 4, 2, D, dtype=BF), out_dtype=torch.float32), "out_dtype"),
-    (dict(workspace=torch.zeros(4)), "workspace")])
-def test_decode_attention_refusals(change, match):
-    a = dict(q=torch.zeros(1, 4, 2, D, dtype=BF), cache=torch.zeros(1, 2, 8, REC, dtype=torch.uint8),
-             n=torch.zeros(1, dtype=torch.int32))
-    a.update(change)
-    with pytest.raises(RuntimeError, match=match):
-        kv4.decode_attention(**{n: _fake(t) if isinstance(t, torch.Tensor) else t for n, t in a.items()})
+    (dict(cache=torch.zeros(1, 2, 8, REC)), "uint8"),
+    (dict(cache=torch.zeros(1, 2, 8, 160, dtype=torch.uint8)[..., :REC]), "contiguous records"),
+    (dict(cache=_c(2, 8)), "cache must be"), (dict(cache=torch.zeros(1, 2, 8, 128, dtype=torch.uint8)), "cache must be"),
+    (dict(cache=_c(1, 1, 8).expand(1, 2, 8, REC)), "expanded"), (dict(cache=_c(1, 3, 8)), "k must be"),
+    (dict(cache=torch.zeros(2 * 8 * REC + 8, dtype=torch.uint8)[8:].view(1, 2, 8, REC)), "16-byte"),
+    (dict(v=_r(1, 2, 3)), "v must be"), (dict(start=_i(4)), "start must hold"), (dict(start=None), "start must be given"),
+    (dict(lens=torch.zeros(1)), "lens must be")])
+def test_append_refusals(entry, change, match):
+    _refused(kv4.append, dict(cache=_c(1, 2, 8), k=_r(1, 2, 2), v=_r(1, 2, 2), start=_i()), change, match)
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(q=torch.zeros(4, D)), "q must be"), (dict(cache=torch.zeros(3, 8, REC, dtype=torch.uint8)), "multiple of the cache's"),
+    (dict(q=_r(1, 4, 3)), "q must be"), (dict(q=_r(1, 4, 2, dtype=torch.float32)), "q must be torch.bfloat16"),
+    (dict(cos=torch.zeros(8, 40), sin=torch.zeros(8, 40)), "multiple of 16"), (dict(k_weight=torch.zeros(3)), "norm weights"),
+    (dict(q_out=_r(1, 3, 2)), "q_out must be"), (dict(cache=_c(1, 1, 8).expand(1, 2, 8, REC)), "expanded")])
+def test_rope_append_refusals(entry, change, match):
+    cos, sin = P.table(8, 128)
+    _refused(kv4.rope_append, dict(cache=_c(1, 2, 8), q=_r(1, 4, 2), k=_r(1, 2, 2), v=_r(1, 2, 2), cos=cos, sin=sin,
+                                   start=_i()), change, match)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(T=-1), "T must be"), (dict(k_out=_r(1, 2, 3)), "k_out must be"), (dict(v_out=_r(1, 2, 3)), "v_out must be"),
+    (dict(k_out=_r(1, 2, 2, dtype=torch.float16)), "bf16 or fp32"), (dict(start=_i(5)), "start must hold"),
+    (dict(k_out=_r(1, 2, 2), v_out=_r(1, 2, 2, dtype=torch.float32)), "v_out must be torch.bfloat16"),
+    (dict(v_out=_r(1, 1, 2).expand(1, 2, 2, D)), "expanded")])
+def test_unpack_refusals(entry, change, match):
+    _refused(kv4.unpack, dict(cache=_c(1, 2, 8), start=_i(), T=2, k_out=_r(1, 2, 2), v_out=_r(1, 2, 2)), change, match)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(cache=_c(2, 2, 8)), "same requests"), (dict(cache=_c(1, 3, 8)), "multiple of the KV heads"),
+    (dict(cache=_c(1, 8, 8)), "multiple of the KV heads"), (dict(cache=_c(1, 0, 8)), "multiple of the KV heads"),
+    (dict(n=None), "n must be given"), (dict(n=_i(2)), "n must hold"), (dict(n=torch.zeros(1)), "n must be"),
+    (dict(out=_r(1, 4, 2, dtype=torch.float16)), "bf16 or fp32"), (dict(out=_r(1, 4, 1)), "out must be"),
+    (dict(out=_r(1, 4, 2), out_dtype=torch.float32), "out_dtype"),
+    (dict(out=_r(1, 1, 2).expand(1, 4, 2, D)), "expanded"),
+    (dict(workspace=torch.zeros(4)), "workspace must be"),
+    (dict(workspace=torch.zeros(64, dtype=torch.uint8)), "needs a 16-byte aligned workspace of"),
+    (dict(q=_r(1, 4, 2).requires_grad_()), "no backward pass")])
+def test_decode_attention_refusals(entry, change, match):
+    _refused(kv4.decode_attention, dict(q=_r(1, 4, 2), cache=_c(1, 2, 8), n=_i(), out=_r(1, 4, 2),
+                                        workspace=torch.zeros(16, dtype=torch.uint8)), change, match)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=_r(4, dtype=torch.float32)), "q must be"), (dict(q=torch.zeros(4, 64, dtype=BF)), r"\(4, 128\)"),
+    (dict(cache=_c(3, 8)), "multiple of the cache's"), (dict(cache=_c(1, 2, 8)), "cache must be"),
     (dict(sel_idx=torch.zeros(4, 2, dtype=torch.int64)), "sel_idx"), (dict(exp_idx=torch.zeros(3, 2, dtype=torch.int32)), "exp_idx"),
-    (dict(nb=9), "kbar must be"), (dict(nb=-1), "nb must not"), (dict(vbar=torch.zeros(4, 5, D, dtype=BF)), "vbar"),
-    (dict(log_n=torch.zeros(4, 4)), "log_n"), (dict(out=torch.zeros(4, 64)), "out must be")])
-def test_flash_attention_refusals(change, match):
+    (dict(exp_idx=torch.zeros(4, 4, dtype=torch.int32)[:, ::2]), "contiguous"),
+    (dict(nb=9), "kbar and vbar must be"), (dict(nb=-1), "bad list sizes"), (dict(vbar=_r(4, 5)), "kbar and vbar"),
+    (dict(kbar=_r(3, 6), vbar=_r(3, 6)), "kbar and vbar must be"), (dict(kbar=None, nb=2), "kbar must be|kbar and vbar"),
+    (dict(log_n=torch.zeros(4, 4)), "log_n"), (dict(out=torch.zeros(4, 64)), r"\(4, 128\)"),
+    (dict(out=_r(1).expand(4, D)), "overlap")])
+def test_flash_attention_refusals(entry, change, match):
     i = torch.zeros(4, 2, dtype=torch.int32)
-    a = dict(q=torch.zeros(4, D, dtype=BF), cache=torch.zeros(2, 8, REC, dtype=torch.uint8), sel_idx=i, exp_idx=i,
-             kbar=torch.zeros(4, 6, D, dtype=BF), vbar=torch.zeros(4, 6, D, dtype=BF), log_n=torch.zeros(4, 6))
-    a.update(change)
-    with pytest.raises(RuntimeError, match=match):
-        kv4.flash_attention(**{n: _fake(t) if isinstance(t, torch.Tensor) else t for n, t in a.items()})
+    _refused(kv4.flash_attention, dict(q=_r(4), cache=_c(2, 8), sel_idx=i, exp_idx=i, kbar=_r(4, 6), vbar=_r(4, 6),
+                                       log_n=torch.zeros(4, 6)), change, match)
 
 
-def _status(name, args, match):
-    lib = _lib.load()
-    assert getattr(lib, name)(*args) == 1
-    assert match in lib.oa_last_error_string(), lib.oa_last_error_string()
+def test_blocks_match_the_header():
+    """Each packed block has the size and the field kinds of the header's struct."""
+    src = open(os.path.join(os.path.dirname(__file__), "..", "include", "openattention_b200.h")).read()
+    src = re.sub(r"/\*.*?\*/", "", src, flags=re.S)
+    structs = {name: body for body, name in re.findall(r"typedef struct \{([^}]*)\} (\w+);", src)}
 
+    def fields(body):
+        out = ""
+        for decl in (d.strip() for d in body.split(";")):
+            if not decl:
+                continue
+            kind = re.match(r"(?:const )?(\w+)", decl).group(1)
+            for name in decl.split(","):
+                n = int((re.search(r"\[(\d)\]", name) or [0, 1])[1])
+                out += fields(structs[kind]) * n if kind in structs else ("d" if kind == "double" else "q") * n
+        return out
 
-def test_c_entries_check_their_arguments():
-    """Status 1 and a message, before any device work (the pointers are host addresses)."""
-    buf = ctypes.create_string_buffer(4096)
-    a = (ctypes.addressof(buf) + 255) // 256 * 256
-    f = ctypes.c_float
-
-    def rope(q=a, sb=0, R=128, dtype=0, B=1, HKV=1, start=a, cos=a, w=0):
-        return (q, sb, 0, 0, a, 0, 0, 0, a, 0, 0, 0, a, 0, 0, 0, dtype, B, 1, 1, HKV, cos, a, 8, R, start, 0, 0, 0, 0, 0, 0, w, 0,
-                1, f(1e-5), 0, 0, None)
-
-    _status("oa_qk_norm_rope", rope(R=24), b"multiple of 16")
-    _status("oa_qk_norm_rope", rope(R=144), b"multiple of 16")
-    _status("oa_qk_norm_rope", rope(dtype=7), b"dtype")
-    _status("oa_qk_norm_rope", rope(q=a + 2), b"16-byte")
-    _status("oa_qk_norm_rope", rope(q=0), b"null rows")
-    _status("oa_qk_norm_rope", rope(sb=4), b"16-byte")
-    _status("oa_qk_norm_rope", rope(HKV=0), b"bad sizes")
-    _status("oa_qk_norm_rope", rope(B=-1), b"bad sizes")
-    _status("oa_qk_norm_rope", rope(start=0), b"null start")
-    _status("oa_qk_norm_rope", rope(cos=a + 4), b"cos/sin")
-    _status("oa_qk_norm_rope", rope(w=a + 2), b"weights")
-
-    def append(k=a, cache=a, c_sb=0, HQ=0, cos=0, Lmax=4, start=a):
-        return (0, 0, 0, 0, k, 0, 0, 0, a, 0, 0, 0, 0, 0, 0, 0, cache, c_sb, 0, Lmax, 1, 1, HQ, 1, cos, cos, 4, 128, start, 0, 0, 0,
-                0, 0, 0, 0, 0, 1, f(0), 0, None)
-
-    _status("oa_kv4_append", append(k=0), b"null rows")
-    _status("oa_kv4_append", append(cache=0), b"cache")
-    _status("oa_kv4_append", append(cache=a + 8), b"cache")
-    _status("oa_kv4_append", append(c_sb=8), b"strides")
-    _status("oa_kv4_append", append(Lmax=-1), b"cache length")
-    _status("oa_kv4_append", append(HQ=1), b"cos/sin")
-    _status("oa_kv4_append", append(HQ=1, cos=a), b"null rows")
-    _status("oa_kv4_append", append(start=0), b"null start")
-
-    def unpack(cache=a, out=a, st=128, dtype=0, T=1):
-        return (cache, 0, 0, 4, a, 0, 0, 0, 0, 0, 0, out, 0, 0, st, out, 0, 0, 128, dtype, 1, T, 1, 0, 0, None)
-
-    _status("oa_kv4_unpack", unpack(cache=a + 1), b"cache")
-    _status("oa_kv4_unpack", unpack(out=0), b"null rows")
-    _status("oa_kv4_unpack", unpack(st=6), b"16-byte")
-    _status("oa_kv4_unpack", unpack(dtype=3), b"dtype")
-    _status("oa_kv4_unpack", unpack(T=-1), b"bad sizes")
-
-    def dense(q=a, cache=a, n=a, HQ=4, HKV=2, out=a, dtype=0, c_sh=144, B=1):
-        return (q, 0, 0, 0, cache, 0, c_sh, 64, n, 0, 0, 0, out, 0, 128, 0, dtype, B, HQ, HKV, 1, f(1), 0, 0, None)
-
-    _status("oa_kv4_attention", dense(HQ=5), b"multiple of HKV")
-    _status("oa_kv4_attention", dense(HKV=0), b"multiple of HKV")
-    _status("oa_kv4_attention", dense(B=-1), b"B, T >= 0")
-    _status("oa_kv4_attention", dense(cache=a + 8), b"16 bytes")
-    _status("oa_kv4_attention", dense(c_sh=100), b"16 bytes")
-    _status("oa_kv4_attention", dense(n=0), b"null q/out/n")
-    _status("oa_kv4_attention", dense(q=a + 8), b"16-byte")
-    _status("oa_kv4_attention", dense(dtype=2), b"out_dtype")
-
-    def lists(q=a, BQ=4, BH=2, sel=a, NB=0, kbar=0, qs=128, n_exp=0, dtype=1, Lmax=8):
-        return (q, qs, a, 8 * REC, Lmax, sel, 1, 0, n_exp, kbar, kbar, 0, 0, 1, kbar, 0, a, 128, dtype, BQ, BH, NB, f(1), None)
-
-    _status("oa_kv4_flash", lists(BQ=3), b"multiple of BH")
-    _status("oa_kv4_flash", lists(BH=0), b"multiple of BH")
-    _status("oa_kv4_flash", lists(sel=0), b"null index list")
-    _status("oa_kv4_flash", lists(n_exp=2), b"null index list")
-    _status("oa_kv4_flash", lists(NB=2), b"null kbar")
-    _status("oa_kv4_flash", lists(NB=2, kbar=a + 2), b"kbar/vbar")
-    _status("oa_kv4_flash", lists(qs=4), b"16-byte")
-    _status("oa_kv4_flash", lists(q=0), b"null q")
-    _status("oa_kv4_flash", lists(dtype=5), b"out_dtype")
-    _status("oa_kv4_flash", lists(Lmax=-1), b"bad list sizes")
+    for name, block in _lib.BLOCKS.items():
+        flat = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([qd])", block.format))
+        assert flat == fields(structs[name + "_args"]), name
+        assert _lib.load()[name](None, None) == 1 and b"null arguments" in _lib.load().oa_last_error_string()
 
 
 def test_plain_record_round_trip():
