@@ -10,9 +10,6 @@
 namespace oa {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kHalfWarps = kThreads / 16;
-
 struct DenseArgs {
   Rows q, o;
   const unsigned char* cache;
@@ -45,67 +42,16 @@ struct ListArgs {
   float qk_scale;
 };
 
-// One half-warp's online softmax; lane hl holds dims 4hl..4hl+3 (i < 4) and 64 + 4hl.. (i >= 4).
-struct State {
-  float q[8], acc[8], m, l;
-  __device__ __forceinline__ void init(const __nv_bfloat16* qp, int hl) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      q[i] = __bfloat162float(qp[(i < 4 ? 4 * hl + i : 64 + 4 * hl + i - 4)]);
-      acc[i] = 0.f;
-    }
-    m = -INFINITY;
-    l = 0.f;
-  }
-  __device__ __forceinline__ void add(const float (&k)[8], const float (&v)[8], float scale, float bias, unsigned hmask) {
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) d = fmaf(q[i], k[i], d);
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) d += __shfl_xor_sync(hmask, d, o);
-    const float z = fmaf(d, scale, bias);
-    const float mx = fmaxf(m, z);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    const float al = exp2f(m - base), p = exp2f(z - base);
-    l = fmaf(l, al, p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(acc[i], al, p * v[i]);
-    m = mx;
-  }
-};
-
-__device__ __forceinline__ void record_side(const unsigned char* rec, int side, int hl, float (&x)[8]) {
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + kRecV * side + 4 * hl);
-  const uint2 mt = *reinterpret_cast<const uint2*>(rec + kRecMeta + 8 * side);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = fmaf(bf_lo(mt.x), (float)((w >> (8 * i)) & 15u), bf_hi(mt.x));
-    x[4 + i] = fmaf(bf_lo(mt.y), (float)((w >> (8 * i + 4)) & 15u), bf_hi(mt.y));
-  }
+__device__ __forceinline__ void unpack8(const uint4& w, float* f) {
+  f[0] = bf_lo(w.x); f[1] = bf_hi(w.x); f[2] = bf_lo(w.y); f[3] = bf_hi(w.y);
+  f[4] = bf_lo(w.z); f[5] = bf_hi(w.z); f[6] = bf_lo(w.w); f[7] = bf_hi(w.w);
 }
-
-__device__ __forceinline__ void merge_store(const State& s, int hw, int hl, void* out, int64_t at, int f32) {
-  __shared__ float s_m[kHalfWarps], s_l[kHalfWarps], s_acc[kHalfWarps][kD];
-  if (hl == 0) {
-    s_m[hw] = s.m;
-    s_l[hw] = s.l;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s_acc[hw][i < 4 ? 4 * hl + i : 64 + 4 * hl + i - 4] = s.acc[i];
-  __syncthreads();
-  float M = -INFINITY, L = 0.f, A = 0.f;
-  for (int h = 0; h < kHalfWarps; ++h) M = fmaxf(M, s_m[h]);
-  const float base = M == -INFINITY ? 0.f : M;
-  for (int h = 0; h < kHalfWarps; ++h) {
-    const float w = exp2f(s_m[h] - base);
-    L = fmaf(w, s_l[h], L);
-    A = fmaf(w, s_acc[h][threadIdx.x], A);
-  }
+__device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, float A, float L) {
   const float o = L == 0.f ? 0.f : A / L;
-  if (f32)
-    static_cast<float*>(out)[at + threadIdx.x] = o;
+  if (a.out_f32)
+    static_cast<float*>(a.out)[r * a.out_stride + d] = o;
   else
-    static_cast<__nv_bfloat16*>(out)[at + threadIdx.x] = __float2bfloat16_rn(o);
+    static_cast<__nv_bfloat16*>(a.out)[r * a.out_stride + d] = __float2bfloat16_rn(o);
 }
 
 // ---------------------------------------------------------------- dense
@@ -579,36 +525,233 @@ __global__ void __launch_bounds__(1024) dense_merge_kernel(const DenseArgs a, co
   store_out4(const_cast<void*>(a.o.p), a.out_f32, b * a.o.sb + (int64_t)(kvh * G + hh) * a.o.sh + tt * a.o.st, lane, A, L);
 }
 
-__global__ void __launch_bounds__(kThreads) list_kernel(const ListArgs a) {
-  const int lane = threadIdx.x & 31, hl = lane & 15, hw = threadIdx.x >> 4;
-  const unsigned hmask = 0xffffu << (lane & 16);
-  const int64_t r = blockIdx.x;
-  const int64_t kvh = r / a.G;
+// ---------------------------------------------------------------- index lists and proxies
+// A row's entries (sel, then exp) are taken in tiles of 32, its proxies one per half-warp, by the W warps of a CTA
+// or, where rows are few, of a cluster of CTAs.  The 144-byte records of a tile are gathered into shared memory by
+// asynchronous copies (a record's nine 16-byte chunks go to neighbouring lanes) and the valid ones packed to the
+// front, so a tile is masked by a count.  A list belongs to one query row: one of the MMA's query columns is
+// used, which is still less work than unpacking codes to fp32 for plain FMAs (384 instructions a tile of 32
+// against about 770 on the same pipes).  Proxies are bf16 rows and stay on fp32 FMAs, while the gathers land.
+// Partial states: two half-warps and one MMA state per warp, merged in shared memory, then over the cluster.
+// stages of a warp's ring: with eight warps in a CTA, two CTAs share an SM only if they hold two
+template <int W>
+constexpr int list_stages() { return W == 8 ? 2 : 3; }
+constexpr int kStates = 3;  // per warp
+constexpr int kStateFloats = kD + 4;
+
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int W>
+constexpr size_t list_smem() {
+  return (size_t)W * (list_stages<W>() * kTileBytes + kStates * kStateFloats * sizeof(float));
+}
+
+template <int W>
+__global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, int S) {
+  constexpr int kListStages = list_stages<W>();
+  extern __shared__ __align__(16) unsigned char s_dyn[];  // [warp][stage][tile], then the states
+  __shared__ int s_idx[W][32];
+  __shared__ int s_cnt[W][kListStages];
+  __shared__ float s_cta[kD + 2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = S > 1 ? blockIdx.x % S : 0;
+  const int64_t r = blockIdx.x / S, kvh = r / a.G;
+  const int wi = rank * W + warp, nw = W * S;
+  const int total = a.n_sel + a.n_exp, tiles = (total + kTile - 1) / kTile;
   const unsigned char* base = a.cache + kvh * a.c_sh;
-  State s;
-  s.init(a.q + r * a.q_stride, hl);
-  for (int j = hw; j < a.n_sel + a.n_exp; j += kHalfWarps) {
-    const int t = j < a.n_sel ? a.sel[r * a.n_sel + j] : a.exp[r * a.n_exp + (j - a.n_sel)];
-    if (t < 0 || (int64_t)t >= a.Lmax) continue;
-    float k[8], v[8];
-    record_side(base + (int64_t)t * kRec, 0, hl, k);
-    record_side(base + (int64_t)t * kRec, 1, hl, v);
-    s.add(k, v, a.qk_scale, 0.f, hmask);
-  }
-  const int64_t pr = a.per_qhead ? r : kvh;
-  for (int j = hw; j < a.NB; j += kHalfWarps) {
-    const float ln = a.logn[r * a.ln_stride + j];
-    if (ln == -INFINITY) continue;
-    float k[8], v[8];
+  const uint32_t ring = smem_u32(s_dyn) + warp * (kListStages * kTileBytes);
+  float* s_state = reinterpret_cast<float*>(s_dyn + W * (kListStages * kTileBytes)) + warp * (kStates * kStateFloats);
+
+  auto entry = [&](int j) {  // the lane's index of tile j
+    const int e = j * kTile + lane;
+    if (j >= tiles || e >= total) return -1;
+    return e < a.n_sel ? a.sel[r * a.n_sel + e] : a.exp[r * a.n_exp + (e - a.n_sel)];
+  };
+  auto gather = [&](int t, int stage) {  // t: entry() of the tile
+    const bool ok = t >= 0 && (int64_t)t < a.Lmax;
+    const unsigned in = __ballot_sync(0xffffffffu, ok);
+    if (ok) s_idx[warp][__popc(in & ((1u << lane) - 1u))] = t;
+    if (lane == 0) s_cnt[warp][stage] = __popc(in);
+    __syncwarp();
+    const int chunks = 9 * __popc(in);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = i < 4 ? 4 * hl + i : 64 + 4 * hl + i - 4;
-      k[i] = __bfloat162float(a.kbar[pr * a.kb_sh + j * a.kb_sb + d]);
-      v[i] = __bfloat162float(a.vbar[pr * a.kb_sh + j * a.kb_sb + d]);
+    for (int i = 0; i < 9; ++i) {
+      const int c = lane + 32 * i, rec = c / 9;
+      if (c < chunks) cp_async16(ring + stage * kTileBytes + 16 * c, base + (int64_t)s_idx[warp][rec] * kRec + 16 * (c - 9 * rec));
     }
-    s.add(k, v, a.qk_scale, ln * kLog2e, hmask);
+    __syncwarp();
+  };
+  int first[kListStages];
+#pragma unroll
+  for (int i = 0; i < kListStages; ++i) first[i] = entry(wi + i * nw);
+
+  // ---- proxies: half-warp h of the row's 2 nw takes h, h + 2 nw, ...; lane hl dims 8 hl .. 8 hl + 7
+  {
+    constexpr int kUnroll = 4;
+    const int hl = lane & 15;
+    const unsigned hmask = 0xffffu << (lane & 16);
+    const int64_t pr = (a.per_qhead ? r : kvh) * a.kb_sh;
+    float qf[8], acc[8], m = -INFINITY, l = 0.f;
+    unpack8(*reinterpret_cast<const uint4*>(a.q + r * a.q_stride + 8 * hl), qf);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    bool started = false;
+    for (int j0 = 2 * wi + (lane >> 4); j0 - (lane >> 4) < a.NB || !started; j0 += 2 * nw * kUnroll) {
+      uint4 kw[kUnroll], vw[kUnroll];
+      float bias[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int j = j0 + 2 * nw * u;
+        bias[u] = j < a.NB ? a.logn[r * a.ln_stride + j] * kLog2e : -INFINITY;
+        kw[u] = vw[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (!(bias[u] == -INFINITY)) {
+          kw[u] = ldg_stream(a.kbar + pr + j * a.kb_sb + 8 * hl);
+          vw[u] = ldg_stream(a.vbar + pr + j * a.kb_sb + 8 * hl);
+        }
+      }
+      if (!started) {  // the records' copies go out behind the first proxies' loads
+        started = true;
+#pragma unroll
+        for (int i = 0; i < kListStages - 1; ++i) {
+          gather(first[i], i);
+          cp_async_commit();
+        }
+      }
+      float z[kUnroll], mx = m;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float kf[8], d = 0.f;
+        unpack8(kw[u], kf);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d = fmaf(qf[i], kf[i], d);
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) d += __shfl_xor_sync(hmask, d, o);
+        z[u] = bias[u] == -INFINITY ? -INFINITY : fmaf(d, a.qk_scale, bias[u]);
+        mx = fmaxf(mx, z[u]);
+      }
+      const float bm = biased(mx), al = ex2(m - bm);
+      m = mx;
+      l *= al;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= al;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const float p = ex2(z[u] - bm);
+        float vf[8];
+        unpack8(vw[u], vf);
+        l += p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(p, vf[i], acc[i]);
+      }
+    }
+    float* st = s_state + (lane >> 4) * kStateFloats;
+    reinterpret_cast<float4*>(st)[2 * hl] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    reinterpret_cast<float4*>(st)[2 * hl + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    if (hl == 0) {
+      st[kD] = m;
+      st[kD + 1] = l;
+    }
   }
-  merge_store(s, hw, hl, a.out, r * a.out_stride, a.out_f32);
+
+  // ---- records
+  WarpAttention<true> at;
+  at.lane_addresses();
+  at.load_q(at.op_col() == 0 ? a.q + r * a.q_stride : nullptr);
+  at.begin(a.qk_scale);
+  int stage = 0, ahead = first[kListStages - 1];
+  for (int j = wi; j < tiles; j += nw) {
+    // tile j + 2 nw goes out; the index after it is asked for
+    const int t = ahead;
+    ahead = entry(j + kListStages * nw);
+    gather(t, stage == 0 ? kListStages - 1 : stage - 1);
+    cp_async_commit();
+    cp_async_wait<kListStages - 1>();
+    __syncwarp();
+    const int cnt = s_cnt[warp][stage];
+    const int lim[2] = {cnt, cnt};
+    if (cnt == kTile)
+      at.tile<false>(ring + stage * kTileBytes, lim);
+    else if (cnt > 0)
+      at.tile<true>(ring + stage * kTileBytes, lim);
+    __syncwarp();
+    stage = stage + 1 == kListStages ? 0 : stage + 1;
+  }
+  cp_async_wait<0>();
+  at.finish(s_state + 2 * kStateFloats, s_state + 2 * kStateFloats + kD, 1);
+  __syncthreads();
+
+  // ---- merge the CTA's states, then the cluster's
+  const float* st = reinterpret_cast<const float*>(s_dyn + W * (kListStages * kTileBytes));
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < W * kStates; ++i) M = fmaxf(M, st[i * kStateFloats + kD]);
+  float f[W * kStates];
+#pragma unroll
+  for (int i = 0; i < W * kStates; ++i) {
+    f[i] = ex2(st[i * kStateFloats + kD] - biased(M));
+    L = fmaf(f[i], st[i * kStateFloats + kD + 1], L);
+  }
+  for (int d = tid; d < kD; d += 32 * W) {
+    float A = 0.f;
+#pragma unroll
+    for (int i = 0; i < W * kStates; ++i) A = fmaf(f[i], st[i * kStateFloats + d], A);
+    if (S == 1)
+      store_list(a, r, d, A, L);
+    else
+      s_cta[d] = A;
+  }
+  if (S == 1) return;
+  if (tid == 0) {
+    s_cta[kD] = M;
+    s_cta[kD + 1] = L;
+  }
+  cluster_sync();
+  if (rank == 0) {
+    M = -INFINITY;
+    for (int k = 0; k < S; ++k) M = fmaxf(M, ld_cluster(cluster_addr(s_cta + kD, k)));
+    L = 0.f;
+    for (int k = 0; k < S; ++k)
+      L = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - biased(M)), ld_cluster(cluster_addr(s_cta + kD + 1, k)), L);
+    for (int d = tid; d < kD; d += 32 * W) {
+      float A = 0.f;
+      for (int k = 0; k < S; ++k)
+        A = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - biased(M)), ld_cluster(cluster_addr(s_cta + d, k)), A);
+      store_list(a, r, d, A, L);
+    }
+  }
+  cluster_sync();  // no CTA leaves while its state is read
+}
+
+template <int W>
+int launch_list(const ListArgs& a, int64_t rows, int S, const char* fn, cudaStream_t st) {
+  const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(&list_kernel<W>), list_smem<W>(), fn, true);
+  if (rc != OA_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * S));
+  cfg.blockDim = dim3(32 * W);
+  cfg.dynamicSmemBytes = list_smem<W>();
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)S;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, &list_kernel<W>, a, S);
+  if (e != cudaSuccess) return oa_fail(OA_ERR_CUDA, "%s: %s", fn, cudaGetErrorString(e));
+  return oa_check_launch(fn);
 }
 
 // the hand-out counter, then every row's spread
@@ -739,6 +882,17 @@ extern "C" int oa_kv4_flash(const oa_kv4_flash_args* args, void* stream) {
   a.out_f32 = g.out_dtype == OA_F32;
   a.G = (int)(BQ / BH);
   a.qk_scale = (float)(g.sm_scale * (double)oa::kLog2e);
-  oa::list_kernel<<<(unsigned)BQ, oa::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return oa_check_launch(fn);
+  // Warps per row: enough that all rows together fill the GPU's 16 warps per SM, but a tile (or eight proxies)
+  // each; up to 8 in a CTA, beyond that a cluster of CTAs.  Two at least: 64 threads write the row.
+  const int64_t fill = 148 * 16 / BQ, work = (n_sel + n_exp + oa::kTile - 1) / oa::kTile + (NB + 7) / 8;
+  const int64_t warps = std::min(fill, work);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (warps >= 16) {
+    const int S = warps >= 64 ? 8 : warps >= 32 ? 4 : 2;
+    OA_REQUIRE(BQ * S <= 0x7fffffff, "%s: too many rows", fn);
+    return oa::launch_list<8>(a, BQ, S, fn, st);
+  }
+  if (warps >= 8) return oa::launch_list<8>(a, BQ, 1, fn, st);
+  if (warps >= 4) return oa::launch_list<4>(a, BQ, 1, fn, st);
+  return oa::launch_list<2>(a, BQ, 1, fn, st);
 }
