@@ -61,6 +61,10 @@ __device__ __forceinline__ void cp_async_wait_all() {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {  // dst: shared-space address
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// 16 zero bytes where `live` is false (src is then not read)
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
 // in groups: close a group of this thread's copies; wait until at most N younger groups are unfinished
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

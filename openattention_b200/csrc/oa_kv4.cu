@@ -108,6 +108,8 @@ __device__ __forceinline__ int dense_len(const DenseArgs& a, int64_t b) {
   const int64_t n = min(per_request(a.n, b) + a.offset, a.Lmax);
   return n < 0 ? 0 : (int)n;
 }
+// the lowest n bits (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 // a row without records still has its zeros to write: one (empty) tile
 __device__ __forceinline__ int dense_tiles(int n) { return n <= kTile ? 1 : (int)(((unsigned)n + kTile - 1) / kTile); }
 
@@ -389,11 +391,11 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
       cp_async_wait<kStages - 2>();
       __syncwarp();
       if ((k + 1) * kTile <= whole) {
-        const int none[2] = {kTile, kTile};
-        at.template tile<false>(ring + stage * kStageBytes, none);
+        const uint32_t all[2] = {~0u, ~0u};
+        at.template tile<false>(ring + stage * kStageBytes, all);
       } else {
-        const int lim[2] = {max(0, min(kTile, sees[0] - k * kTile)), max(0, min(kTile, sees[1] - k * kTile))};
-        at.template tile<true>(ring + stage * kStageBytes, lim);
+        const uint32_t in[2] = {first_bits(sees[0] - k * kTile), first_bits(sees[1] - k * kTile)};
+        at.template tile<true>(ring + stage * kStageBytes, in);
       }
       __syncwarp();
       if (k + (kStages - 1) * kWarps < t1) fetch(n - (k + (kStages - 1) * kWarps) * kTile, stage == 0 ? kStages - 1 : stage - 1);
@@ -526,18 +528,15 @@ __global__ void __launch_bounds__(1024) dense_merge_kernel(const DenseArgs a, co
 }
 
 // ---------------------------------------------------------------- index lists and proxies
-// A row's entries (sel, then exp) are taken in tiles of 32, its proxies one per half-warp, by the W warps of a CTA
-// or, where rows are few, of a cluster of CTAs.  The 144-byte records of a tile are gathered into shared memory by
-// asynchronous copies (a record's nine 16-byte chunks go to neighbouring lanes) and the valid ones packed to the
-// front, so a tile is masked by a count.  A list belongs to one query row: one of the MMA's query columns is
-// used, which is still less work than unpacking codes to fp32 for plain FMAs (384 instructions a tile of 32
-// against about 770 on the same pipes).  Proxies are bf16 rows and stay on fp32 FMAs, while the gathers land.
-// Partial states: two half-warps and one MMA state per warp, merged in shared memory, then over the cluster.
-// stages of a warp's ring: with eight warps in a CTA, two CTAs share an SM only if they hold two
-template <int W>
-constexpr int list_stages() { return W == 8 ? 2 : 3; }
-constexpr int kStates = 3;  // per warp
-constexpr int kStateFloats = kD + 4;
+// A row's work is a line of items of about 4 KB: its entries (sel, then exp) in tiles of 32 records, then its proxies
+// in tiles of 8 bf16 row pairs.  The W warps of a CTA or, where rows are few, of a cluster of CTAs take them in
+// turn, each with a ring of three: asynchronous copies fetch two items ahead (records three to an instruction,
+// nine 16-byte chunks each), the indices and log counts of a third are asked for.  Padding entries and skipped
+// proxies are masked by a bit and not fetched.  A list belongs to one query row: one of the MMA's query columns is
+// used, which is still less work than unpacking codes to fp32 for plain FMAs (a tile of 32 takes some 350
+// instructions, against about 770 on the same pipes).  The warps' states are merged in shared memory, then over the
+// cluster.
+constexpr int kRowsPerTile = 8;
 
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   uint32_t r;
@@ -554,159 +553,118 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 template <int W>
-constexpr size_t list_smem() {
-  return (size_t)W * (list_stages<W>() * kTileBytes + kStates * kStateFloats * sizeof(float));
-}
+constexpr size_t list_smem() { return (size_t)W * kStages * kTileBytes; }
 
 template <int W>
 __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, int S) {
-  constexpr int kListStages = list_stages<W>();
-  extern __shared__ __align__(16) unsigned char s_dyn[];  // [warp][stage][tile], then the states
-  __shared__ int s_idx[W][32];
-  __shared__ int s_cnt[W][kListStages];
+  extern __shared__ __align__(16) unsigned char s_dyn[];  // [warp][stage][item]; a warp's state when it is done
   __shared__ float s_cta[kD + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = S > 1 ? blockIdx.x % S : 0;
   const int64_t r = blockIdx.x / S, kvh = r / a.G;
-  const int wi = rank * W + warp, nw = W * S;
-  const int total = a.n_sel + a.n_exp, tiles = (total + kTile - 1) / kTile;
-  const unsigned char* base = a.cache + kvh * a.c_sh;
-  const uint32_t ring = smem_u32(s_dyn) + warp * (kListStages * kTileBytes);
-  float* s_state = reinterpret_cast<float*>(s_dyn + W * (kListStages * kTileBytes)) + warp * (kStates * kStateFloats);
+  const int nw = W * S, total = a.n_sel + a.n_exp;
+  const int tiles = (total + kTile - 1) / kTile, items = tiles + (a.NB + kRowsPerTile - 1) / kRowsPerTile;
+  const uint32_t ring = smem_u32(s_dyn) + warp * (kStages * kTileBytes);
 
-  auto entry = [&](int j) {  // the lane's index of tile j
-    const int e = j * kTile + lane;
-    if (j >= tiles || e >= total) return -1;
-    return e < a.n_sel ? a.sel[r * a.n_sel + e] : a.exp[r * a.n_exp + (e - a.n_sel)];
+  // what an item's copies wait for: the lane's index (-1: none), or its proxy's log count (-inf: none)
+  auto ask = [&](int j) {
+    int v = -1;
+    if (j < tiles) {
+      const int e = j * kTile + lane;
+      if (e < total) v = e < a.n_sel ? a.sel[r * a.n_sel + e] : a.exp[r * a.n_exp + (e - a.n_sel)];
+    } else if (j < items) {
+      const int e = (j - tiles) * kRowsPerTile + lane;
+      v = __float_as_int(lane < kRowsPerTile && e < a.NB ? a.logn[r * a.ln_stride + e] : -INFINITY);
+    }
+    return v;
   };
-  auto gather = [&](int t, int stage) {  // t: entry() of the tile
-    const bool ok = t >= 0 && (int64_t)t < a.Lmax;
-    const unsigned in = __ballot_sync(0xffffffffu, ok);
-    if (ok) s_idx[warp][__popc(in & ((1u << lane) - 1u))] = t;
-    if (lane == 0) s_cnt[warp][stage] = __popc(in);
-    __syncwarp();
-    const int chunks = 9 * __popc(in);
+  const int third = lane / 9;  // lanes 27..31 have no part in a record
+  const unsigned char* rec = a.cache + kvh * a.c_sh + 16 * (lane - 9 * third);
+  const int64_t prow = (a.per_qhead ? r : kvh) * a.kb_sh + 8 * (lane & 15);
+  auto fetch = [&](int j, int v, int stage) {  // starts an item's copies; returns its live entries
+    const uint32_t dst = ring + stage * kTileBytes;
+    uint32_t in = 0u;
+    if (j < tiles) {
+      in = __ballot_sync(0xffffffffu, v >= 0 && (int64_t)v < a.Lmax);
 #pragma unroll
-    for (int i = 0; i < 9; ++i) {
-      const int c = lane + 32 * i, rec = c / 9;
-      if (c < chunks) cp_async16(ring + stage * kTileBytes + 16 * c, base + (int64_t)s_idx[warp][rec] * kRec + 16 * (c - 9 * rec));
+      for (int i = 0; i < 11; ++i) {
+        const int e = 3 * i + third;
+        const int64_t at = (int64_t)__shfl_sync(0xffffffffu, v, e & 31) * kRec;
+        if (third < 3 && e < kTile && (in >> (e & 31) & 1u)) cp_async16(dst + 3 * i * kRec + 16 * lane, rec + at);
+      }
+    } else if (j < items) {
+      in = __ballot_sync(0xffffffffu, !(__int_as_float(v) == -INFINITY));
+      const int e0 = (j - tiles) * kRowsPerTile;
+#pragma unroll
+      for (int i = 0; i < kRowsPerTile; i += 2) {
+        const int e = i + (lane >> 4);
+        const bool live = in >> e & 1u;
+        const int64_t at = live ? prow + (int64_t)(e0 + e) * a.kb_sb : prow;
+        const uint32_t to = dst + e * 256 + (((lane & 15) ^ e) << 4);
+        cp_async16_or_zero(to, a.kbar + at, live);
+        cp_async16_or_zero(to + 2048, a.vbar + at, live);
+      }
     }
-    __syncwarp();
+    cp_async_commit();
+    return in;
   };
-  int first[kListStages];
-#pragma unroll
-  for (int i = 0; i < kListStages; ++i) first[i] = entry(wi + i * nw);
-
-  // ---- proxies: half-warp h of the row's 2 nw takes h, h + 2 nw, ...; lane hl dims 8 hl .. 8 hl + 7
-  {
-    constexpr int kUnroll = 4;
-    const int hl = lane & 15;
-    const unsigned hmask = 0xffffu << (lane & 16);
-    const int64_t pr = (a.per_qhead ? r : kvh) * a.kb_sh;
-    float qf[8], acc[8], m = -INFINITY, l = 0.f;
-    unpack8(*reinterpret_cast<const uint4*>(a.q + r * a.q_stride + 8 * hl), qf);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-    bool started = false;
-    for (int j0 = 2 * wi + (lane >> 4); j0 - (lane >> 4) < a.NB || !started; j0 += 2 * nw * kUnroll) {
-      uint4 kw[kUnroll], vw[kUnroll];
-      float bias[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int j = j0 + 2 * nw * u;
-        bias[u] = j < a.NB ? a.logn[r * a.ln_stride + j] * kLog2e : -INFINITY;
-        kw[u] = vw[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (!(bias[u] == -INFINITY)) {
-          kw[u] = ldg_stream(a.kbar + pr + j * a.kb_sb + 8 * hl);
-          vw[u] = ldg_stream(a.vbar + pr + j * a.kb_sb + 8 * hl);
-        }
-      }
-      if (!started) {  // the records' copies go out behind the first proxies' loads
-        started = true;
-#pragma unroll
-        for (int i = 0; i < kListStages - 1; ++i) {
-          gather(first[i], i);
-          cp_async_commit();
-        }
-      }
-      float z[kUnroll], mx = m;
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        float kf[8], d = 0.f;
-        unpack8(kw[u], kf);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d = fmaf(qf[i], kf[i], d);
-#pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) d += __shfl_xor_sync(hmask, d, o);
-        z[u] = bias[u] == -INFINITY ? -INFINITY : fmaf(d, a.qk_scale, bias[u]);
-        mx = fmaxf(mx, z[u]);
-      }
-      const float bm = biased(mx), al = ex2(m - bm);
-      m = mx;
-      l *= al;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] *= al;
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const float p = ex2(z[u] - bm);
-        float vf[8];
-        unpack8(vw[u], vf);
-        l += p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(p, vf[i], acc[i]);
-      }
-    }
-    float* st = s_state + (lane >> 4) * kStateFloats;
-    reinterpret_cast<float4*>(st)[2 * hl] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    reinterpret_cast<float4*>(st)[2 * hl + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    if (hl == 0) {
-      st[kD] = m;
-      st[kD + 1] = l;
-    }
-  }
-
-  // ---- records
-  WarpAttention<true> at;
+  int j = rank * W + warp;
+  int v0 = ask(j), v1 = ask(j + nw), v2 = ask(j + 2 * nw);
+  WarpAttention<true, 1> at;
   at.lane_addresses();
   at.load_q(at.op_col() == 0 ? a.q + r * a.q_stride : nullptr);
+  uint32_t in0 = fetch(j, v0, 0), in1 = fetch(j + nw, v1, 1);
   at.begin(a.qk_scale);
-  int stage = 0, ahead = first[kListStages - 1];
-  for (int j = wi; j < tiles; j += nw) {
-    // tile j + 2 nw goes out; the index after it is asked for
-    const int t = ahead;
-    ahead = entry(j + kListStages * nw);
-    gather(t, stage == 0 ? kListStages - 1 : stage - 1);
-    cp_async_commit();
-    cp_async_wait<kListStages - 1>();
+  bool rows = false;
+  for (int stage = 0; j < items; j += nw) {
+    const int before = stage == 0 ? kStages - 1 : stage - 1;
+    const uint32_t in2 = fetch(j + 2 * nw, v2, before);
+    const int v3 = ask(j + 3 * nw);
+    cp_async_wait<kStages - 1>();
     __syncwarp();
-    const int cnt = s_cnt[warp][stage];
-    const int lim[2] = {cnt, cnt};
-    if (cnt == kTile)
-      at.tile<false>(ring + stage * kTileBytes, lim);
-    else if (cnt > 0)
-      at.tile<true>(ring + stage * kTileBytes, lim);
+    const uint32_t sm = ring + stage * kTileBytes;
+    if (j < tiles) {
+      const uint32_t sees[2] = {in0, in0};
+      if (in0 == ~0u)
+        at.template tile<false>(sm, sees);
+      else if (in0)
+        at.template tile<true>(sm, sees);
+    } else {
+      if (!rows) at.begin_rows(a.q + r * a.q_stride);
+      rows = true;
+      if (in0) at.rows(sm, in0, __int_as_float(v0) * kLog2e, a.qk_scale);
+    }
     __syncwarp();
-    stage = stage + 1 == kListStages ? 0 : stage + 1;
+    in0 = in1;
+    in1 = in2;
+    v0 = v1;
+    v1 = v2;
+    v2 = v3;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   cp_async_wait<0>();
-  at.finish(s_state + 2 * kStateFloats, s_state + 2 * kStateFloats + kD, 1);
+  __syncwarp();
+  {
+    float* state = reinterpret_cast<float*>(s_dyn + warp * (kStages * kTileBytes));
+    at.finish(state, state + kD, 1);
+  }
   __syncthreads();
 
   // ---- merge the CTA's states, then the cluster's
-  const float* st = reinterpret_cast<const float*>(s_dyn + W * (kListStages * kTileBytes));
-  float M = -INFINITY, L = 0.f;
+  const float* st = reinterpret_cast<const float*>(s_dyn);
+  constexpr int kNext = kStages * kTileBytes / 4;  // floats from one warp's state to the next
+  float M = -INFINITY, L = 0.f, f[W];
 #pragma unroll
-  for (int i = 0; i < W * kStates; ++i) M = fmaxf(M, st[i * kStateFloats + kD]);
-  float f[W * kStates];
+  for (int i = 0; i < W; ++i) M = fmaxf(M, st[i * kNext + kD]);
 #pragma unroll
-  for (int i = 0; i < W * kStates; ++i) {
-    f[i] = ex2(st[i * kStateFloats + kD] - biased(M));
-    L = fmaf(f[i], st[i * kStateFloats + kD + 1], L);
+  for (int i = 0; i < W; ++i) {
+    f[i] = ex2(st[i * kNext + kD] - biased(M));
+    L = fmaf(f[i], st[i * kNext + kD + 1], L);
   }
   for (int d = tid; d < kD; d += 32 * W) {
     float A = 0.f;
 #pragma unroll
-    for (int i = 0; i < W * kStates; ++i) A = fmaf(f[i], st[i * kStateFloats + d], A);
+    for (int i = 0; i < W; ++i) A = fmaf(f[i], st[i * kNext + d], A);
     if (S == 1)
       store_list(a, r, d, A, L);
     else
@@ -882,9 +840,9 @@ extern "C" int oa_kv4_flash(const oa_kv4_flash_args* args, void* stream) {
   a.out_f32 = g.out_dtype == OA_F32;
   a.G = (int)(BQ / BH);
   a.qk_scale = (float)(g.sm_scale * (double)oa::kLog2e);
-  // Warps per row: enough that all rows together fill the GPU's 16 warps per SM, but a tile (or eight proxies)
-  // each; up to 8 in a CTA, beyond that a cluster of CTAs.  Two at least: 64 threads write the row.
-  const int64_t fill = 148 * 16 / BQ, work = (n_sel + n_exp + oa::kTile - 1) / oa::kTile + (NB + 7) / 8;
+  // Warps per row: enough that all rows together fill the GPU's 16 warps per SM, but two items each; up to 8 in a
+  // CTA, beyond that a cluster of CTAs.
+  const int64_t fill = 148 * 16 / BQ, work = ((n_sel + n_exp + oa::kTile - 1) / oa::kTile + (NB + oa::kRowsPerTile - 1) / oa::kRowsPerTile + 1) / 2;
   const int64_t warps = std::min(fill, work);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (warps >= 16) {

@@ -39,6 +39,19 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -80,8 +93,8 @@ __device__ __forceinline__ int row_token(int r) { return (r & 1) ? 8 + ((r + 3) 
 // PAIR: at most four columns, and the MMA's eight columns hold each twice: columns 0..3 are the four query rows
 // against half 0 of the head, columns 4..7 against half 1.  A lane then serves one half: half the scales to read,
 // weights to form and turn; the halves' scores meet through one shuffle.  Otherwise eight columns, each lane
-// both halves.
-template <bool PAIR>
+// both halves.  J: accumulator columns of a lane that are in use (1 where there is one query row).
+template <bool PAIR, int J = 2>
 struct WarpAttention {
   static constexpr int kHalves = PAIR ? 1 : 2;  // halves a lane serves
   uint32_t qf[16];            // q operand: half h, word i -> qf[8 h + 2 i], +1
@@ -200,11 +213,13 @@ struct WarpAttention {
     cap[h] = pow2i(kTop) / next;
   }
 
-  // One tile of 32 records at shared address `sm`.  MASK: the lane's accumulator column j sees only the tokens
-  // below lim[j] of the tile; what masked records hold (stale bytes, NaN scales) does not enter.
+  // One tile of 32 records at shared address `sm`.  MASK: the lane's accumulator column j sees only the tokens whose
+  // bit is set in sees[j]; what the others' records hold (stale bytes, NaN scales) does not enter.
   template <bool MASK>
-  __device__ __forceinline__ void tile(uint32_t sm, const int (&lim)[2]) {
-    const int tok = MASK ? row_token(lane() >> 2) : 0;
+  __device__ __forceinline__ void tile(uint32_t sm, const uint32_t (&sees)[2]) {
+    uint32_t in[2];  // bit 16 b + k: this lane's token k of block b
+#pragma unroll
+    for (int j = 0; j < 2; ++j) in[j] = MASK ? sees[j] >> row_token(lane() >> 2) : 0u;
     float x[2][4];
     uint32_t vm[2][2][kHalves];  // value scale and offset of this lane's four tokens
 #pragma unroll
@@ -242,7 +257,7 @@ struct WarpAttention {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < J; ++j) {
           float y = bf_lo(km[k][0]) * c[0][2 * k + j], z = bf_hi(km[k][0]) * qs[j][0];
           if (!PAIR) {
             y = fmaf(bf_lo(km[k][kHalves - 1]), c[kHalves - 1][2 * k + j], y);
@@ -250,7 +265,7 @@ struct WarpAttention {
           }
           float v = fmaf(y, scale[j], z);
           if (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);
-          if (MASK && 16 * b + tok + k >= lim[j]) v = -INFINITY;
+          if (MASK && !(in[j] >> (16 * b + k) & 1u)) v = -INFINITY;
           x[b][2 * k + j] = v;
         }
     }
@@ -258,19 +273,19 @@ struct WarpAttention {
     // a scale above the cap): weights up to 2^kSlack are as good as weights up to 1, and new maxima are common
     float mx[2], s[kHalves];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) mx[j] = fmaxf(fmaxf(x[0][j], x[0][2 + j]), fmaxf(x[1][j], x[1][2 + j]));
+    for (int j = 0; j < J; ++j) mx[j] = fmaxf(fmaxf(x[0][j], x[0][2 + j]), fmaxf(x[1][j], x[1][2 + j]));
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       s[h] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool in = !MASK || 16 * (i >> 1) + tok + (i & 1) < max(lim[0], lim[1]);
-        s[h] = fmaxf(s[h], in ? bf_lo(vm[i >> 1][i & 1][h]) : 0.f);
+        const bool used = !MASK || ((in[0] | in[J - 1]) >> (16 * (i >> 1) + (i & 1)) & 1u);
+        s[h] = fmaxf(s[h], used ? bf_lo(vm[i >> 1][i & 1][h]) : 0.f);
       }
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack || s[0] > cap[0] || s[kHalves - 1] > cap[kHalves - 1])) {
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[J - 1] > m[J - 1] + kSlack || s[0] > cap[0] || s[kHalves - 1] > cap[kHalves - 1])) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < J; ++j) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
         const float nm = fmaxf(m[j], mx[j]);
@@ -294,22 +309,22 @@ struct WarpAttention {
       uint32_t pw[2][kHalves];  // weights, turned: tokens of MMA rows 0..7, of rows 8..15
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float p0 = ex2(x[b][2 * k] - bm[0]), p1 = ex2(x[b][2 * k + 1] - bm[1]);
+        const float p0 = ex2(x[b][2 * k] - bm[0]), p1 = J > 1 ? ex2(x[b][2 * k + 1] - bm[1]) : 0.f;
         l[0] += p0;
-        l[1] += p1;
+        if (J > 1) l[1] += p1;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
           const float sv = bf_lo(vm[b][k][h]) * r[h], zv = bf_hi(vm[b][k][h]);
-          float w0 = p0 * sv, w1 = p1 * sv;
+          float w0 = p0 * sv, w1 = J > 1 ? p1 * sv : 0.f;
           if (MASK) {
-            const int tk = 16 * b + tok + k;
-            w0 = tk < lim[0] ? w0 : 0.f;
-            w1 = tk < lim[1] ? w1 : 0.f;
-            zs[0][h] += tk < lim[0] ? p0 * zv : 0.f;
-            zs[1][h] += tk < lim[1] ? p1 * zv : 0.f;
+            const bool in0 = in[0] >> (16 * b + k) & 1u, in1 = J > 1 && (in[1] >> (16 * b + k) & 1u);
+            w0 = in0 ? w0 : 0.f;
+            w1 = in1 ? w1 : 0.f;
+            zs[0][h] += in0 ? p0 * zv : 0.f;
+            if (J > 1) zs[1][h] += in1 ? p1 * zv : 0.f;
           } else {
             zs[0][h] = fmaf(p0, zv, zs[0][h]);
-            zs[1][h] = fmaf(p1, zv, zs[1][h]);
+            if (J > 1) zs[1][h] = fmaf(p1, zv, zs[1][h]);
           }
           pw[k][h] = transpose8x8(pack_half2(w0, w1));
         }
@@ -328,11 +343,85 @@ struct WarpAttention {
     }
   }
 
+  // ---- bf16 rows among the records (PAIR, J = 1: one query row, in columns 0 and 4): tiles of 8 rows of K, then 8
+  // of V, 256 bytes each, 16-byte chunk c of row i at chunk c ^ i.  Scores: MMA rows g and g + 8 are the two halves
+  // of K row g, columns 0 and 1 the halves of q; the score is their diagonal's sum.  Values go into the records'
+  // accumulators: weights carry the factors that those carry, as two bf16 terms (16 bits) in columns 0, 1 (half 0)
+  // and 4, 5 (half 1).
+  __device__ __forceinline__ void begin_rows(const __nv_bfloat16* q) {
+    const int g = lane() >> 2, t = lane() & 3;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qf[i] = 0u;
+    if (g < 2) {  // step i: dims 64 g + 16 i + 2t, + 1 and + 8, + 9
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qf[2 * i] = *reinterpret_cast<const uint32_t*>(q + 64 * g + 16 * i + 2 * t);
+        qf[2 * i + 1] = *reinterpret_cast<const uint32_t*>(q + 64 * g + 16 * i + 2 * t + 8);
+      }
+    }
+    // scales of records may have left a factor that would carry a large row past fp32
+    if (r[0] > pow2i(60)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= pow2i(60) / r[0];
+      cap[0] = pow2i(kTop - 60);
+      r[0] = pow2i(60);
+    }
+  }
+  // sm: the tile; in: its live rows (others are zero in memory); bias: this lane's row's (lane < 8) log2 weight
+  __device__ __forceinline__ void rows(uint32_t sm, uint32_t in, float bias, float qk_scale) {
+    const int g = lane() >> 2, t = lane() & 3;
+    // ldmatrix: lane 8 x + i gives row i of matrix x: half x & 1 of K, 8 dims x >> 1 of the 16 of a step
+    const uint32_t i8 = lane() & 7, x = lane() >> 3;
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t k[4];
+      const uint32_t chunk = 8 * (x & 1) + 2 * i + (x >> 1);
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(k[0]), "=r"(k[1]), "=r"(k[2]), "=r"(k[3])
+                   : "r"(sm + i8 * 256 + ((chunk ^ i8) << 4)));
+      mma_bf16(c, k[0], k[1], k[2], k[3], qf[2 * i], qf[2 * i + 1]);
+    }
+    float v = __shfl_sync(0xffffffffu, c[0] + c[3], lane() & 28);  // lane t = 0 of the row has it
+    const float b = __shfl_sync(0xffffffffu, bias, g);
+    v = (in >> g & 1u) && !(t & 1) ? fmaf(v, qk_scale, b) : -INFINITY;
+    if (__any_sync(0xffffffffu, v > m[0] + kSlack)) {
+      float mx = v;
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx = fmaxf(m[0], mx);
+      const float al = ex2(m[0] - biased(mx));
+      m[0] = mx;
+      bm[0] = biased(mx);
+      l[0] *= al;
+      zs[0][0] *= al;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= al;
+    }
+    const float p = ex2(v - bm[0]);
+    l[0] += p;
+    const float w = p * (r[0] * pow2i(half() ? -20 : -24)), hi = bf_round(w);
+    const uint32_t pw = transpose8x8((uint32_t)f2bf_bits(hi) | ((uint32_t)f2bf_bits(w - hi) << 16));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t r0 = 2 * t, r1 = 2 * t + 1, ch = 8 * h + g;
+      const uint4 a = lds128(sm + 2048 + r0 * 256 + ((ch ^ r0) << 4), 0), d = lds128(sm + 2048 + r1 * 256 + ((ch ^ r1) << 4), 0);
+      mma_bf16_k8(acc[4 * h], __byte_perm(a.x, d.x, 0x5410), __byte_perm(a.x, d.x, 0x7632), pw);
+      mma_bf16_k8(acc[4 * h + 1], __byte_perm(a.y, d.y, 0x5410), __byte_perm(a.y, d.y, 0x7632), pw);
+      mma_bf16_k8(acc[4 * h + 2], __byte_perm(a.z, d.z, 0x5410), __byte_perm(a.z, d.z, 0x7632), pw);
+      mma_bf16_k8(acc[4 * h + 3], __byte_perm(a.w, d.w, 0x5410), __byte_perm(a.w, d.w, 0x7632), pw);
+    }
+  }
+
   // The warp's unnormalised result of each column c < ncol: part[c * kD + d], ml[2 c] = m, ml[2 c + 1] = l.
   __device__ __forceinline__ void finish(float* part, float* ml, int ncol) {
     const int g = lane() >> 2;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < J; ++j) {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
@@ -341,7 +430,7 @@ struct WarpAttention {
       }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < J; ++j) {
       const int c = acc_col(j);
       if (c < ncol) {
 #pragma unroll
@@ -353,8 +442,10 @@ struct WarpAttention {
           float o[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            o[2 * i] = fmaf(acc[4 * h + i][j] * u, f, z);
-            o[2 * i + 1] = fmaf(acc[4 * h + i][2 + j] * u, f, z);
+            // J = 1: the second column holds the rows' second weight term
+            const float* c2 = acc[4 * h + i];
+            o[2 * i] = fmaf((J == 1 ? c2[0] + c2[1] : c2[j]) * u, f, z);
+            o[2 * i + 1] = fmaf((J == 1 ? c2[2] + c2[3] : c2[2 + j]) * u, f, z);
           }
           float4* dst = reinterpret_cast<float4*>(part + c * kD + 64 * h + 8 * g);
           dst[0] = make_float4(o[0], o[1], o[2], o[3]);
