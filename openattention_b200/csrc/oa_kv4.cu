@@ -60,14 +60,14 @@ __device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, 
 // of a tile are contiguous).  Lengths live on the device, so each CTA finds its share itself:
 //  - each row its own CTAs, grid / rows of them (no more than one per 8 tiles), where that balances;
 //  - else the tiles of all rows in one line, cut into equal parts; a CTA then ends one row and begins the next.
-// A row that one CTA covers is written by it.  Otherwise each part leaves (m, l, O) in the workspace and a second
-// kernel merges the parts in the order of their items, so the result does not depend on who took which item.
+// A row that one CTA covers is written by it.  Otherwise each part leaves (m, l, O) in the workspace and the
+// last CTA to arrive (atomic ticket, no waiting) merges the parts in CTA order, so the result does not depend
+// on which CTA is last.
 constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kCols = 8;
-constexpr int kRowUnits = 10;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
-constexpr unsigned kLongShare = 384;  // units per CTA from which the line is cut into kLevels times as many items
+constexpr int kRowUnits = 12;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
 constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
 constexpr int kRingBytes = kWarps * kStages * kTileBytes;
 
@@ -75,7 +75,6 @@ struct DensePlan {
   int blocks;    // column blocks of a KV head: ceil(G T / 8)
   int64_t rows;  // B * HKV * blocks
   int grid;
-  int64_t most_units;  // on the line, with every request as long as the cache
 };
 
 DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax) {
@@ -91,7 +90,6 @@ DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax
   const int64_t tiles = (Lmax + kTile - 1) / kTile;
   const int64_t parts = std::max<int64_t>(1, (tiles + kWarps - 1) / kWarps);
   // two CTAs per SM (their rings fill its shared memory); no more than one per row and 8 tiles
-  p.most_units = p.rows * (std::max<int64_t>(tiles, 1) + kRowUnits);
   p.grid = p.rows > 2 * sms ? 2 * sms : (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, p.rows * parts));
   return p;
 }
@@ -99,9 +97,8 @@ DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax
 struct DenseWork {
   unsigned blocks, per_req, rows;  // column blocks of a KV head; rows of a request; rows
   unsigned cpr;                    // CTAs a row can have to itself: grid / rows
-  float* parts;                    // 2 per work item: [0] of a row that began in an earlier item, [1] of one that begins there
-  uint2* spread;                   // per row: its first item and how many share it (0: written by one CTA)
-  unsigned* taken;                 // items handed out beyond the CTAs' first; zero between calls
+  float* parts;                    // 2 per CTA: [0] of a row that began in an earlier CTA, [1] of one that begins here
+  unsigned* tickets;               // one per row, zero between calls
 };
 
 __device__ __forceinline__ int dense_len(const DenseArgs& a, int64_t b) {
@@ -133,56 +130,103 @@ __device__ __forceinline__ void store_out4(void* out, int out_f32, int64_t at, i
   }
 }
 
-// The cut of the call's work, found by every CTA from the lengths.  `own`: item i is one CTA's part of one row.
-// Else the line of all rows' units is cut into `levels` stretches, each into `active` equal items: 12, 3 and 1
-// sixteenths of the line, or the whole line at once when that is short.  Counts of units fit 31 bits (checked by
-// the host).
-struct DenseCut {
-  unsigned total, active, levels;
-  int most;  // tiles of the longest row
-  bool own;
-};
-constexpr unsigned kLevels = 3;
-__device__ __forceinline__ unsigned level_begin(const DenseCut& c, unsigned level) {  // of the line's units
-  if (level >= c.levels) return c.total;
-  return level == 0 ? 0u : c.total / 16u * (level == 1 ? 12u : 15u);
-}
-__device__ __forceinline__ unsigned item_begin(const DenseCut& c, unsigned item) {
-  const unsigned level = item / c.active, i = item - level * c.active;
-  const unsigned u = level_begin(c, level), len = level_begin(c, level + 1) - u, each = len / c.active;
-  return u + i * each + min(i, len - each * c.active);
-}
-__device__ __forceinline__ unsigned item_of(const DenseCut& c, unsigned unit) {  // the item that a unit is in
-  unsigned level = 0;
-  while (level + 1 < c.levels && unit >= level_begin(c, level + 1)) ++level;
-  const unsigned u = level_begin(c, level), len = level_begin(c, level + 1) - u, each = len / c.active;
-  const unsigned extra = len - each * c.active, big = extra * (each + 1);
-  unit -= u;
-  return level * c.active + (unit < big ? unit / (each + 1) : extra + (unit - big) / each);
+// The parts of one row, part v at src (v = 0) or src + (2 v - 1) kPartFloats.  Every thread sums four dims of one
+// column over its share of the parts, kAhead loads in flight; the first ones are issued before the weights
+// 2^(m_v - M) are known.  The shares are added in a fixed order.  o_at: the output row of column `warp`.
+// Inlined, and kAhead no larger: a call, or more loads held, spills the caller's main loop.
+template <int kAhead>
+__device__ __forceinline__ void merge_parts(const float* src, int parts, int ncol, float* sh, void* out, int out_f32,
+                                         int64_t o_at) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float* s_l = sh;                   // per column
+  float* s_f = sh + kCols;           // [part][column]
+  float* s_a = s_f + kCols * parts;  // [share][column][128]
+  const int quads = ncol * (kD / 4), shares = kDenseThreads / quads;  // ncol <= 8: at least one share
+  const int share = tid / quads, qd = tid - share * quads, col = qd / (kD / 4);
+  auto at = [&](int v) { return src + (v ? 2 * v - 1 : 0) * (int64_t)kPartFloats; };
+  float4 x[kAhead];
+  if (share < shares) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (share + i * shares < parts) x[i] = __ldcg(reinterpret_cast<const float4*>(at(share + i * shares)) + qd);
+  }
+  if (warp < ncol) {  // the weights of column `warp`
+    float M = -INFINITY, L = 0.f;
+    for (int v = lane; v < parts; v += 32) {
+      const float m = __ldcg(at(v) + kCols * kD + 2 * warp);
+      s_f[v * kCols + warp] = m;
+      M = fmaxf(M, m);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    M = biased(M);
+    for (int v = lane; v < parts; v += 32) {
+      const float f = ex2(s_f[v * kCols + warp] - M);
+      L = fmaf(f, __ldcg(at(v) + kCols * kD + 2 * warp + 1), L);
+      s_f[v * kCols + warp] = f;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) s_l[warp] = L;
+  }
+  __syncthreads();
+  if (share < shares) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int v = share; v < parts;) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i, v += shares)
+        if (v < parts) axpy(acc, s_f[v * kCols + col], x[i]);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + i * shares < parts) x[i] = __ldcg(reinterpret_cast<const float4*>(at(v + i * shares)) + qd);
+    }
+    reinterpret_cast<float4*>(s_a)[share * quads + qd] = acc;
+  }
+  __syncthreads();
+  if (warp < ncol) {
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int v = 0; v < shares; ++v) axpy(A, 1.f, reinterpret_cast<const float4*>(s_a)[v * quads + 32 * warp + lane]);
+    store_out4(out, out_f32, o_at, lane, A, s_l[warp]);
+  }
 }
 
-// One CTA's part of one row: what the whole CTA needs to know of it.
-struct DensePart {
-  unsigned b, r;      // request, row within it
-  int n, tiles;       // the request's length, a row's tiles
-  int tile, share;    // first tile and number of tiles of the part
-  unsigned item;      // the work item it belongs to
-  unsigned line;      // where the part begins on the line (units)
-  int left, off;      // units of the item from there on; units of the row before the part
-  unsigned first, parts;  // own: the row's items
+// A CTA's way along the line of rows: the row it is at and its tiles of that row.  Counts of units fit 31 bits
+// (checked by the host).
+struct DenseShare {
+  unsigned b, r;          // request, row within it
+  int n, tiles;           // the request's length, a row's tiles
+  int tile, share;        // first tile and number of tiles of this CTA's part
+  bool own;               // the row's CTAs serve no other row
+  unsigned line;          // where the part begins on the line (units)
+  int left, off;          // units of this CTA's share from there on; units of the row before the part
+  unsigned each, extra;   // the line's cut: `extra` CTAs take each + 1 units, the others `each`
+  unsigned first, parts;  // own: the row's CTAs
 };
+// the CTA that unit u belongs to, and where a CTA's units begin
+__device__ __forceinline__ unsigned cta_of(const DenseShare& s, unsigned u) {
+  const unsigned big = s.extra * (s.each + 1);
+  return u < big ? u / (s.each + 1) : s.extra + (u - big) / s.each;
+}
+__device__ __forceinline__ unsigned cta_begin(const DenseShare& s, unsigned cta) {
+  return cta * s.each + min(cta, s.extra);
+}
 
-__device__ __forceinline__ void dense_cut(const DenseArgs& a, const DenseWork& w, unsigned* s_pre, DenseCut& cut) {
+// False: nothing for this CTA.  Every thread of the CTA finds the same.
+__device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
+  __shared__ unsigned s_pre[kDenseThreads];  // units of a row of each request before thread i's requests
   __shared__ unsigned s_sum[kWarps];
   __shared__ int s_most[kWarps];
-  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grid = gridDim.x;
+  const unsigned tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned grid = gridDim.x, cta = blockIdx.x;
+  const unsigned c = ((unsigned)a.B + kDenseThreads - 1) / kDenseThreads;  // requests a thread sums
+  const bool same = a.n.stride == 0;
   unsigned units;
   int most;
-  if (a.n.stride == 0) {
-    most = dense_tiles(dense_len(a, 0));
+  if (same) {
+    s.n = dense_len(a, 0);
+    most = dense_tiles(s.n);
     units = a.B * (unsigned)(most + kRowUnits);
-  } else {  // thread i sums requests [i c, i c + c)
-    const unsigned c = ((unsigned)a.B + kDenseThreads - 1) / kDenseThreads;
+  } else {
     unsigned sum = 0;
     most = 0;
     for (unsigned b = tid * c; b < min((tid + 1) * c, (unsigned)a.B); ++b) {
@@ -208,54 +252,45 @@ __device__ __forceinline__ void dense_cut(const DenseArgs& a, const DenseWork& w
       units += s_sum[i];
       most = max(most, s_most[i]);
     }
-    s_pre[tid] = before + inc - sum;  // units of a row of each request before thread tid's
+    s_pre[tid] = before + inc - sum;
     __syncthreads();
   }
-  cut.most = most;
-  cut.total = units * w.per_req;
-  cut.levels = cut.total >= kLongShare * grid ? kLevels : 1u;
-  // rows to themselves: where no dynamic items are due and the longest row's CTA gets at most 9/8 of the mean
-  cut.own = cut.levels == 1 && w.cpr >= 1 &&
-            (kRowUnits + (most + w.cpr - 1) / w.cpr) * (8u * grid) <= max((kRowUnits + kWarps) * 8u * grid, 9u * cut.total);
-  cut.active = cut.levels > 1 ? grid : min(grid, (cut.total + kRowUnits + kWarps - 1) / (kRowUnits + kWarps));
-}
-
-// The first part of an item; false: there is none.  One thread.
-__device__ bool dense_item(const DenseArgs& a, const DenseWork& w, const DenseCut& cut, const unsigned* s_pre,
-                           unsigned item, DensePart& s) {
-  s.item = item;
-  if (cut.own) {
-    const unsigned row = item / w.cpr, j = item - row * w.cpr;
+  const unsigned total = units * w.per_req;
+  s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * (8u * grid) <= max((kRowUnits + kWarps) * 8u * grid, 9u * total);
+  if (s.own) {
+    const unsigned row = cta / w.cpr, j = cta - row * w.cpr;
     if (row >= w.rows) return false;
     s.b = row / w.per_req;
     s.r = row - s.b * w.per_req;
-    s.n = dense_len(a, s.b);
+    if (!same) s.n = dense_len(a, s.b);
     s.tiles = dense_tiles(s.n);
     s.parts = min(w.cpr, (unsigned)(s.tiles + kWarps - 1) / kWarps);
     if (j >= s.parts) return false;
     const unsigned each = s.tiles / s.parts, extra = s.tiles - each * s.parts;
     s.tile = j * each + min(j, extra);
     s.share = each + (j < extra ? 1 : 0);
-    s.first = item - j;
+    s.first = cta - j;
     return true;
   }
-  if (item >= cut.active * cut.levels) return false;
-  s.line = item_begin(cut, item);
-  s.left = item_begin(cut, item + 1) - s.line;
+  const unsigned active = min(grid, (total + kRowUnits + kWarps - 1) / (kRowUnits + kWarps));
+  if (cta >= active) return false;
+  s.each = total / active;
+  s.extra = total - s.each * active;
+  s.line = cta_begin(s, cta);
+  s.left = s.each + (cta < s.extra ? 1 : 0);
   const unsigned v = s.line / w.per_req;
   unsigned p;
-  if (a.n.stride == 0) {
-    s.n = dense_len(a, 0);
-    s.tiles = cut.most;
-    s.b = v / (cut.most + kRowUnits);
-    p = s.b * (cut.most + kRowUnits);
+  if (same) {
+    s.tiles = most;
+    s.b = v / (most + kRowUnits);
+    p = s.b * (most + kRowUnits);
   } else {
     unsigned lo = 0, hi = kDenseThreads;  // the last thread whose requests begin at or before v
     while (hi - lo > 1) {
       const unsigned mid = (lo + hi) >> 1;
       if (s_pre[mid] <= v) lo = mid; else hi = mid;
     }
-    s.b = lo * (((unsigned)a.B + kDenseThreads - 1) / kDenseThreads);
+    s.b = lo * c;
     p = s_pre[lo];
     s.n = dense_len(a, s.b);
     s.tiles = dense_tiles(s.n);
@@ -273,8 +308,8 @@ __device__ bool dense_item(const DenseArgs& a, const DenseWork& w, const DenseCu
   return true;
 }
 
-// The same item's part of the next row, into s; false: the item ends before that row's first tile.
-__device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& w, DensePart& s) {
+// The next row on the line, if any of its tiles are this CTA's.
+__device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
   const int step = s.tiles + kRowUnits - s.off;
   s.line += step;
   s.left -= step;
@@ -295,132 +330,94 @@ __device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& 
 
 template <bool PAIR>
 __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
-  extern __shared__ __align__(16) unsigned char s_ring[];  // [stage][warp][tile]
-  __shared__ unsigned s_pre[kDenseThreads];
-  __shared__ DenseCut s_cut;
-  __shared__ DensePart s_now, s_next;  // the same for all threads: kept out of the main loop's registers
-  __shared__ unsigned s_more;
+  extern __shared__ __align__(16) unsigned char s_ring[];
+  __shared__ unsigned s_last;
+  __shared__ DenseShare s;  // the same for all threads: kept here, out of the loop's registers
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.HQ / a.HKV, cols = G * a.T;
+  const unsigned cta = blockIdx.x;
   {
-    DenseCut cut;
-    dense_cut(a, w, s_pre, cut);
-    if (tid == 0) {
-      s_cut = cut;
-      bool more = dense_item(a, w, cut, s_pre, blockIdx.x, s_now);
-      while (more && s_now.share <= 0)  // an item that ends before its row's first tile
-        more = cut.levels > 1 && dense_item(a, w, cut, s_pre, cut.active + atomicAdd(w.taken, 1u), s_now);
-      s_more = more ? 1u : 0u;
-    }
+    DenseShare mine;
+    if (!dense_share(a, w, mine)) return;
+    if (tid == 0) s = mine;
   }
   __syncthreads();
-  if (!s_more) return;
 
-  const uint32_t ring = smem_u32(s_ring) + warp * kTileBytes;
-  constexpr uint32_t kStageBytes = kWarps * kTileBytes;
-  // the merge's room is the last stage: free between a row's last tile and the next row's third
-  float* s_part = reinterpret_cast<float*>(s_ring + (kStages - 1) * kStageBytes);
-  const unsigned char* src = nullptr;  // the next tile this warp copies, at this lane's bytes
-  auto fetch = [&](int records, uint32_t stage) {  // `records` of the tile are the request's
-    const uint32_t dst = ring + stage * kStageBytes + 16 * lane;
-    if (records >= kTile) {
-#pragma unroll
-      for (int i = 0; i < kTileBytes / 512; ++i) cp_async16(dst + 512 * i, src + 512 * i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kTileBytes / 512; ++i)
-        if (16 * lane + 512 * i < records * kRec) cp_async16(dst + 512 * i, src + 512 * i);
-    }
-    src += (int64_t)kWarps * kTileBytes;
-  };
-  // the first tiles of a part: its warp w takes tiles w, w + 8, ... of it
-  auto fetch_first = [&](const DensePart& s) {
-    const int t0 = s.tile + warp, t1 = s.tile + s.share;
-    src = a.cache + s.b * a.c_sb + (int64_t)(s.r / w.blocks) * a.c_sh + (int64_t)t0 * kTileBytes + 16 * lane;
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (t0 + i * kWarps < t1) fetch(s.n - (t0 + i * kWarps) * kTile, i);
-      cp_async_commit();
-    }
-  };
-  // column c of a row: head and query token
-  auto split = [&](int c, int& hh, int& tt) {
-    hh = a.T == 1 ? c : c / a.T;
-    tt = c - hh * a.T;
-  };
+  const uint32_t ring = smem_u32(s_ring) + warp * (kStages * kTileBytes);
+  float* s_part = reinterpret_cast<float*>(s_ring);  // reused once a row's tiles are done
   WarpAttention<PAIR> at;
   at.lane_addresses();
-  auto load_q = [&](const DensePart& s) {
-    const int kvh = s.r / w.blocks, c = (s.r - kvh * w.blocks) * kCols + at.op_col();
-    int hh, tt;
-    split(c, hh, tt);
-    at.load_q(c < cols ? static_cast<const __nv_bfloat16*>(a.q.p) + s.b * a.q.sb + (int64_t)(kvh * G + hh) * a.q.sh +
-                             tt * a.q.st
-                       : nullptr);
-  };
-  load_q(s_now);
-  fetch_first(s_now);
 
   for (;;) {
+    if (s.share <= 0) return;  // the share ends before the row's first tile
+    const int kvh = s.r / w.blocks;
+    const int col0 = (s.r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
+    // the query row of column c: head h0 + (col0 + c) / T, query token (col0 + c) % T
+    const int64_t q_at = s.b * a.q.sb + (int64_t)(kvh * G) * a.q.sh;
+    auto split = [&](int c, int& hh, int& tt) {
+      hh = a.T == 1 ? col0 + c : (col0 + c) / a.T;
+      tt = col0 + c - hh * a.T;
+    };
+    {
+      int hh, tt;
+      split(at.op_col(), hh, tt);
+      at.load_q(at.op_col() < ncol ? static_cast<const __nv_bfloat16*>(a.q.p) + q_at + hh * a.q.sh + tt * a.q.st : nullptr);
+    }
+    const int t0 = s.tile + warp, t1 = s.tile + s.share, n = s.n;  // this warp: t0, t0 + 8, ...
+    const unsigned char* src = a.cache + s.b * a.c_sb + kvh * a.c_sh + (int64_t)t0 * kTileBytes + 16 * lane;
+    auto fetch = [&](int k, uint32_t slot) {  // tile k, `src` at it
+      const uint32_t dst = ring + slot * kTileBytes + 16 * lane;
+      const int records = n - k * kTile;
+      if (records >= kTile) {
+#pragma unroll
+        for (int i = 0; i < kTileBytes / 512; ++i) cp_async16(dst + 512 * i, src + 512 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTileBytes / 512; ++i)
+          if (16 * lane + 512 * i < records * kRec) cp_async16(dst + 512 * i, src + 512 * i);
+      }
+      src += (int64_t)kWarps * kTileBytes;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (t0 + i * kWarps < t1) fetch(t0 + i * kWarps, i);
+      cp_async_commit();
+    }
     at.begin(a.qk_scale);
-    const int t0 = s_now.tile + warp, t1 = s_now.tile + s_now.share, n = s_now.n;
-    const int kvh = s_now.r / w.blocks, col0 = (s_now.r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
     const int whole = n - a.T + 1;  // tokens that every column sees
-    int sees[2];                    // tokens that the lane's columns see
+    int sees[2];                      // tokens that the lane's columns see
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       int hh, tt;
-      split(col0 + at.acc_col(j), hh, tt);
+      split(at.acc_col(j), hh, tt);
       sees[j] = whole + tt;
     }
-    // thread 0 looks for the CTA's next part: the item's next row, or another item (asked for now, used when
-    // this part's tiles are done)
-    unsigned item = 0;
-    bool next = false;
-    if (tid == 0 && !s_cut.own) {
-      DensePart s = s_now;
-      next = dense_next(a, w, s);
-      if (next)
-        s_next = s;
-      else if (s_cut.levels > 1)
-        item = s_cut.active + atomicAdd(w.taken, 1u);
-    }
-    __syncwarp();
-    uint32_t stage = 0;
+    uint32_t slot = 0;
     for (int k = t0; k < t1; k += kWarps) {
       cp_async_wait<kStages - 2>();
       __syncwarp();
       if ((k + 1) * kTile <= whole) {
         const uint32_t all[2] = {~0u, ~0u};
-        at.template tile<false>(ring + stage * kStageBytes, all);
+        at.template tile<false>(ring + slot * kTileBytes, all);
       } else {
         const uint32_t in[2] = {first_bits(sees[0] - k * kTile), first_bits(sees[1] - k * kTile)};
-        at.template tile<true>(ring + stage * kStageBytes, in);
+        at.template tile<true>(ring + slot * kTileBytes, in);
       }
       __syncwarp();
-      if (k + (kStages - 1) * kWarps < t1) fetch(n - (k + (kStages - 1) * kWarps) * kTile, stage == 0 ? kStages - 1 : stage - 1);
+      if (k + (kStages - 1) * kWarps < t1) fetch(k + (kStages - 1) * kWarps, slot == 0 ? kStages - 1 : slot - 1);
       cp_async_commit();
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
-    if (tid == 0) {
-      if (!next && s_cut.levels > 1) {
-        next = dense_item(a, w, s_cut, s_pre, item, s_next);
-        while (next && s_next.share <= 0) next = dense_item(a, w, s_cut, s_pre, s_cut.active + atomicAdd(w.taken, 1u), s_next);
-      }
-      s_more = next ? 1u : 0u;
-    }
 
-    // ---- the next part's first tiles are on their way while the 8 warps merge: warp c takes column c
-    __syncthreads();  // every warp is done with its tiles; s_next is known
-    const bool more = s_more != 0u;
-    if (more) fetch_first(s_next);
+    // ---- merge the 8 warps: warp c takes column c, a lane four dims
+    const bool begins = s.tile == 0, alone = begins && s.share == s.tiles;
+    __syncthreads();  // every warp is done with its ring
     at.finish(s_part + warp * kPartFloats, s_part + warp * kPartFloats + kCols * kD, ncol);
     __syncthreads();
-    const bool begins = s_now.tile == 0, alone = begins && s_now.share == s_now.tiles;
     int hh, tt;
-    split(col0 + warp, hh, tt);
-    const int64_t o_at = s_now.b * a.o.sb + (int64_t)(kvh * G + hh) * a.o.sh + tt * a.o.st;
+    split(warp, hh, tt);
+    const int64_t o_at = s.b * a.o.sb + (int64_t)(kvh * G + hh) * a.o.sh + tt * a.o.st;
     if (warp < ncol) {
       float f[kWarps], M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -439,92 +436,36 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
       if (alone) {
         store_out4(const_cast<void*>(a.o.p), a.out_f32, o_at, lane, A, L);
       } else {
-        float* part = w.parts + (2 * s_now.item + (begins ? 1 : 0)) * (int64_t)kPartFloats;
+        float* part = w.parts + (2 * cta + (begins ? 1 : 0)) * (int64_t)kPartFloats;
         reinterpret_cast<float4*>(part)[32 * warp + lane] = A;
         if (lane == 0) *reinterpret_cast<float2*>(part + kCols * kD + 2 * warp) = make_float2(M, L);
       }
     }
-    if (begins && tid == kDenseThreads - 1) {
-      uint2 sp = make_uint2(s_now.first, s_now.parts);
-      if (!s_cut.own) {  // the items of the row's first and last tile
-        const unsigned u = s_now.line - s_now.off + kRowUnits;
-        sp.x = s_now.item;
-        sp.y = item_of(s_cut, u + s_now.tiles - 1) - sp.x + 1;
+    if (!alone) {
+      unsigned first = s.first, parts = s.parts;
+      if (!s.own) {  // the CTAs of the row's first and last tile
+        const unsigned u = s.line - s.off + kRowUnits;
+        first = cta_of(s, u);
+        parts = cta_of(s, u + s.tiles - 1) - first + 1;
       }
-      w.spread[s_now.b * w.per_req + s_now.r] = make_uint2(sp.x, alone ? 0u : sp.y);
+      unsigned* ticket = w.tickets + s.b * w.per_req + s.r;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(ticket, 1u) == parts - 1 ? 1u : 0u;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        merge_parts<PAIR ? 6 : 4>(w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part,
+                                  const_cast<void*>(a.o.p), a.out_f32, o_at);
+        if (tid == 0) *ticket = 0u;
+      }
     }
-    if (!more) return;
-    load_q(s_next);
-    __syncthreads();  // s_part is a stage again
-    if (tid == 0) s_now = s_next;
+    if (s.own) return;
     __syncthreads();
+    if (tid == 0) s_last = dense_next(a, w, s) ? 1u : 0u;
+    __syncthreads();  // s_part is the ring again
+    if (!s_last) return;
   }
-}
-
-// Rows whose parts lie in the workspace: part v at src (v = 0) or src + (2 v - 1) kPartFloats.  One CTA per row; a
-// warp sums a lane's four dims of one column over its share of the parts, the shares are added in order.
-__global__ void __launch_bounds__(1024) dense_merge_kernel(const DenseArgs a, const DenseWork w) {
-  __shared__ __align__(16) float s_a[32][kD];
-  __shared__ float s_m[32], s_l[32];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *w.taken = 0u;
-  const uint2 sp = w.spread[blockIdx.x];
-  if (sp.y == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, parts = (int)sp.y;
-  const unsigned b = blockIdx.x / w.per_req, r = blockIdx.x - b * w.per_req;
-  const int G = a.HQ / a.HKV, kvh = r / w.blocks, col0 = (r - kvh * w.blocks) * kCols, ncol = min(kCols, G * a.T - col0);
-  const int col = warp % ncol, share = warp / ncol, shares = warps / ncol;
-  const float* src = w.parts + (2 * (int64_t)sp.x + 1) * kPartFloats;
-  float M = -INFINITY, L = 0.f;
-  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (share < shares) {
-    for (int v0 = share; v0 < parts; v0 += 8 * shares) {
-      float4 x[8];
-      float2 ml[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int v = v0 + i * shares;
-        ml[i] = make_float2(-INFINITY, 0.f);
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (v < parts) {
-          const float* p = src + (v ? 2 * v - 1 : 0) * (int64_t)kPartFloats;
-          ml[i] = __ldcg(reinterpret_cast<const float2*>(p + kCols * kD) + col);
-          x[i] = __ldcg(reinterpret_cast<const float4*>(p) + 32 * col + lane);
-        }
-      }
-      float nm = M;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) nm = fmaxf(nm, ml[i].x);
-      const float base = biased(nm), f = ex2(M - base);
-      M = nm;
-      L *= f;
-      A = make_float4(A.x * f, A.y * f, A.z * f, A.w * f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = ex2(ml[i].x - base);
-        L = fmaf(e, ml[i].y, L);
-        axpy(A, e, x[i]);
-      }
-    }
-  }
-  if (lane == 0) {
-    s_m[warp] = M;
-    s_l[warp] = L;
-  }
-  reinterpret_cast<float4*>(s_a[warp])[lane] = A;
-  __syncthreads();
-  if (warp >= ncol) return;
-  M = -INFINITY;
-  for (int i = 0; i < shares; ++i) M = fmaxf(M, s_m[warp + i * ncol]);
-  M = biased(M);
-  L = 0.f;
-  A = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < shares; ++i) {
-    const float e = ex2(s_m[warp + i * ncol] - M);
-    L = fmaf(e, s_l[warp + i * ncol], L);
-    axpy(A, e, reinterpret_cast<const float4*>(s_a[warp + i * ncol])[lane]);
-  }
-  const int c = col0 + warp, hh = a.T == 1 ? c : c / a.T, tt = c - hh * a.T;
-  store_out4(const_cast<void*>(a.o.p), a.out_f32, b * a.o.sb + (int64_t)(kvh * G + hh) * a.o.sh + tt * a.o.st, lane, A, L);
 }
 
 // ---------------------------------------------------------------- index lists and proxies
@@ -712,13 +653,7 @@ int launch_list(const ListArgs& a, int64_t rows, int S, const char* fn, cudaStre
   return oa_check_launch(fn);
 }
 
-// the hand-out counter, then every row's spread
-size_t spread_bytes(int64_t rows) { return (16 + (size_t)rows * sizeof(uint2) + 255) & ~size_t(255); }
-
-// a call has as many items as CTAs, or kLevels times as many when its cache can hold enough units for that
-size_t part_bytes(const DensePlan& p) {
-  return (size_t)p.grid * (p.most_units >= (int64_t)kLongShare * p.grid ? kLevels : 1) * 2 * kPartFloats * sizeof(float);
-}
+size_t ticket_bytes(int64_t rows) { return ((size_t)rows * sizeof(unsigned) + 255) & ~size_t(255); }
 
 }  // namespace
 }  // namespace oa
@@ -726,7 +661,7 @@ size_t part_bytes(const DensePlan& p) {
 extern "C" size_t oa_kv4_attention_workspace_bytes(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax) {
   if (B <= 0 || T <= 0 || HKV <= 0 || HQ < HKV || Lmax < 0) return 0;
   const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
-  return oa::spread_bytes(p.rows) + oa::part_bytes(p);
+  return oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
 }
 
 extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream) {
@@ -755,9 +690,10 @@ extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream)
   const size_t workspace_bytes = (size_t)std::max<int64_t>(g.workspace_bytes, 0);
   const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
   // units on the line (and 9 of them per row of the grid's widest product) are counted in 32 bits
-  OA_REQUIRE(p.most_units <= 0xffffffffll / 9 && p.most_units / p.rows * 8 * p.grid <= 0xffffffffll,
+  const int64_t most_units = p.rows * ((Lmax + oa::kTile - 1) / oa::kTile + 1 + oa::kRowUnits);
+  OA_REQUIRE(most_units <= 0xffffffffll / 9 && most_units / std::max<int64_t>(p.rows, 1) * 8 * p.grid <= 0xffffffffll,
              "%s: too many records (B * HKV * Lmax) for one call", fn);
-  const size_t need = oa::spread_bytes(p.rows) + oa::part_bytes(p);
+  const size_t need = oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
   OA_REQUIRE(workspace && workspace_bytes >= need && oa_aligned16(workspace),
              "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, workspace_bytes);
   oa::DenseWork w;
@@ -765,17 +701,12 @@ extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream)
   w.per_req = (unsigned)(HKV * p.blocks);
   w.rows = (unsigned)p.rows;
   w.cpr = (unsigned)(p.grid / p.rows);
-  w.taken = static_cast<unsigned*>(workspace);
-  w.spread = reinterpret_cast<uint2*>(static_cast<char*>(workspace) + 16);
-  w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + oa::spread_bytes(p.rows));
+  w.tickets = static_cast<unsigned*>(workspace);
+  w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + oa::ticket_bytes(p.rows));
   const auto kernel = HQ / HKV * T <= 4 ? &oa::dense_kernel<true> : &oa::dense_kernel<false>;
   const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(kernel), oa::kRingBytes, fn, true);
   if (rc != OA_OK) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  kernel<<<(unsigned)p.grid, oa::kDenseThreads, oa::kRingBytes, st>>>(a, w);
-  // no row can be spread where each has a CTA and at most one tile per warp
-  if (Lmax > oa::kWarps * oa::kTile || w.cpr == 0)
-    oa::dense_merge_kernel<<<w.rows, w.rows <= 296 ? 1024 : 256, 0, st>>>(a, w);
+  kernel<<<(unsigned)p.grid, oa::kDenseThreads, oa::kRingBytes, static_cast<cudaStream_t>(stream)>>>(a, w);
   return oa_check_launch(fn);
 }
 
