@@ -8,8 +8,10 @@
 // separately in fp32, as the eager expression does, so a caller that moves from it keeps its bits; the
 // result is rounded once to the rows' type.
 //
-// Layout: a half-warp owns one head row at a time, lane l dims 8l .. 8l+7 (16 bytes of bf16), so the
-// rotation's partner dims are R/16 lanes away and a quantisation group is eight lanes.
+// Layout: a half-warp owns one head row at a time, lane l dims 4l .. 4l+3 and 64 + 4l .. + 3: a full rotation (R =
+// 128) mixes dims of one lane, a byte of codes is one lane's, and loads and stores are 128-byte runs.  A warp takes a
+// token's rows two at a time ("slots": two query rows, or the K and the V row of one head, whose record it writes
+// whole), kSlots loads in flight; cos and sin stay in registers for all of them.
 #include "oa_kv4.cuh"
 
 namespace oa {
@@ -19,7 +21,7 @@ constexpr int kRowThreads = 256;
 
 struct RowArgs {
   Rows q, k, v;
-  Rows qo, ko;         // outputs (p is written)
+  Rows qo, ko;           // outputs (p is written)
   unsigned char* cache;  // records, or NULL
   int64_t c_sb, c_sh, Lmax;
   const float* cos;
@@ -34,160 +36,270 @@ struct RowArgs {
   float eps;
   int zero_q, zero_k;  // write zeros into padding rows
   int B, T, HQ, HKV;
-  int heads;   // head rows per token this call handles: HQ + HKV, + HKV values with a cache
-  int chunks;  // half-warps per token
+  int slots, per;      // slots of a token, slots a warp takes
 };
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  x[0] = bf_lo(w.x); x[1] = bf_hi(w.x); x[2] = bf_lo(w.y); x[3] = bf_hi(w.y);
-  x[4] = bf_lo(w.z); x[5] = bf_hi(w.z); x[6] = bf_lo(w.w); x[7] = bf_hi(w.w);
-}
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
+// The lane's part of a row: dims 4l .. (a) and 64 + 4l .. (b); p at dim 4l.  Held as loaded, so that several rows'
+// loads are in flight before the first is used.
+template <typename E>
+struct Quads;
+template <>
+struct Quads<__nv_bfloat16> {
+  uint2 a, b;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    a = __ldg(reinterpret_cast<const uint2*>(p));
+    b = __ldg(reinterpret_cast<const uint2*>(p + 64));
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = bf_lo(a.x); x[1] = bf_hi(a.x); x[2] = bf_lo(a.y); x[3] = bf_hi(a.y);
+    x[4] = bf_lo(b.x); x[5] = bf_hi(b.x); x[6] = bf_lo(b.y); x[7] = bf_hi(b.y);
+  }
+};
+template <>
+struct Quads<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const float4*>(p));
+    b = __ldg(reinterpret_cast<const float4*>(p + 64));
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return (uint32_t)f2bf_bits(lo) | ((uint32_t)f2bf_bits(hi) << 16);
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+__device__ __forceinline__ void store_quads(__nv_bfloat16* p, const float (&x)[8]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+  *reinterpret_cast<uint2*>(p + 64) = make_uint2(pack2(x[4], x[5]), pack2(x[6], x[7]));
 }
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ void store_quads(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 64) = make_float4(x[4], x[5], x[6], x[7]);
+}
+// cos or sin of the lane's dims (0 beyond R)
+__device__ __forceinline__ void load_table(const float* row, int R, int hl, float (&c)[8]) {
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4 a = 4 * hl < R ? *reinterpret_cast<const float4*>(row + 4 * hl) : none;
+  const float4 b = 64 + 4 * hl < R ? *reinterpret_cast<const float4*>(row + 64 + 4 * hl) : none;
+  c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
+  c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
 }
 
-// The half-warp's row x (bf16 values) quantised into one side of a record: `codes` its 64 code bytes,
-// `meta` its two (scale, offset) words.
-__device__ __forceinline__ void quantise_row(const float (&x)[8], unsigned char* codes, unsigned char* meta,
-                                             unsigned hmask) {
-  const int hl = threadIdx.x & 15;
-  float lo = x[0], hi = x[0];
-  bool finite = true;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) < INFINITY;
+// the lane's norm weights
+__device__ __forceinline__ void load_weights(const void* w, int w_f32, int hl, float (&wf)[8]) {
+  if (w_f32) {
+    Quads<float> v;
+    v.load(static_cast<const float*>(w) + 4 * hl);
+    v.get(wf);
+  } else {
+    Quads<__nv_bfloat16> v;
+    v.load(static_cast<const __nv_bfloat16*>(w) + 4 * hl);
+    v.get(wf);
   }
+}
+__device__ __forceinline__ void norm_row(float (&x)[8], const float (&wf)[8], float eps) {
+  float ss = 0.f;
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(hmask, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(hmask, hi, o));
-  }
-  const unsigned bad = __ballot_sync(hmask, !finite);
-  float s = bf_round(__fdiv_rn(hi - lo, 15.f));
-  const bool ok = (bad & (0xffu << (threadIdx.x & 24))) == 0u && s < INFINITY;  // a range past fp32 counts as infinite
-  if (!ok) s = __uint_as_float(0x7fc00000u);
-  uint32_t w[2];
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    w[h] = 0u;
+  for (int o = 8; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float inv = rsqrtf(ss * (1.f / kD) + eps);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * wf[i];
+}
+
+// FULL: R = 128, a lane's dims d and d + 64 rotate into each other.  Else the partner of quad i (of 32) is quad
+// i +- R/8, in another lane.  Called by whole warps.
+template <bool FULL>
+__device__ __forceinline__ void rotate_row(float (&x)[8], const float (&cs)[8], const float (&sn)[8], int R, int hl) {
+  if (FULL) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float c = s > 0.f ? fminf(rintf(__fdiv_rn(x[4 * h + i] - lo, s)), 15.f) : 0.f;
-      w[h] |= (uint32_t)c << (8 * i);
+      const float a = x[i], b = x[4 + i];
+      x[i] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, sn[i]));
+      x[4 + i] = __fadd_rn(__fmul_rn(b, cs[4 + i]), __fmul_rn(a, sn[4 + i]));
+    }
+    return;
+  }
+  const int h = R >> 3;  // quads in half a rotation
+  float y[8];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int quad = 16 * s + hl;
+    const bool first = quad < h, any = quad < 2 * h;
+    const int from = any ? (first ? quad + h : quad - h) : quad;
+    const int src = (threadIdx.x & 16) | (from & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = __shfl_sync(0xffffffffu, x[i], src), b = __shfl_sync(0xffffffffu, x[4 + i], src);
+      const float other = from < 16 ? a : b;
+      y[4 * s + i] = any ? __fadd_rn(__fmul_rn(x[4 * s + i], cs[4 * s + i]), __fmul_rn(first ? -other : other, sn[4 * s + i]))
+                         : x[4 * s + i];
     }
   }
-  // lane l < 8 holds the low nibbles of bytes 8l .. 8l+7, lane l + 8 their high nibbles: each writes four bytes
-  const bool upper = hl >= 8;
-  const uint32_t other = __shfl_xor_sync(hmask, upper ? w[0] : w[1], 8);
-  const uint32_t word = upper ? (other | (w[1] << 4)) : (w[0] | (other << 4));
-  *reinterpret_cast<uint32_t*>(codes + 8 * (hl & 7) + (upper ? 4 : 0)) = word;
-  if ((hl & 7) == 0) *reinterpret_cast<uint32_t*>(meta + (upper ? 4 : 0)) = pack2(s, ok ? lo : 0.f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = y[i];
 }
 
-template <typename E, bool CACHE, int HPW>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
-  const int lane = threadIdx.x & 31, hl = lane & 15;
-  const unsigned hmask = 0xffffu << (lane & 16);
-  const int64_t hw = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 4;
-  const int64_t token = hw / a.chunks;
-  if (token >= (int64_t)a.B * a.T) return;
-  const int chunk = (int)(hw - token * a.chunks);
-  const int64_t b = token / a.T, t = token - b * a.T;
-  const int64_t pos = per_request(a.start, b) + a.offset + t;
-  bool live = a.lens.p == nullptr || t < per_request(a.lens, b);
-  if (a.cos) live = live && pos >= 0 && pos < a.P;
-  const int h0 = chunk * HPW, h1 = min(h0 + HPW, a.heads);
-  const int d0 = 8 * hl;
+__device__ __forceinline__ uint32_t min_bf2(uint32_t a, uint32_t b) {  // NaN if either is
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
-  float x[HPW][8];
+// a / b rounded to nearest, from r = 1 / b rounded to nearest: the product, and one correction by its remainder
+// (Markstein's theorem), where nothing over- or underflows
+__device__ __forceinline__ float divide(float a, float b, float r) {
+  const float q = a * r;
+  return fmaf(fmaf(-q, b, a), r, q);
+}
+
+// The half-warp's row, as bf16x2 of dims (4l + i, 64 + 4l + i), into one side of a record.  The halves of the head lie
+// side by side, so one bf16x2 minimum and maximum serve both groups; NaN and infinities show in them.  Adding
+// 3 * 2^22 to a quotient rounds it to the nearest whole number, ties to even, in the low bits.  Scales near fp32's
+// smallest are lifted by 2^80 first.  Called by whole warps.
+__device__ __forceinline__ void quantise_row(const uint32_t (&v)[4], bool store, unsigned char* codes, unsigned char* meta, int hl) {
+  uint32_t lo2 = min_bf2(min_bf2(v[0], v[1]), min_bf2(v[2], v[3]));
+  uint32_t hi2 = max_bf2(max_bf2(v[0], v[1]), max_bf2(v[2], v[3]));
 #pragma unroll
-  for (int j = 0; j < HPW; ++j) {
-    const int h = h0 + j;
-    if (live && h < h1) {
-      const bool isq = h < a.HQ, isk = !isq && h < a.HQ + a.HKV;
-      const Rows& r = isq ? a.q : isk ? a.k : a.v;
-      const int64_t hh = isq ? h : isk ? h - a.HQ : h - a.HQ - a.HKV;
-      load8(static_cast<const E*>(r.p) + b * r.sb + hh * r.sh + t * r.st + d0, x[j]);
+  for (int o = 8; o >= 1; o >>= 1) {
+    lo2 = min_bf2(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
+    hi2 = max_bf2(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
+  }
+  constexpr float kRound = 12582912.f;  // 0x4b400000
+  // the codes are the low nibbles of 0x4b400000 + code, each shifted to its place; the constants' sum is taken away
+  constexpr uint32_t kBias = 0x4b400000u + (0x4b400000u << 8) + (0x4b400000u << 16) + (0x4b400000u << 24);
+  uint32_t word = 0u, out[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float lo = g ? bf_hi(lo2) : bf_lo(lo2), hi = g ? bf_hi(hi2) : bf_lo(hi2);
+    const uint32_t sz = pack2(divide(hi - lo, 15.f, 1.f / 15.f), lo);
+    const float s = bf_lo(sz);
+    const bool ok = s < INFINITY;  // a NaN, an infinity or a range past fp32 is not
+    const float lift = s < 0x1p-60f ? 0x1p80f : 1.f, ss = s * lift;
+    const float inv = s > 0.f ? __frcp_rn(ss) : 0.f;
+    uint32_t w = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float d = ((g ? bf_hi(v[i]) : bf_lo(v[i])) - lo) * lift;
+      w += __float_as_uint(fminf(divide(d, ss, inv), 15.f) + kRound) << (8 * i);
     }
+    word += ok ? (w - kBias) << (4 * g) : 0u;
+    out[g] = ok ? sz : 0x00007fc0u;
+  }
+  if (!store) return;
+  *reinterpret_cast<uint32_t*>(codes + 4 * hl) = word;
+  if (hl == 0) *reinterpret_cast<uint2*>(meta) = make_uint2(out[0], out[1]);
+}
+
+// One half-warp's rows h0, h0 + step, ... below h1 of one token, kSlots at a time: normalised, rotated, stored.  Rows
+// behind h1 are read as row h0 and dropped.  Called by whole warps (their half-warps differ in h0).
+template <typename E, bool FULL, int kSlots>
+__device__ __forceinline__ void rotate_rows(const E* p, int64_t sh, E* out, int64_t oh, int h0, int h1, int half, const void* weight,
+                                            const RowArgs& a, const float (&cs)[8], const float (&sn)[8], int hl) {
+  float wf[8];
+  if (weight) load_weights(weight, a.w_f32, hl, wf);
+  for (int h = h0; h < h1; h += 2 * kSlots) {
+    Quads<E> raw[kSlots];
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const int r = h + 2 * j + half;
+      raw[j].load(p + (r < h1 ? r : h0) * sh);
+    }
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j) {
+      const int r = h + 2 * j + half;
+      float x[8];
+      raw[j].get(x);
+      if (weight) norm_row(x, wf, a.eps);
+      rotate_row<FULL>(x, cs, sn, a.R, hl);
+      if (r < h1) store_quads(out + r * oh, x);
+    }
+  }
+}
+
+// Slots of a token: with a cache, slot i < HKV is K (first half-warp) and V (second) of head i, then two query rows
+// each; else two query rows each, then two key rows each.
+template <typename E, bool CACHE, bool FULL, int kSlots>
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
+  const int lane = threadIdx.x & 31, hl = lane & 15, half = lane >> 4;
+  const unsigned token = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  if (token >= (unsigned)a.B * a.T) return;
+  const unsigned b = a.T == 1 ? token : token / a.T, t = token - b * a.T;
+  const int64_t pos = per_request(a.start, b) + a.offset + t;
+  bool live = a.lens.p == nullptr || (int64_t)t < per_request(a.lens, b);
+  if (a.cos) live = live && pos >= 0 && pos < a.P;
+  const int s0 = blockIdx.y * a.per, s1 = min(s0 + a.per, a.slots);
+  const E* q = static_cast<const E*>(a.q.p) + b * a.q.sb + t * a.q.st + 4 * hl;
+  E* qo = static_cast<E*>(const_cast<void*>(a.qo.p)) + b * a.qo.sb + t * a.qo.st + 4 * hl;
+  // this warp's query rows [q0, q1) and key (or key and value) rows [k0, k1)
+  const int nq = (a.HQ + 1) / 2;
+  const int q0 = 2 * (CACHE ? max(0, s0 - a.HKV) : min(s0, nq)), q1 = min(a.HQ, 2 * (CACHE ? max(0, s1 - a.HKV) : s1));
+  const int k0 = CACHE ? s0 : 2 * max(0, s0 - nq), k1 = min(a.HKV, CACHE ? s1 : 2 * max(0, s1 - nq));
+  if (!live) {
+    const float zero[8] = {};
+    if (a.zero_q)
+      for (int h = q0 + half; h < q1; h += 2) store_quads(qo + h * a.qo.sh, zero);
+    if (!CACHE && a.zero_k) {
+      E* ko = static_cast<E*>(const_cast<void*>(a.ko.p)) + b * a.ko.sb + t * a.ko.st + 4 * hl;
+      for (int h = k0 + half; h < k1; h += 2) store_quads(ko + h * a.ko.sh, zero);
+    }
+    return;
   }
   float cs[8], sn[8];
-  const bool rot = a.cos && d0 < a.R;
-  int src = hl;
-  float sign = 0.f;
-  if (live && rot) {
-    load8(a.cos + pos * a.R + d0, cs);
-    load8(a.sin + pos * a.R + d0, sn);
-    const bool first = d0 < (a.R >> 1);
-    src = first ? hl + (a.R >> 4) : hl - (a.R >> 4);
-    sign = first ? -1.f : 1.f;
+  if (a.cos) {
+    load_table(a.cos + pos * a.R, a.R, hl, cs);
+    load_table(a.sin + pos * a.R, a.R, hl, sn);
   }
+  if (CACHE && k0 < k1) {
+    const bool keeps = pos >= 0 && pos < a.Lmax;
+    const Rows& r = half ? a.v : a.k;
+    const E* p = static_cast<const E*>(r.p) + b * r.sb + t * r.st + 4 * hl;
+    const int64_t sh = r.sh;
+    unsigned char* codes = a.cache + b * a.c_sb + pos * kRec + (half ? kRecV : 0);
+    unsigned char* meta = a.cache + b * a.c_sb + pos * kRec + kRecMeta + (half ? 8 : 0);
+    float wf[8];
+    if (a.wk) load_weights(a.wk, a.w_f32, hl, wf);
+    for (int h = k0; h < k1; h += kSlots) {
+      Quads<E> raw[kSlots];
 #pragma unroll
-  for (int j = 0; j < HPW; ++j) {
-    const int h = h0 + j;
-    if (h >= h1) continue;
-    const bool isq = h < a.HQ, isk = !isq && h < a.HQ + a.HKV;
-    const int64_t hh = isq ? h : isk ? h - a.HQ : h - a.HQ - a.HKV;
-    if (live && (isq || isk)) {
-      const void* w = isq ? a.wq : a.wk;
-      if (w != nullptr) {
-        float ss = 0.f;
+      for (int j = 0; j < kSlots; ++j) raw[j].load(p + (h + j < k1 ? h + j : k0) * sh);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[j][i], x[j][i], ss);
+      for (int j = 0; j < kSlots; ++j) {
+        if (h + j >= k1) break;
+        float x[8];
+        raw[j].get(x);
+        uint32_t v[4];
 #pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) ss += __shfl_xor_sync(hmask, ss, o);
-        const float inv = rsqrtf(ss * (1.f / kD) + a.eps);
-        float wf[8];
-        if (a.w_f32)
-          load8(static_cast<const float*>(w) + d0, wf);
-        else
-          load8(static_cast<const __nv_bfloat16*>(w) + d0, wf);
+        for (int i = 0; i < 4; ++i) v[i] = pack2(x[i], x[4 + i]);
+        if (a.cos) {  // the V rows of the warp go through the shuffles with the K rows and come out as they were
+          if (a.wk) norm_row(x, wf, a.eps);
+          rotate_row<FULL>(x, cs, sn, a.R, hl);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] = x[j][i] * inv * wf[i];
-      }
-      if (a.cos) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float other = __shfl_sync(hmask, x[j][i], (lane & 16) | src);
-          if (rot) x[j][i] = __fadd_rn(__fmul_rn(x[j][i], cs[i]), __fmul_rn(sign * other, sn[i]));
+          for (int i = 0; i < 4; ++i) v[i] = half ? v[i] : pack2(x[i], x[4 + i]);  // the cache holds bf16 rows
         }
+        quantise_row(v, keeps, codes + (h + j) * a.c_sh, meta + (h + j) * a.c_sh, hl);
       }
-    }
-    if (isq || (isk && !CACHE)) {
-      const Rows& o = isq ? a.qo : a.ko;
-      E* dst = static_cast<E*>(const_cast<void*>(o.p)) + b * o.sb + hh * o.sh + t * o.st + d0;
-      if (live) {
-        store8(dst, x[j]);
-      } else if (isq ? a.zero_q : a.zero_k) {
-        const float zero[8] = {};
-        store8(dst, zero);
-      }
-    } else if (CACHE && live && pos >= 0 && pos < a.Lmax) {
-      unsigned char* rec = a.cache + b * a.c_sb + hh * a.c_sh + pos * kRec;
-      if (isk) {  // the cache holds bf16 rows' values: round the rotated key first
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[j][i] = bf_round(x[j][i]);
-      }
-      quantise_row(x[j], rec + (isk ? 0 : kRecV), rec + kRecMeta + (isk ? 0 : 8), hmask);
     }
   }
+  if (!CACHE && k0 < k1) {
+    const E* k = static_cast<const E*>(a.k.p) + b * a.k.sb + t * a.k.st + 4 * hl;
+    E* ko = static_cast<E*>(const_cast<void*>(a.ko.p)) + b * a.ko.sb + t * a.ko.st + 4 * hl;
+    rotate_rows<E, FULL, kSlots>(k, a.k.sh, ko, a.ko.sh, k0, k1, half, a.wk, a, cs, sn, hl);
+  }
+  if (q0 < q1) rotate_rows<E, FULL, kSlots>(q, a.q.sh, qo, a.qo.sh, q0, q1, half, a.wq, a, cs, sn, hl);
 }
 
-// Records back to rows: a half-warp per record, lane l the code words l (dims 4l.. and 64 + 4l..).
+// Records back to rows: a half-warp per record, lane l the code words l (dims 4l.. and 64 + 4l..), kRecords in flight.
 struct UnpackArgs {
   const unsigned char* cache;
   int64_t c_sb, c_sh, Lmax;
@@ -196,70 +308,82 @@ struct UnpackArgs {
   Rows ko, vo;
   int zero_k, zero_v;
   int B, T, HKV;
+  unsigned ctas;  // for one head's T records
 };
 
-template <typename E>
-__device__ __forceinline__ void store4(E* p, float a, float b, float c, float d);
-template <>
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack2(a, b), pack2(c, d));
-}
-template <>
-__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
-  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
-}
-
-template <typename E>
-__device__ __forceinline__ void unpack_row(uint32_t w, uint32_t m0, uint32_t m1, E* dst) {
+// a word's eight codes as values: bytes 0..3 low nibbles, then high ones.  0x4b000000 + n is the float 2^23 + n.
+__device__ __forceinline__ void unpack_word(uint32_t w, uint32_t m0, uint32_t m1, float (&v)[8]) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
   const float s0 = bf_lo(m0), z0 = bf_hi(m0), s1 = bf_lo(m1), z1 = bf_hi(m1);
-  float v[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = fmaf(s0, (float)((w >> (8 * i)) & 15u), z0);
-    v[4 + i] = fmaf(s1, (float)((w >> (8 * i + 4)) & 15u), z1);
+    v[i] = fmaf(s0, __uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 + i)) - 8388608.f, z0);
+    v[4 + i] = fmaf(s1, __uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 + i)) - 8388608.f, z1);
   }
-  store4(dst, v[0], v[1], v[2], v[3]);
-  store4(dst + 64, v[4], v[5], v[6], v[7]);
 }
+
+constexpr int kRecords = 2;
 
 template <typename E>
 __global__ void __launch_bounds__(kRowThreads) unpack_kernel(const UnpackArgs a) {
   const int hl = threadIdx.x & 15;
-  const int64_t hw = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) >> 4;
-  if (hw >= (int64_t)a.B * a.HKV * a.T) return;
-  const int64_t bh = hw / a.T, t = hw - bh * a.T;
-  const int64_t b = bh / a.HKV, h = bh - b * a.HKV;
-  const int64_t pos = per_request(a.start, b) + a.offset + t;
-  const bool live = (a.lens.p == nullptr || t < per_request(a.lens, b)) && pos >= 0 && pos < a.Lmax;
-  E* kd = static_cast<E*>(const_cast<void*>(a.ko.p)) + b * a.ko.sb + h * a.ko.sh + t * a.ko.st + 4 * hl;
-  E* vd = static_cast<E*>(const_cast<void*>(a.vo.p)) + b * a.vo.sb + h * a.vo.sh + t * a.vo.st + 4 * hl;
-  if (live) {
-    const unsigned char* rec = a.cache + b * a.c_sb + h * a.c_sh + pos * kRec;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(rec + 4 * hl);
-    const uint32_t vw = *reinterpret_cast<const uint32_t*>(rec + kRecV + 4 * hl);
-    const uint4 m = *reinterpret_cast<const uint4*>(rec + kRecMeta);
-    unpack_row(kw, m.x, m.y, kd);
-    unpack_row(vw, m.z, m.w, vd);
-  } else {
-    if (a.zero_k) store4(kd, 0.f, 0.f, 0.f, 0.f), store4(kd + 64, 0.f, 0.f, 0.f, 0.f);
-    if (a.zero_v) store4(vd, 0.f, 0.f, 0.f, 0.f), store4(vd + 64, 0.f, 0.f, 0.f, 0.f);
+  const unsigned head = blockIdx.x / a.ctas, b = head / a.HKV, h = head - b * a.HKV;
+  const unsigned hw = ((blockIdx.x - head * a.ctas) * kRowThreads + threadIdx.x) >> 4;
+  const int64_t first = per_request(a.start, b) + a.offset;
+  const int64_t len = a.lens.p ? per_request(a.lens, b) : a.T;
+  const unsigned char* rec = a.cache + b * a.c_sb + h * a.c_sh;
+  uint32_t kw[kRecords], vw[kRecords];
+  uint4 m[kRecords];
+  bool live[kRecords];
+#pragma unroll
+  for (int i = 0; i < kRecords; ++i) {
+    const int64_t t = (int64_t)hw * kRecords + i, pos = first + t;
+    live[i] = t < a.T && t < len && pos >= 0 && pos < a.Lmax;
+    kw[i] = vw[i] = 0u;
+    m[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (live[i]) {
+      const unsigned char* p = rec + pos * kRec;
+      kw[i] = *reinterpret_cast<const uint32_t*>(p + 4 * hl);
+      vw[i] = *reinterpret_cast<const uint32_t*>(p + kRecV + 4 * hl);
+      m[i] = *reinterpret_cast<const uint4*>(p + kRecMeta);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRecords; ++i) {  // what is not live reads as zeros
+    const int64_t t = (int64_t)hw * kRecords + i;
+    if (t >= a.T) break;
+    float v[8];
+    if (live[i] || a.zero_k) {
+      unpack_word(kw[i], m[i].x, m[i].y, v);
+      store_quads(static_cast<E*>(const_cast<void*>(a.ko.p)) + b * a.ko.sb + h * a.ko.sh + t * a.ko.st + 4 * hl, v);
+    }
+    if (live[i] || a.zero_v) {
+      unpack_word(vw[i], m[i].z, m[i].w, v);
+      store_quads(static_cast<E*>(const_cast<void*>(a.vo.p)) + b * a.vo.sb + h * a.vo.sh + t * a.vo.st + 4 * hl, v);
+    }
   }
 }
 
 // ---------------------------------------------------------------- host side
+template <typename E, bool CACHE, bool FULL>
+int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
+  a.slots = (CACHE ? a.HKV : (a.HKV + 1) / 2) + (a.HQ + 1) / 2;
+  const int64_t tokens = (int64_t)a.B * a.T;
+  if (tokens == 0 || a.slots == 0) return OA_OK;
+  OA_REQUIRE(tokens <= 0x7fffffff, "%s: too many rows", fn);
+  // a warp keeps a token's table entries for as many slots as still leave 24 warps to each of 148 SMs
+  a.per = (int)std::min<int64_t>(a.slots, std::max<int64_t>(1, tokens * a.slots / (148 * 24)));
+  while ((a.slots + a.per - 1) / a.per > 65535) a.per *= 2;
+  const dim3 grid((unsigned)((tokens + kRowThreads / 32 - 1) / (kRowThreads / 32)), (a.slots + a.per - 1) / a.per);
+  if (a.per >= 4)
+    rows_kernel<E, CACHE, FULL, 4><<<grid, kRowThreads, 0, st>>>(a);
+  else
+    rows_kernel<E, CACHE, FULL, 1><<<grid, kRowThreads, 0, st>>>(a);
+  return oa_check_launch(fn);
+}
 template <typename E, bool CACHE>
 int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
-  if (a.B == 0 || a.T == 0 || a.heads == 0) return OA_OK;
-  const int hpw = (int64_t)a.B * a.T * a.heads >= 148 * 512 ? 4 : 1;
-  a.chunks = (a.heads + hpw - 1) / hpw;
-  const int64_t hws = (int64_t)a.B * a.T * a.chunks;
-  const int64_t grid = (hws * 16 + kRowThreads - 1) / kRowThreads;
-  OA_REQUIRE(grid <= 0x7fffffff, "%s: too many rows", fn);
-  if (hpw == 4)
-    rows_kernel<E, CACHE, 4><<<(unsigned)grid, kRowThreads, 0, st>>>(a);
-  else
-    rows_kernel<E, CACHE, 1><<<(unsigned)grid, kRowThreads, 0, st>>>(a);
-  return oa_check_launch(fn);
+  return a.cos == nullptr || a.R == kD ? launch_rows<E, CACHE, true>(a, fn, st) : launch_rows<E, CACHE, false>(a, fn, st);
 }
 
 // The parts of a block that oa_qk_norm_rope and oa_kv4_append share.
@@ -303,7 +427,6 @@ extern "C" int oa_qk_norm_rope(const oa_qk_norm_rope_args* args, void* stream) {
   a.zero_k = g.zero_k != 0;
   a.offset = g.offset;
   a.B = (int)B; a.T = (int)T; a.HQ = (int)HQ; a.HKV = (int)HKV;
-  a.heads = (int)(HQ + HKV);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return g.dtype == OA_F32 ? oa::launch_rows<float, false>(a, fn, st) : oa::launch_rows<__nv_bfloat16, false>(a, fn, st);
 }
@@ -333,7 +456,6 @@ extern "C" int oa_kv4_append(const oa_kv4_append_args* args, void* stream) {
   OA_TRY(oa_take_index(fn, "lens", g.lens, B, false, &a.lens));
   a.offset = g.offset;
   a.B = (int)B; a.T = (int)T; a.HQ = (int)HQ; a.HKV = (int)HKV;
-  a.heads = (int)(HQ + 2 * HKV);
   return oa::launch_rows<__nv_bfloat16, true>(a, fn, static_cast<cudaStream_t>(stream));
 }
 
@@ -356,12 +478,14 @@ extern "C" int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream) {
   a.zero_v = g.zero_v != 0;
   a.B = (int)B; a.T = (int)T; a.HKV = (int)HKV;
   if (B == 0 || T == 0 || HKV == 0) return OA_OK;
-  const int64_t grid = (B * T * HKV * 16 + oa::kRowThreads - 1) / oa::kRowThreads;
-  OA_REQUIRE(grid <= 0x7fffffff, "%s: too many rows", fn);
+  const int64_t per_cta = oa::kRowThreads / 16 * oa::kRecords, ctas = (T + per_cta - 1) / per_cta;
+  OA_REQUIRE(B * HKV <= 0x7fffffff / ctas, "%s: too many rows", fn);
+  a.ctas = (unsigned)ctas;
+  const unsigned grid = (unsigned)(B * HKV * ctas);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (g.dtype == OA_F32)
-    oa::unpack_kernel<float><<<(unsigned)grid, oa::kRowThreads, 0, st>>>(a);
+    oa::unpack_kernel<float><<<grid, oa::kRowThreads, 0, st>>>(a);
   else
-    oa::unpack_kernel<__nv_bfloat16><<<(unsigned)grid, oa::kRowThreads, 0, st>>>(a);
+    oa::unpack_kernel<__nv_bfloat16><<<grid, oa::kRowThreads, 0, st>>>(a);
   return oa_check_launch(fn);
 }
