@@ -54,6 +54,13 @@ struct Quads<__nv_bfloat16> {
     x[0] = bf_lo(a.x); x[1] = bf_hi(a.x); x[2] = bf_lo(a.y); x[3] = bf_hi(a.y);
     x[4] = bf_lo(b.x); x[5] = bf_hi(b.x); x[6] = bf_lo(b.y); x[7] = bf_hi(b.y);
   }
+  // bf16x2 of dims (4l + i, 64 + 4l + i)
+  __device__ __forceinline__ void pairs(uint32_t (&v)[4]) const {
+    v[0] = __byte_perm(a.x, b.x, 0x5410);
+    v[1] = __byte_perm(a.x, b.x, 0x7632);
+    v[2] = __byte_perm(a.y, b.y, 0x5410);
+    v[3] = __byte_perm(a.y, b.y, 0x7632);
+  }
 };
 template <>
 struct Quads<float> {
@@ -66,6 +73,7 @@ struct Quads<float> {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
     x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
+  __device__ __forceinline__ void pairs(uint32_t (&v)[4]) const {}  // caches take bf16 rows
 };
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -156,18 +164,57 @@ __device__ __forceinline__ uint32_t max_bf2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// a / b rounded to nearest, from r = 1 / b rounded to nearest: the product, and one correction by its remainder
-// (Markstein's theorem), where nothing over- or underflows
+// a / b from r, 1 / b to within an ulp: the product, and one correction by its remainder, where nothing over- or
+// underflows.  Exact where the quotient is a float (a tie between two codes among them), else within an ulp of it.
 __device__ __forceinline__ float divide(float a, float b, float r) {
   const float q = a * r;
   return fmaf(fmaf(-q, b, a), r, q);
+}
+
+__device__ __forceinline__ float reciprocal(float x) {  // of a normal number with a normal reciprocal, within an ulp
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return fmaf(fmaf(-x, r, 1.f), r, r);
+}
+
+// Scale of the group in the low (0) or high (1) halves of the two packed extremes.
+__device__ __forceinline__ float group_scale(uint32_t lo2, uint32_t hi2, int g) {
+  const float lo = g ? bf_hi(lo2) : bf_lo(lo2), hi = g ? bf_hi(hi2) : bf_lo(hi2);
+  return bf_round(divide(hi - lo, 15.f, 1.f / 15.f));
+}
+// The lane's eight codes as four bytes, and both groups' (scale, offset) words.  kLift: some scale is near fp32's
+// smallest numbers (or zero).
+template <bool kLift>
+__device__ __forceinline__ void code_groups(const uint32_t (&v)[4], uint32_t lo2, float s0, float s1, uint32_t& word,
+                                            uint32_t (&out)[2]) {
+  constexpr float kRound = 12582912.f;  // 0x4b400000: a code is the sum's lowest byte
+  word = 0u;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float lo = g ? bf_hi(lo2) : bf_lo(lo2), s = g ? s1 : s0;
+    const bool ok = s < INFINITY;  // a NaN, an infinity or a range past fp32 is not
+    const float lift = kLift && s < 0x1p-60f ? 0x1p80f : 1.f, ss = kLift ? s * lift : s;
+    const float inv = !kLift || s > 0.f ? reciprocal(ss) : 0.f;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d = (g ? bf_hi(v[i]) : bf_lo(v[i])) - lo;
+      if (kLift) d *= lift;
+      float q = divide(d, ss, inv);
+      if (kLift) q = fminf(q, 15.f);  // a normal scale is off by 2^-9 at most, its quotients stay under 15.1
+      w[i] = __float_as_uint(q + kRound);
+    }
+    const uint32_t codes4 = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+    word |= ok ? codes4 << (4 * g) : 0u;
+    out[g] = ok ? pack2(s, lo) : 0x00007fc0u;
+  }
 }
 
 // The half-warp's row, as bf16x2 of dims (4l + i, 64 + 4l + i), into one side of a record.  The halves of the head lie
 // side by side, so one bf16x2 minimum and maximum serve both groups; NaN and infinities show in them.  Adding
 // 3 * 2^22 to a quotient rounds it to the nearest whole number, ties to even, in the low bits.  Scales near fp32's
 // smallest are lifted by 2^80 first.  Called by whole warps.
-__device__ __forceinline__ void quantise_row(const uint32_t (&v)[4], bool store, unsigned char* codes, unsigned char* meta, int hl) {
+__device__ __forceinline__ void quantise_row(const uint32_t (&v)[4], unsigned char* codes, int meta, int hl) {
   uint32_t lo2 = min_bf2(min_bf2(v[0], v[1]), min_bf2(v[2], v[3]));
   uint32_t hi2 = max_bf2(max_bf2(v[0], v[1]), max_bf2(v[2], v[3]));
 #pragma unroll
@@ -175,30 +222,14 @@ __device__ __forceinline__ void quantise_row(const uint32_t (&v)[4], bool store,
     lo2 = min_bf2(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
     hi2 = max_bf2(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
   }
-  constexpr float kRound = 12582912.f;  // 0x4b400000
-  // the codes are the low nibbles of 0x4b400000 + code, each shifted to its place; the constants' sum is taken away
-  constexpr uint32_t kBias = 0x4b400000u + (0x4b400000u << 8) + (0x4b400000u << 16) + (0x4b400000u << 24);
-  uint32_t word = 0u, out[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const float lo = g ? bf_hi(lo2) : bf_lo(lo2), hi = g ? bf_hi(hi2) : bf_lo(hi2);
-    const uint32_t sz = pack2(divide(hi - lo, 15.f, 1.f / 15.f), lo);
-    const float s = bf_lo(sz);
-    const bool ok = s < INFINITY;  // a NaN, an infinity or a range past fp32 is not
-    const float lift = s < 0x1p-60f ? 0x1p80f : 1.f, ss = s * lift;
-    const float inv = s > 0.f ? __frcp_rn(ss) : 0.f;
-    uint32_t w = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float d = ((g ? bf_hi(v[i]) : bf_lo(v[i])) - lo) * lift;
-      w += __float_as_uint(fminf(divide(d, ss, inv), 15.f) + kRound) << (8 * i);
-    }
-    word += ok ? (w - kBias) << (4 * g) : 0u;
-    out[g] = ok ? sz : 0x00007fc0u;
-  }
-  if (!store) return;
+  uint32_t word, out[2];
+  const float s0 = group_scale(lo2, hi2, 0), s1 = group_scale(lo2, hi2, 1);
+  if (__any_sync(0xffffffffu, fminf(s0, s1) < 0x1p-60f))
+    code_groups<true>(v, lo2, s0, s1, word, out);
+  else
+    code_groups<false>(v, lo2, s0, s1, word, out);
   *reinterpret_cast<uint32_t*>(codes + 4 * hl) = word;
-  if (hl == 0) *reinterpret_cast<uint2*>(meta) = make_uint2(out[0], out[1]);
+  if (hl == 0) *reinterpret_cast<uint2*>(codes + meta) = make_uint2(out[0], out[1]);
 }
 
 // One half-warp's rows h0, h0 + step, ... below h1 of one token, kSlots at a time: normalised, rotated, stored.  Rows
@@ -260,35 +291,40 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
     load_table(a.cos + pos * a.R, a.R, hl, cs);
     load_table(a.sin + pos * a.R, a.R, hl, sn);
   }
-  if (CACHE && k0 < k1) {
-    const bool keeps = pos >= 0 && pos < a.Lmax;
+  if (CACHE && k0 < k1 && pos >= 0 && pos < a.Lmax) {
     const Rows& r = half ? a.v : a.k;
-    const E* p = static_cast<const E*>(r.p) + b * r.sb + t * r.st + 4 * hl;
+    const E* p = static_cast<const E*>(r.p) + b * r.sb + t * r.st + 4 * hl + k0 * r.sh;
     const int64_t sh = r.sh;
-    unsigned char* codes = a.cache + b * a.c_sb + pos * kRec + (half ? kRecV : 0);
-    unsigned char* meta = a.cache + b * a.c_sb + pos * kRec + kRecMeta + (half ? 8 : 0);
+    unsigned char* codes = a.cache + b * a.c_sb + k0 * a.c_sh + pos * kRec + (half ? kRecV : 0);
+    const int meta = half ? kRecMeta + 8 - kRecV : kRecMeta;
     float wf[8];
     if (a.wk) load_weights(a.wk, a.w_f32, hl, wf);
-    for (int h = k0; h < k1; h += kSlots) {
+    auto write = [&](const Quads<E>& raw) {  // one head's K and V row into its record
+      uint32_t v[4];
+      raw.pairs(v);
+      if (a.cos) {  // the V rows of the warp go through the shuffles with the K rows and come out as they were
+        float x[8];
+        raw.get(x);
+        if (a.wk) norm_row(x, wf, a.eps);
+        rotate_row<FULL>(x, cs, sn, a.R, hl);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = half ? v[i] : pack2(x[i], x[4 + i]);  // the cache holds bf16 rows
+      }
+      quantise_row(v, codes, meta, hl);
+      codes += a.c_sh;
+    };
+    int h = k0;
+    for (; h + kSlots <= k1; h += kSlots) {
       Quads<E> raw[kSlots];
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) raw[j].load(p + (h + j < k1 ? h + j : k0) * sh);
+      for (int j = 0; j < kSlots; ++j, p += sh) raw[j].load(p);
 #pragma unroll
-      for (int j = 0; j < kSlots; ++j) {
-        if (h + j >= k1) break;
-        float x[8];
-        raw[j].get(x);
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = pack2(x[i], x[4 + i]);
-        if (a.cos) {  // the V rows of the warp go through the shuffles with the K rows and come out as they were
-          if (a.wk) norm_row(x, wf, a.eps);
-          rotate_row<FULL>(x, cs, sn, a.R, hl);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = half ? v[i] : pack2(x[i], x[4 + i]);  // the cache holds bf16 rows
-        }
-        quantise_row(v, keeps, codes + (h + j) * a.c_sh, meta + (h + j) * a.c_sh, hl);
-      }
+      for (int j = 0; j < kSlots; ++j) write(raw[j]);
+    }
+    for (; h < k1; ++h, p += sh) {
+      Quads<E> raw;
+      raw.load(p);
+      write(raw);
     }
   }
   if (!CACHE && k0 < k1) {
