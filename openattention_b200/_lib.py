@@ -101,13 +101,17 @@ def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise RuntimeError with the library's message on failure."""
     status = getattr(_lib or load(), name)(*args)
     if status != 0:
-        msg = load().oa_last_error_string().decode(errors="replace")
-        raise RuntimeError(f"{name} failed (status {status}): {msg}")
+        fail(name, status)
 
 
-def call_block(name: str, stream: int, *fields) -> None:
-    """call() of an entry that takes its arguments in a block."""
-    call(name, BLOCKS[name].pack(*fields), stream)
+def fail(name: str, status: int):
+    msg = load().oa_last_error_string().decode(errors="replace")
+    raise RuntimeError(f"{name} failed (status {status}): {msg}")
+
+
+def block_entry(name: str):
+    """(pack, function) of an entry that takes its arguments in a block: function(pack(*fields), stream) -> status."""
+    return BLOCKS[name].pack, getattr(load(), name)
 
 
 def ptr(t) -> int:

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .geometry import D, HKV
-from .rotary import _call, _CODE, _current_stream, _index, _like, _rows, _same_device, _table, _weights
+from .rotary import _call, _CODE, _current_stream, _device_of, _index, _like, _rows, _same_device, _table, _weights
 
 REC = 144
 
@@ -49,10 +49,8 @@ def append(cache, k, v, start, *, offset=0, lens=None):
     """Writes k, v (B, hkv, T, 128) bf16 into the cache (B, hkv, Lmax, 144): row i of request b at position
     start[b] + offset + i.  Rows i >= lens[b] (default T) and positions outside [0, Lmax) write nothing.
     Calls that write the same positions must be ordered (one stream, or events)."""
-    fc, dev = _cache(cache), cache.get_device()
-    fk, fv = _rows("k", k, torch.bfloat16), _rows("v", v, torch.bfloat16)
-    _same_device(dev, k=k, v=v)
-    _call(dev, "oa_kv4_append", *_NO_ROWS, *fk, *fv, *_NO_ROWS, *fc, 0, 0, 0, 0, *_index("start", start, dev),
+    fc, dev, bf = _cache(cache), cache.get_device(), torch.bfloat16
+    _call(dev, "oa_kv4_append", *_NO_ROWS, *_rows("k", k, bf, dev), *_rows("v", v, bf, dev), *_NO_ROWS, *fc, 0, 0, 0, 0, *_index("start", start, dev),
           *_index("lens", lens, dev), 0, 0, offset, _lib.OA_F32, 0, 0.0)
 
 
@@ -63,14 +61,13 @@ def rope_append(cache, q, k, v, cos, sin, start, *, offset=0, lens=None, q_weigh
     whose position is outside the tables or behind lens are padding (no record; q as in qk_norm_rope), rows at
     positions past the cache rotate q and write no record."""
     fc, dev, bf = _cache(cache), cache.get_device(), torch.bfloat16
-    fq, fk, fv = _rows("q", q, bf), _rows("k", k, bf), _rows("v", v, bf)
+    fq = _rows("q", q, bf, dev)
     zero = q_out is None
     if zero:
         q_out = _like(q)
-    _same_device(dev, q=q, k=k, v=v, q_out=q_out)
     qp, kp, wd = _weights(q_weight, k_weight, bf, dev)
-    _call(dev, "oa_kv4_append", *fq, *fk, *fv, *_rows("q_out", q_out, bf), *fc, *_table(cos, sin, dev),
-          *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, wd, zero, eps)
+    _call(dev, "oa_kv4_append", *fq, *_rows("k", k, bf, dev), *_rows("v", v, bf, dev), *_rows("q_out", q_out, bf, dev), *fc,
+          *_table(cos, sin, dev), *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, wd, zero, eps)
     return q_out
 
 
@@ -79,9 +76,9 @@ def unpack(cache, start, T, *, offset=0, lens=None, out_dtype=torch.bfloat16, k_
     i < T.  Rows i >= lens[b] and positions outside the cache are zero in outputs that this call allocates and
     left as they were in k_out / v_out."""
     fc, dev = _cache(cache), cache.get_device()
-    shape = (cache.shape[0], cache.shape[1], T, D)
-    _same_device(dev, k_out=k_out, v_out=v_out)
+    shape = (*cache.shape[:2], T, D)
     if k_out is not None or v_out is not None:
+        _same_device(dev, k_out=k_out, v_out=v_out)
         out_dtype = (v_out if k_out is None else k_out).dtype
     if T < 0 or out_dtype not in _CODE:
         raise RuntimeError(f"T must be >= 0 and the outputs bf16 or fp32, got {T}, {out_dtype}")
@@ -89,10 +86,10 @@ def unpack(cache, start, T, *, offset=0, lens=None, out_dtype=torch.bfloat16, k_
     if zk:
         k_out = torch.empty(shape, dtype=out_dtype, device=cache.device)
     if zv:
-        v_out = torch.empty(shape, dtype=out_dtype, device=cache.device)
-    if k_out.shape != shape:
+        v_out = _like(k_out)
+    if not zk and k_out.shape != shape:
         raise RuntimeError(f"k_out must be {shape}, got {tuple(k_out.shape)}")
-    _call(dev, "oa_kv4_unpack", *fc, *_rows("k_out", k_out, out_dtype), *_rows("v_out", v_out, out_dtype),
+    _call(dev, "oa_kv4_unpack", *fc, *_rows("k_out", k_out, out_dtype, dev), *_rows("v_out", v_out, out_dtype, dev),
           *_index("start", start, dev), *_index("lens", lens, dev), offset, _CODE[out_dtype], zk, zv)
     return k_out, v_out
 
@@ -134,10 +131,13 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
     workspace: attention_workspace(...) of the same sizes.  By default one is kept for each device, stream and
     size; a call that is being captured allocates its own from the graph's pool (graphs may then be replayed
     side by side), so a decode loop that captures many layers passes one."""
-    fq, fc, dev = _rows("q", q, torch.bfloat16), _cache(cache), q.get_device()
+    dev, fc = _device_of("q", q), _cache(cache)
+    fq = _rows("q", q, torch.bfloat16, dev)
     if out is None:
         out = _like(q) if out_dtype is None else torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    _same_device(dev, cache=cache, out=out, workspace=workspace)
+    elif not isinstance(out, torch.Tensor):
+        raise RuntimeError("out must be a CUDA tensor")
+    _same_device(dev, cache=cache, workspace=workspace)
     dt = out.dtype
     if dt not in _CODE or (out_dtype is not None and out_dtype != dt):
         raise RuntimeError(f"the output must be bf16 or fp32 and out of type out_dtype, got {dt}, out_dtype {out_dtype}")
@@ -145,7 +145,7 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
         workspace = _workspace(dev, *fq[1:3], fc[2], fq[3], fc[3])
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise RuntimeError("workspace must be a contiguous uint8 tensor")
-    _call(dev, "oa_kv4_attention", *fq, *fc, *_rows("out", out, dt), *_index("n", n, dev), workspace.data_ptr(),
+    _call(dev, "oa_kv4_attention", *fq, *fc, *_rows("out", out, dt, dev), *_index("n", n, dev), workspace.data_ptr(),
           workspace.numel(), offset, _CODE[dt], D ** -0.5 if sm_scale is None else sm_scale)
     return out
 

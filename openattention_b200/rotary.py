@@ -18,22 +18,32 @@ _current_device = torch._C._cuda_getDevice
 _current_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _bad_rows(name, t, dtype):
+def _bad_rows(name, t, dtype, dev):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != 4:
         raise RuntimeError(f"{name} must be (B, heads, T, 128), got {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{name} must be a tensor on cuda:{dev}, got {t.device}")
     raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (use torch.no_grad())")
 
 
-def _rows(name, t, dtype):
-    """The block's fields of (B, heads, T, 128) rows; sizes, strides and alignment are checked by the entry."""
+def _rows(name, t, dtype, dev):
+    """The block's fields of (B, heads, T, 128) rows on GPU `dev`; sizes, strides and alignment are checked by the
+    entry.  Every call of a decode step comes through here: one expression, and the message is made apart."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not dtype or t.dim() != 4 or \
-            (t.requires_grad and torch.is_grad_enabled()):
-        _bad_rows(name, t, dtype)
+            t.get_device() != dev or (t.requires_grad and torch.is_grad_enabled()):
+        _bad_rows(name, t, dtype, dev)
     return t.data_ptr(), *t.shape, *t.stride()
+
+
+def _device_of(name, t):
+    """The GPU of a call's leading tensor."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    return t.get_device()
 
 
 def _same_device(dev, **tensors):
@@ -56,8 +66,8 @@ def _index(name, t, dev):
 
 def _table(cos, sin, dev):
     for name, t in (("cos", cos), ("sin", sin)):
-        if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype is not torch.float32 or t.dim() != 2 or \
-                not t.is_contiguous() or t.shape != cos.shape:
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != dev or t.dim() != 2 or \
+                not t.is_contiguous() or (t is not cos and t.shape != cos.shape):
             raise RuntimeError(f"{name} must be a contiguous fp32 (positions, rotated dims) table on cuda:{dev}, the "
                                "same shape for both")
     return cos.data_ptr(), sin.data_ptr(), *cos.shape
@@ -65,9 +75,9 @@ def _table(cos, sin, dev):
 
 def _weights(q_weight, k_weight, dtype, dev):
     """(q pointer, k pointer, dtype code) of the norm weights: both in the rows' type or both fp32."""
-    given = [w for w in (q_weight, k_weight) if w is not None]
-    if not given:
+    if q_weight is None and k_weight is None:
         return 0, 0, _lib.OA_F32
+    given = [w for w in (q_weight, k_weight) if w is not None]
     for w in given:
         if not isinstance(w, torch.Tensor) or w.get_device() != dev or w.shape != (D,) or not w.is_contiguous() or \
                 w.dtype not in (dtype, torch.float32) or w.dtype != given[0].dtype:
@@ -79,13 +89,22 @@ def _like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+_entries: dict = {}
+
+
 def _call(dev, name, *fields):
-    """_lib.call_block on the current stream of GPU `dev` (a launch needs its stream's device to be current)."""
+    """An entry with its argument block, on the current stream of GPU `dev` (a launch needs its stream's device to be
+    current)."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = _lib.block_entry(name)
     if dev == _current_device():
-        _lib.call_block(name, _current_stream(dev), *fields)
+        status = entry[1](entry[0](*fields), _current_stream(dev))
     else:
         with torch.cuda.device(dev):
-            _lib.call_block(name, _current_stream(dev), *fields)
+            status = entry[1](entry[0](*fields), _current_stream(dev))
+    if status:
+        _lib.fail(name, status)
 
 
 def qk_norm_rope(q, k, cos, sin, start, *, offset=0, lens=None, q_weight=None, k_weight=None, eps=1e-5, q_out=None,
@@ -102,14 +121,16 @@ def qk_norm_rope(q, k, cos, sin, start, *, offset=0, lens=None, q_weight=None, k
     lens[b] (default T) rows of request b are real.  Rows behind them, and rows whose position is outside
     the table, are padding: they are zero in outputs that this call allocates and left as they were in
     q_out / k_out.  q_out may be q and k_out may be k (in place); otherwise outputs must not overlap inputs."""
-    dt = torch.float32 if getattr(q, "dtype", None) is torch.float32 else torch.bfloat16
-    fq, fk = _rows("q", q, dt), _rows("k", k, dt)
-    dev, given = q.get_device(), (q_out is not None, k_out is not None)
-    q_out = q_out if given[0] else _like(q)
-    k_out = k_out if given[1] else _like(k)
-    _same_device(dev, k=k, q_out=q_out, k_out=k_out)
+    dev = _device_of("q", q)
+    dt = torch.float32 if q.dtype is torch.float32 else torch.bfloat16
+    fq, fk = _rows("q", q, dt, dev), _rows("k", k, dt, dev)
+    zq, zk = q_out is None, k_out is None
+    if zq:
+        q_out = _like(q)
+    if zk:
+        k_out = _like(k)
     qp, kp, wd = _weights(q_weight, k_weight, dt, dev)
-    _call(dev, "oa_qk_norm_rope", *fq, *fk, *_rows("q_out", q_out, dt), *_rows("k_out", k_out, dt), *_table(cos, sin, dev),
-          *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, _CODE[dt], wd, not given[0],
-          not given[1], eps)
+    _call(dev, "oa_qk_norm_rope", *fq, *fk, *_rows("q_out", q_out, dt, dev), *_rows("k_out", k_out, dt, dev),
+          *_table(cos, sin, dev), *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, _CODE[dt], wd,
+          zq, zk, eps)
     return q_out, k_out
