@@ -9,6 +9,10 @@ layers with `OursB200.decode` as the attention and picks the next token greedily
 step (all layers) is captured once as a CUDA graph: the write position and the current length are
 device counters (C.kv_idx, C.n_dev), so the graph replays step after step.
 
+Queries and keys are rotated by `rotary.qk_norm_rope`, which writes a prompt's keys straight into the cache.
+With `LlamaConfig(kv4=True)` the cache is a 4-bit one (kv4.py) and decode attends to all of it densely: 3.6 times
+less cache memory and no index to build, at a step time that grows with the context.
+
 Weights are random (there are no checkpoints in this environment); the numbers it produces are
 timings and the sparse path's behaviour, not language-model quality.
 """
@@ -21,6 +25,7 @@ import torch
 import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
+from . import kv4, rotary
 from . import method as Mth
 from .geometry import D, HKV, HQ, llama31_inv_freq
 
@@ -40,11 +45,12 @@ class LlamaConfig:
     vocab: int = 128256
     eps: float = 1e-5
     qlen: int = 40              # question rows the index build uses (C.qlen)
+    kv4: bool = False           # 4-bit K/V cache and dense decode attention instead of OpenAttention over bf16
 
 
 class RandomLlama:
     """Random bf16 weights (std 1/sqrt(fan-in)), caches and the OpenAttention method for B requests
-    of up to Lmax positions."""
+    of up to Lmax positions (cfg.kv4: 4-bit caches `cache4` and no method)."""
 
     def __init__(self, cfg: LlamaConfig, B: int, Lmax: int, dev, rho: float = 0.01, seed: int = 0,
                  static_metric=None):
@@ -72,6 +78,14 @@ class RandomLlama:
         pos = torch.arange(Lmax, device=self.dev, dtype=torch.float32)
         emb = torch.cat([pos[:, None] * inv[None], pos[:, None] * inv[None]], -1)
         self.cos, self.sin = emb.cos(), emb.sin()
+        self.zero = torch.zeros(1, dtype=torch.int64, device=self.dev)  # where a prompt starts
+        self.graph = None
+        if cfg.kv4:
+            self.method = None
+            self.cache4 = [kv4.new_cache(B, Lmax, self.dev) for _ in range(cfg.layers)]
+            # one for all layers: their calls run in order
+            self.attn_ws = kv4.attention_workspace(B, HQ, 1, Lmax, self.dev)
+            return
         self.K = [torch.zeros(B, HKV, Lmax, D, dtype=torch.bfloat16, device=self.dev) for _ in range(cfg.layers)]
         self.V = [torch.zeros(B, HKV, Lmax, D, dtype=torch.bfloat16, device=self.dev) for _ in range(cfg.layers)]
         Mth.C.K, Mth.C.V, Mth.C.qlen = self.K, self.V, [cfg.qlen] * B
@@ -82,20 +96,11 @@ class RandomLlama:
             static_metric = static_metric_standin(7, cfg.layers)
         self.method = Mth.OursB200(types.SimpleNamespace(rho=rho, static_metric=static_metric), B, Lmax, self.dev,
                                    layers=cfg.layers)
-        self.graph = None
 
     # ------------------------------------------------------------------ pieces
     def _rms(self, x, w):
         xf = x.float()
         return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + self.cfg.eps)).to(torch.bfloat16) * w
-
-    @staticmethod
-    def _rope(x, cos, sin):
-        """x (..., T, D) with cos / sin (T, D) broadcast over the leading dims."""
-        h = D // 2
-        xf = x.float()
-        rot = torch.cat([-xf[..., h:], xf[..., :h]], -1)
-        return (xf * cos + rot * sin).to(torch.bfloat16)
 
     def _mlp(self, x, l):
         gu = x @ self.wgu[l]
@@ -108,7 +113,6 @@ class RandomLlama:
         """tokens (B, T) int64.  Fills every layer's K/V cache for positions [0, T), builds the index of
         every layer and request, and returns the greedy next token (B,)."""
         B, T = tokens.shape
-        cos, sin = self.cos[:T], self.sin[:T]
         nxt = torch.empty(B, dtype=torch.long, device=self.dev)
         for b in range(B):
             x = self.embed[tokens[b]]                                      # (T, H)
@@ -116,26 +120,30 @@ class RandomLlama:
             for l in range(self.cfg.layers):
                 h = self._rms(x, self.ln1[l])
                 qkv = h @ self.wqkv[l]
-                q = qkv[:, :HQ * D].view(T, HQ, D).transpose(0, 1)          # (32, T, D)
-                k = qkv[:, HQ * D:(HQ + HKV) * D].view(T, HKV, D).transpose(0, 1)
-                v = qkv[:, (HQ + HKV) * D:].view(T, HKV, D).transpose(0, 1)
-                q = self._rope(q, cos, sin)
-                k = self._rope(k, cos, sin)
-                self.K[l][b, :, :T] = k
-                self.V[l][b, :, :T] = v
+                q = qkv[:, :HQ * D].view(1, T, HQ, D).transpose(1, 2)       # (1, 32, T, D)
+                k = qkv[:, HQ * D:(HQ + HKV) * D].view(1, T, HKV, D).transpose(1, 2)
+                v = qkv[:, (HQ + HKV) * D:].view(1, T, HKV, D).transpose(1, 2)
+                k_out = None if self.cfg.kv4 else self.K[l][b:b + 1, :, :T]
+                q, k = rotary.qk_norm_rope(q, k, self.cos, self.sin, self.zero, k_out=k_out)
+                if self.cfg.kv4:
+                    kv4.append(self.cache4[l][b:b + 1], k, v, self.zero)
+                else:
+                    self.V[l][b, :, :T] = v[0]
                 g = HQ // HKV  # grouped-query: each KV head serves 4 query heads
                 with sdpa_kernel(_DENSE_BACKENDS):  # never the T x T math path
-                    o = F.scaled_dot_product_attention(q.unsqueeze(0), k.repeat_interleave(g, 0).unsqueeze(0),
-                                                       v.repeat_interleave(g, 0).unsqueeze(0), is_causal=True)[0]
+                    o = F.scaled_dot_product_attention(q, k.repeat_interleave(g, 1), v.repeat_interleave(g, 1),
+                                                       is_causal=True)[0]
                 x = x + o.transpose(0, 1).reshape(T, HQ * D) @ self.wo[l]
                 for t0 in range(0, T, chunk):                            # MLP in row chunks (activation memory)
                     t1 = min(T, t0 + chunk)
                     x[t0:t1] = x[t0:t1] + self._mlp(self._rms(x[t0:t1], self.ln2[l]), l)
-                finish = self.method.build_async(l, b, q.unsqueeze(0), T)
-                if pending is not None:
-                    pending()
-                pending = finish
-            pending()
+                if self.method is not None:
+                    finish = self.method.build_async(l, b, q, T)
+                    if pending is not None:
+                        pending()
+                    pending = finish
+            if pending is not None:
+                pending()
             logits = self._rms(x[-1:], self.norm) @ self.lm_head
             nxt[b] = logits.float().argmax(-1)[0]
         return nxt
@@ -146,18 +154,21 @@ class RandomLlama:
         C, B = Mth.C, self.B
         C.n_dev.add_(1)
         C.kv_idx.add_(1)
-        cos = self.cos.index_select(0, C.kv_idx)                          # (1, D)
-        sin = self.sin.index_select(0, C.kv_idx)
         x = self.embed.index_select(0, tok)                               # (B, H)
         for l in range(self.cfg.layers):
             h = self._rms(x, self.ln1[l])
             qkv = h @ self.wqkv[l]
-            q = self._rope(qkv[:, :HQ * D].view(B, HQ, D), cos, sin)
-            k = self._rope(qkv[:, HQ * D:(HQ + HKV) * D].view(B, HKV, D), cos, sin)
-            v = qkv[:, (HQ + HKV) * D:].view(B, HKV, D)
+            q = qkv[:, :HQ * D].view(B, HQ, 1, D)
+            k = qkv[:, HQ * D:(HQ + HKV) * D].view(B, HKV, 1, D)
+            v = qkv[:, (HQ + HKV) * D:].view(B, HKV, 1, D)
             # this layer's new K/V rows are written at position n - 1 (the counters advanced at the step's
-            # start) by the index update's launch
-            o = self.method.decode(l, q.view(B, HQ, 1, D), n_host, k_new=k.contiguous(), v_new=v.contiguous())
+            # start) by the rotation's launch, or by the index update's
+            if self.cfg.kv4:
+                q = kv4.rope_append(self.cache4[l], q, k, v, self.cos, self.sin, C.kv_idx)
+                o = kv4.decode_attention(q, self.cache4[l], C.n_dev, workspace=self.attn_ws)
+            else:
+                q, k = rotary.qk_norm_rope(q, k, self.cos, self.sin, C.kv_idx)
+                o = self.method.decode(l, q, n_host, k_new=k.view(B, HKV, D), v_new=v.view(B, HKV, D).contiguous())
             x = x + o.reshape(B, HQ * D) @ self.wo[l]
             x = x + self._mlp(self._rms(x, self.ln2[l]), l)
         logits = self._rms(x, self.norm) @ self.lm_head
@@ -185,7 +196,8 @@ class RandomLlama:
         warm-up, so the next replay is the next step."""
         C = Mth.C
         n_snap, kv_snap, tok_snap = C.n_dev.clone(), C.kv_idx.clone(), self.tok.clone()
-        st_snap = [{k: st[k].clone() for k in _STEP_STATE if k in st} for st in self.method.st]
+        st = self.method.st if self.method is not None else []
+        st_snap = [{k: x[k].clone() for k in _STEP_STATE if k in x} for x in st]
         s = torch.cuda.Stream(self.dev)
         s.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(s):
@@ -195,9 +207,9 @@ class RandomLlama:
         C.n_dev.copy_(n_snap)
         C.kv_idx.copy_(kv_snap)
         self.tok.copy_(tok_snap)
-        for st, snap in zip(self.method.st, st_snap):
+        for x, snap in zip(st, st_snap):
             for k, v in snap.items():
-                st[k].copy_(v)
+                x[k].copy_(v)
         del st_snap
         self._tok_in = self.tok
         self.graph = torch.cuda.CUDAGraph()
