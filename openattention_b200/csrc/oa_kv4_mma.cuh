@@ -7,6 +7,11 @@
 // The value side folds the scale into the weight: o = sum_t (p_t s_t) c_t + sum_t p_t z_t, the second sum in
 // fp32 outside the tensor cores.
 //
+// Tensor cores truncate their running sums.  Codes are all positive, so sums of p s c would grow with the context
+// and with them the truncation, while the offsets' part cancels most of them (1.1e-2 of the result was seen at
+// 131072 tokens in one CTA).  So half of the tokens enter complemented, s c + z = -s (15 - c) + (z + 15 s), at no
+// cost (the complement is part of the AND): the sums stay of the result's size.
+//
 // Codes cost one AND each pair: a nibble left in place in a 16-bit word is an fp16 subnormal, code * 2^-24 (low
 // nibble) or 16 * code * 2^-24 (high nibble), exact.  Low and high nibbles are the two halves, so the factor 16
 // belongs to a whole half.  q is scaled by a power of two per column (largest element in [2^13, 2^14)), exact
@@ -314,7 +319,9 @@ struct WarpAttention {
         if (J > 1) l[1] += p1;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          const float sv = bf_lo(vm[b][k][h]) * r[h], zv = bf_hi(vm[b][k][h]);
+          // second tokens enter as -s (15 - c) + (z + 15 s): the codes' sums then stay near zero (below)
+          const float s1 = bf_lo(vm[b][k][h]), sv = s1 * (k ? -r[h] : r[h]);
+          const float zv = k ? fmaf(15.f, s1, bf_hi(vm[b][k][h])) : bf_hi(vm[b][k][h]);
           float w0 = p0 * sv, w1 = J > 1 ? p1 * sv : 0.f;
           if (MASK) {
             const bool in0 = in[0] >> (16 * b + k) & 1u, in1 = J > 1 && (in[1] >> (16 * b + k) & 1u);
@@ -337,8 +344,8 @@ struct WarpAttention {
         const uint32_t u = __byte_perm(i < 2 ? a0.x : a0.y, i < 2 ? a1.x : a1.y, sel);
         const uint32_t w = __byte_perm(i < 2 ? n0.x : n0.y, i < 2 ? n1.x : n1.y, sel);
         const uint32_t u8 = u >> 8, w8 = w >> 8;
-        mma_f16(acc[i], u & kLoMask, u8 & kLoMask, w & kLoMask, w8 & kLoMask, pw[0][0], pw[1][0]);
-        mma_f16(acc[4 + i], u & kHiMask, u8 & kHiMask, w & kHiMask, w8 & kHiMask, pw[0][kHalves - 1], pw[1][kHalves - 1]);
+        mma_f16(acc[i], u & kLoMask, u8 & kLoMask, ~w & kLoMask, ~w8 & kLoMask, pw[0][0], pw[1][0]);
+        mma_f16(acc[4 + i], u & kHiMask, u8 & kHiMask, ~w & kHiMask, ~w8 & kHiMask, pw[0][kHalves - 1], pw[1][kHalves - 1]);
       }
     }
   }

@@ -449,3 +449,25 @@ def test_zero_sized_calls():
     q = torch.ones(2, 4, 1, D, dtype=BF, device="cuda")
     assert not kv4.decode_attention(q, cache[:, :, :0], z + 5).any()
     assert not kv4.decode_attention(q, cache, z).any()
+
+
+def test_dense_long_rows_keep_their_precision():
+    """300 heads read one 131072-token row each (the same records, by an expanded cache), so a CTA sums a whole row.
+    The fp16 roundings of the weights are independent, each at most 2^-11 of weight * scale * code: their sum has a
+    root mean square of at most 2^-11 / sqrt(3) of the root of the summed squares.  Twice 2^-11 is over three times
+    that; a bias that grows with the number of tokens is far above it."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(51)
+    n, H = 131072, 300
+    k = torch.randn(n, D, generator=g, device="cuda") + 1.5 * torch.randn(D, generator=g, device="cuda")
+    v = torch.randn(n, D, generator=g, device="cuda")
+    cache = kv4.new_cache(1, n, "cuda", hkv=1)
+    kv4.append(cache, k.to(BF).view(1, 1, n, D), v.to(BF).view(1, 1, n, D), torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = torch.randn(1, H, 1, D, generator=g, device="cuda").to(BF)
+    got = kv4.decode_attention(q, cache.expand(1, H, n, REC), torch.tensor([n], device="cuda"), out_dtype=torch.float32)
+    K, V = P.values(cache[0, 0], 0), P.values(cache[0, 0], 1)
+    code, s, _ = P.parts(cache[0, 0], 1)
+    for h in range(0, H, 37):
+        w = torch.softmax(K @ q[0, h, 0].double() * D ** -0.5, 0)
+        err = (got[0, h, 0].double() - w @ V).norm()
+        assert err <= 2 * 2.0 ** -11 * ((w[:, None] * s * code).square().sum().sqrt())
