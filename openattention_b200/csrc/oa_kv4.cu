@@ -328,7 +328,7 @@ __device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& 
   return true;
 }
 
-template <bool PAIR>
+template <bool QUAD>
 __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
   extern __shared__ __align__(16) unsigned char s_ring[];
   __shared__ unsigned s_last;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
 
   const uint32_t ring = smem_u32(s_ring) + warp * (kStages * kTileBytes);
   float* s_part = reinterpret_cast<float*>(s_ring);  // reused once a row's tiles are done
-  WarpAttention<PAIR> at;
+  WarpAttention<QUAD> at;
   at.lane_addresses();
 
   for (;;) {
@@ -385,11 +385,12 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
     }
     at.begin(a.qk_scale);
     const int whole = n - a.T + 1;  // tokens that every column sees
-    int sees[2];                      // tokens that the lane's columns see
+    constexpr int J = WarpAttention<QUAD>::J;
+    int sees[J];                      // tokens that the lane's columns see
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < J; ++j) {
       int hh, tt;
-      split(at.acc_col(j), hh, tt);
+      split(at.col(j), hh, tt);
       sees[j] = whole + tt;
     }
     uint32_t slot = 0;
@@ -397,10 +398,12 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
       cp_async_wait<kStages - 2>();
       __syncwarp();
       if ((k + 1) * kTile <= whole) {
-        const uint32_t all[2] = {~0u, ~0u};
+        const uint32_t all[J] = {};
         at.template tile<false>(ring + slot * kTileBytes, all);
       } else {
-        const uint32_t in[2] = {first_bits(sees[0] - k * kTile), first_bits(sees[1] - k * kTile)};
+        uint32_t in[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) in[j] = first_bits(sees[j] - k * kTile);
         at.template tile<true>(ring + slot * kTileBytes, in);
       }
       __syncwarp();
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
       __syncthreads();
       if (s_last) {
         __threadfence();
-        merge_parts<PAIR ? 6 : 4>(w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part,
+        merge_parts<QUAD ? 6 : 4>(w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part,
                                   const_cast<void*>(a.o.p), a.out_f32, o_at);
         if (tid == 0) *ticket = 0u;
       }
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
   };
   int j = rank * W + warp;
   int v0 = ask(j), v1 = ask(j + nw), v2 = ask(j + 2 * nw);
-  WarpAttention<true, 1> at;
+  WarpAttention<true> at;
   at.lane_addresses();
   at.load_q(at.op_col() == 0 ? a.q + r * a.q_stride : nullptr);
   uint32_t in0 = fetch(j, v0, 0), in1 = fetch(j + nw, v1, 1);
@@ -565,7 +568,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
     __syncwarp();
     const uint32_t sm = ring + stage * kTileBytes;
     if (j < tiles) {
-      const uint32_t sees[2] = {in0, in0};
+      const uint32_t sees[1] = {in0};
       if (in0 == ~0u)
         at.template tile<false>(sm, sees);
       else if (in0)
@@ -585,6 +588,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
   }
   cp_async_wait<0>();
   __syncwarp();
+  if (rows) at.end_rows();
   {
     float* state = reinterpret_cast<float*>(s_dyn + warp * (kStages * kTileBytes));
     at.finish(state, state + kD, 1);

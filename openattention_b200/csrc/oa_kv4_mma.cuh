@@ -1,29 +1,30 @@
-// One warp's attention over tiles of 32 cache records (oa_kv4.cuh), on mma.sync.m16n8k16 (fp16 in, fp32
-// accumulated).  The warp attends for up to eight query columns (query heads, query tokens) that read the
-// same records.
+// One warp's attention over tiles of 32 cache records (oa_kv4.cuh) on the warp-level tensor cores (mma.sync).  The warp
+// attends for up to four or eight query columns (query heads, query tokens) that read the same records.  A decode
+// step reads each record once for few columns, so memory bounds it; what the tensor cores are for here is that the
+// codes need not be turned into numbers by the other pipes.  (tcgen05 takes its operands from shared or tensor memory
+// in whole bytes at least: the unpacked codes would have to be written back there first.)
 //
-// Mathematics.  With K = s c + z per half h of the head, q . K = sum_h s_h (q_h . c_h) + z_h (sum q_h): the
-// tensor cores multiply the bare codes, the scales and offsets enter after, in fp32, once per token and half.
-// The value side folds the scale into the weight: o = sum_t (p_t s_t) c_t + sum_t p_t z_t, the second sum in
-// fp32 outside the tensor cores.
+// Scores.  With K = s c + z per half h of the head, q . K = sum_h s_h (q_h . c_h) + z_h (sum q_h): the tensor cores
+// multiply the bare codes, the scales and offsets enter after, in fp32, once per token and half.  Codes cost one AND
+// each pair: a nibble left in place in a 16-bit word is an fp16 subnormal, code * 2^-24 (low nibble) or 16 code * 2^-24
+// (high nibble), exact.  Low and high nibbles are the two halves, so the factor 16 belongs to a whole half.  q is
+// scaled by a power of two per column (largest element in [2^13, 2^14)), exact unless an element is 2^-37 of the
+// largest.  (e4m3 operands would hold a code in a byte, but mma.sync takes them apart into fp16 here: slower.)
+//
+// Values.  The scale goes into the weight: o = sum_t (p_t s_t) c_t + sum_t p_t z_t, the second sum in fp32 outside the
+// tensor cores.  p s is scaled by a power of two per half, chosen so that the largest scale seen gives [2^6, 2^7): it
+// is rounded to fp16 (11 bits) over 20 octaves below the largest, beneath them it is off by 2^-32 of the largest.
 //
 // Tensor cores truncate their running sums.  Codes are all positive, so sums of p s c would grow with the context
 // and with them the truncation, while the offsets' part cancels most of them (1.1e-2 of the result was seen at
 // 131072 tokens in one CTA).  So half of the tokens enter complemented, s c + z = -s (15 - c) + (z + 15 s), at no
 // cost (the complement is part of the AND): the sums stay of the result's size.
 //
-// Codes cost one AND each pair: a nibble left in place in a 16-bit word is an fp16 subnormal, code * 2^-24 (low
-// nibble) or 16 * code * 2^-24 (high nibble), exact.  Low and high nibbles are the two halves, so the factor 16
-// belongs to a whole half.  q is scaled by a power of two per column (largest element in [2^13, 2^14)), exact
-// unless an element is 2^-37 of the largest; p s by a power of two per half, chosen so that the largest scale
-// seen gives [2^6, 2^7): p s is rounded to fp16 (11 bits) over 20 octaves below the largest, beneath them it is
-// off by 2^-32 of the largest.
-//
-// Layout.  Scores are computed transposed, S^T = codes (16 tokens) x q (8 columns), so that columns lie along
-// the accumulator's lanes the same way as in O^T = V^T (16 dims) x P (8 columns): running maxima and sums need
-// no exchange, only P turns (movmatrix).  The contraction's order is free, so a lane's operand words are its
-// 16 contiguous bytes of a K row and 8 bytes of a V row.  Rows of an MMA are assigned to tokens so that both
-// loads touch every bank once although records lie 36 words apart.
+// Layout.  Scores are computed transposed, S^T = codes (16 tokens) x q (columns), so that columns lie along the
+// accumulator's lanes the same way as in O^T = V^T (16 dims) x P (columns): running maxima and sums need no exchange,
+// only P turns (movmatrix).  The contraction's order is free, so a lane's operand words are its 16 contiguous bytes
+// of a K row and 8 bytes of a V row.  Rows of an MMA are assigned to tokens so that both loads touch every bank once
+// although records lie 36 words apart.  A tile costs about 370 instructions, of which 176 unpack codes.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -95,33 +96,32 @@ __device__ __forceinline__ uint32_t lds32(uint32_t at, int imm) {
 // Token (0..15 of a 16-token block) of MMA row r (0..7); row r + 8 holds the next token.
 __device__ __forceinline__ int row_token(int r) { return (r & 1) ? 8 + ((r + 3) & 7) : r; }
 
-// PAIR: at most four columns, and the MMA's eight columns hold each twice: columns 0..3 are the four query rows
-// against half 0 of the head, columns 4..7 against half 1.  A lane then serves one half: half the scales to read,
-// weights to form and turn; the halves' scores meet through one shuffle.  Otherwise eight columns, each lane
-// both halves.  J: accumulator columns of a lane that are in use (1 where there is one query row).
-template <bool PAIR, int J = 2>
+// QUAD: at most four columns.  The MMA's eight columns are each query's two halves, side by side in a lane, which
+// therefore serves one query: column 2c takes half 0 only (its q operand is zero in the other half's steps), 2c + 1
+// half 1, in scores and in weights.  Else eight columns, two queries to a lane, and the halves take sums and weights
+// of their own.
+template <bool QUAD>
 struct WarpAttention {
-  static constexpr int kHalves = PAIR ? 1 : 2;  // halves a lane serves
-  uint32_t qf[16];            // q operand: half h, word i -> qf[8 h + 2 i], +1
-  float scale[2];             // per column: sm_scale log2(e) 2^(24 - exponent of q)
-  float qs[2][kHalves];       // sm_scale log2(e) times the sum of q over the half
-  float acc[8][4];            // O^T: half h, tile i -> acc[4 h + i]; PAIR: valid where h is the lane's half
-  float m[2], bm[2], l[2];    // running maximum (log2 units; bm: 0 while it is -inf), this lane's share of the sum
-  float zs[2][kHalves];       // this lane's share of sum p z
-  float r[kHalves], cap[kHalves];  // power-of-two factor of p s, and the largest scale it holds
+  static constexpr int J = QUAD ? 1 : 2;  // columns (queries) of a lane
+  uint32_t qf[16];          // q operand: half h, word i of the lane's K chunk -> qf[8 h + 2 i], + 1
+  float scale[J];           // per column: sm_scale log2(e) 2^(24 - exponent of q)
+  float qs[J][2];           // sm_scale log2(e) times the sum of q over each half
+  float acc[8][4];          // O^T: half h, tile i -> acc[4 h + i], QUAD: MMA column h of the lane's two counts
+  float m[J], bm[J], l[J];  // running maximum (log2 units; bm: 0 while it is -inf), this lane's share of the sum
+  float zs[J][2];           // this lane's share of sum p z, per half
+  float r[2], cap[2];       // power-of-two factor of p s per half, and the largest scale it holds
   uint32_t at_k, at_m, at_v0, at_v1;  // this lane's addresses in a tile
 
   static __device__ __forceinline__ int lane() { return threadIdx.x & 31; }
-  // the query columns of this lane's accumulator columns 0, 1, and of its operand column
-  static __device__ __forceinline__ int acc_col(int j) { return 2 * (lane() & (PAIR ? 1 : 3)) + j; }
-  static __device__ __forceinline__ int op_col() { return (lane() >> 2) & (PAIR ? 3 : 7); }
-  static __device__ __forceinline__ int half() { return PAIR ? (lane() >> 1) & 1 : 0; }
+  // the query columns of this lane's scores, and of its operand column
+  static __device__ __forceinline__ int col(int j) { return QUAD ? lane() & 3 : 2 * (lane() & 3) + j; }
+  static __device__ __forceinline__ int op_col() { return QUAD ? lane() >> 3 : lane() >> 2; }
 
   __device__ __forceinline__ void lane_addresses() {
     const uint32_t g = lane() >> 2, t = lane() & 3;
     const uint32_t tok = row_token(g);
     at_k = tok * kRec + 16 * t;                              // K codes of MMA row g; row g + 8 is the next record
-    at_m = tok * kRec + kRecMeta + 4 * half();
+    at_m = tok * kRec + kRecMeta;
     at_v0 = 2 * t * kRec + kRecV + 8 * g;                    // V dims 8g .. 8g + 7 (and + 64) of MMA row 2t
     at_v1 = (8 + ((2 * t + 4) & 7)) * kRec + kRecV + 8 * g;  // and of row 2t + 1
   }
@@ -138,63 +138,55 @@ struct WarpAttention {
   }
   __device__ __forceinline__ void begin(float qk_scale) {
     const int t = lane() & 3;
-    float lo[16], hi[16], amax = 0.f, s0 = 0.f, s1 = 0.f;
+    float q[2][16], amax = 0.f, s[2] = {0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const uint4 v = q_raw[w];
-      float* f = (w >= 2 ? hi : lo) + 8 * (w & 1);
+      float* f = q[w >> 1] + 8 * (w & 1);
       f[0] = bf_lo(v.x); f[1] = bf_hi(v.x); f[2] = bf_lo(v.y); f[3] = bf_hi(v.y);
       f[4] = bf_lo(v.z); f[5] = bf_hi(v.z); f[6] = bf_lo(v.w); f[7] = bf_hi(v.w);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-      s0 += lo[i];
-      s1 += hi[i];
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        amax = fmaxf(amax, fabsf(q[h][i]));
+        s[h] += q[h][i];
+      }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+      s[1] += __shfl_xor_sync(0xffffffffu, s[1], o);
     }
     // clamped so that 2^(24 - e) stays finite: |q| up to 2^105 is held
     const int e = amax > 0.f ? min(120, max(-90, 13 - ((__float_as_int(amax) >> 23) - 127))) : 0;
-    float f0 = pow2i(e), f1 = pow2i(e - 4);
-    if (PAIR) (lane() < 16 ? f1 : f0) = 0.f;  // columns 0..3 take half 0 only, 4..7 half 1
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      qf[2 * i] = pack_half2(lo[4 * i] * f0, lo[4 * i + 2] * f0);
-      qf[2 * i + 1] = pack_half2(lo[4 * i + 1] * f0, lo[4 * i + 3] * f0);
-      qf[8 + 2 * i] = pack_half2(hi[4 * i] * f1, hi[4 * i + 2] * f1);
-      qf[8 + 2 * i + 1] = pack_half2(hi[4 * i + 1] * f1, hi[4 * i + 3] * f1);
+    for (int h = 0; h < 2; ++h) {
+      // MMA column lane / 4; QUAD: of query column lane / 8, even ones half 0, odd ones half 1
+      const float f = QUAD && ((lane() >> 2) & 1) != h ? 0.f : pow2i(h ? e - 4 : e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qf[8 * h + 2 * i] = pack_half2(q[h][4 * i] * f, q[h][4 * i + 2] * f);
+        qf[8 * h + 2 * i + 1] = pack_half2(q[h][4 * i + 1] * f, q[h][4 * i + 3] * f);
+      }
     }
     const float sc = qk_scale * pow2i(24 - e);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {  // accumulator column 2t + j is the operand column of the lanes 4 (2t + j) ..
-      const int src = 8 * t + 4 * j;
+    for (int j = 0; j < J; ++j) {  // from a lane whose operand column is the lane's column j
+      const int src = QUAD ? 8 * t : 8 * t + 4 * j;
       scale[j] = __shfl_sync(0xffffffffu, sc, src);
-      const float a = __shfl_sync(0xffffffffu, s0, src) * qk_scale, b = __shfl_sync(0xffffffffu, s1, src) * qk_scale;
-      if (PAIR) {
-        qs[j][0] = half() ? b : a;
-      } else {
-        qs[j][0] = a;
-        qs[j][kHalves - 1] = b;
-      }
+      qs[j][0] = __shfl_sync(0xffffffffu, s[0], src) * qk_scale;
+      qs[j][1] = __shfl_sync(0xffffffffu, s[1], src) * qk_scale;
+      m[j] = -INFINITY;
+      bm[j] = l[j] = zs[j][0] = zs[j][1] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      m[j] = -INFINITY;
-      bm[j] = l[j] = 0.f;
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) zs[j][h] = 0.f;
-    }
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
+    for (int h = 0; h < 2; ++h) {
       r[h] = pow2i(126);
       cap[h] = pow2i(kTop - 126);
     }
@@ -209,47 +201,52 @@ struct WarpAttention {
     const float next = pow2i(kTop - 1 - es);
     // next / r as a power of two; one under 2^-126 drops what is there, which is that much smaller
     const int d = (__float_as_int(next) >> 23) - (__float_as_int(r[h]) >> 23);
-    const float f = d < -126 ? 0.f : pow2i(d);
-#pragma unroll
-    for (int i = 0; i < (PAIR ? 8 : 4); ++i)  // PAIR: the other half's tiles are not read in this lane
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[4 * h + i][j] *= f;
+    scale_half(h, d < -126 ? 0.f : pow2i(d));
     r[h] = next;
     cap[h] = pow2i(kTop) / next;
   }
-
-  // One tile of 32 records at shared address `sm`.  MASK: the lane's accumulator column j sees only the tokens whose
-  // bit is set in sees[j]; what the others' records hold (stale bytes, NaN scales) does not enter.
-  template <bool MASK>
-  __device__ __forceinline__ void tile(uint32_t sm, const uint32_t (&sees)[2]) {
-    uint32_t in[2];  // bit 16 b + k: this lane's token k of block b
+  __device__ __forceinline__ void scale_half(int h, float f) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) in[j] = MASK ? sees[j] >> row_token(lane() >> 2) : 0u;
-    float x[2][4];
-    uint32_t vm[2][2][kHalves];  // value scale and offset of this lane's four tokens
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!QUAD || (j & 1) == h) acc[4 * h + i][j] *= f;
+  }
+  // A score above the running maximum of column j: new maximum, and everything of the column scaled to it.  mx: the
+  // lane's largest.
+  __device__ __forceinline__ void raise_max(float mx, int j) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float nm = fmaxf(m[j], mx);
+    const float al = ex2(m[j] - biased(nm));
+    m[j] = nm;
+    bm[j] = biased(nm);
+    l[j] *= al;
+    zs[j][0] *= al;
+    zs[j][1] *= al;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (QUAD || (k & 1) == j) acc[i][k] *= al;
+  }
+
+  // One tile of 32 records at shared address `sm`.  MASK: the lane's column j sees only the tokens whose bit is set in
+  // sees[j]; what the others' records hold (stale bytes, NaN scales) does not enter.
+  template <bool MASK>
+  __device__ __forceinline__ void tile(uint32_t sm, const uint32_t (&sees)[J]) {
+    uint32_t in[J];  // bit 16 b + k: this lane's token k of block b
+#pragma unroll
+    for (int j = 0; j < J; ++j) in[j] = MASK ? sees[j] >> row_token(lane() >> 2) : 0u;
+    float x[2][2][J];      // scores: block, token, column
+    uint32_t vm[2][2][2];  // value scale and offset of this lane's four tokens, per half
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const uint4 ka = lds128(sm + at_k, 16 * b * kRec), kb = lds128(sm + at_k, (16 * b + 1) * kRec);
-      uint32_t km[2][kHalves];
-      if (PAIR) {
+      const uint4 ma = lds128(sm + at_m, 16 * b * kRec), mb = lds128(sm + at_m, (16 * b + 1) * kRec);
+      float c[2][4];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          km[k][0] = lds32(sm + at_m, (16 * b + k) * kRec);
-          vm[b][k][0] = lds32(sm + at_m, (16 * b + k) * kRec + 8);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint4 w = lds128(sm + at_m, (16 * b + k) * kRec);
-          km[k][0] = w.x;
-          km[k][kHalves - 1] = w.y;
-          vm[b][k][0] = w.z;
-          vm[b][k][kHalves - 1] = w.w;
-        }
-      }
-      float c[kHalves][4];
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[h][i] = 0.f;
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
@@ -257,30 +254,30 @@ struct WarpAttention {
       for (int i = 0; i < 4; ++i) {
         const uint32_t a = wa[i], d = wb[i], a8 = a >> 8, d8 = d >> 8;
         mma_f16(c[0], a & kLoMask, d & kLoMask, a8 & kLoMask, d8 & kLoMask, qf[2 * i], qf[2 * i + 1]);
-        mma_f16(c[kHalves - 1], a & kHiMask, d & kHiMask, a8 & kHiMask, d8 & kHiMask, qf[8 + 2 * i], qf[8 + 2 * i + 1]);
+        mma_f16(c[QUAD ? 0 : 1], a & kHiMask, d & kHiMask, a8 & kHiMask, d8 & kHiMask, qf[8 + 2 * i], qf[8 + 2 * i + 1]);
       }
+      const uint32_t km[2][2] = {{ma.x, ma.y}, {mb.x, mb.y}};
+      vm[b][0][0] = ma.z; vm[b][0][1] = ma.w;
+      vm[b][1][0] = mb.z; vm[b][1][1] = mb.w;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          float y = bf_lo(km[k][0]) * c[0][2 * k + j], z = bf_hi(km[k][0]) * qs[j][0];
-          if (!PAIR) {
-            y = fmaf(bf_lo(km[k][kHalves - 1]), c[kHalves - 1][2 * k + j], y);
-            z = fmaf(bf_hi(km[k][kHalves - 1]), qs[j][kHalves - 1], z);
-          }
+          const float d0 = c[0][2 * k + j], d1 = QUAD ? c[0][2 * k + 1] : c[1][2 * k + j];
+          const float y = fmaf(bf_lo(km[k][1]), d1, bf_lo(km[k][0]) * d0);
+          const float z = fmaf(bf_hi(km[k][1]), qs[j][1], bf_hi(km[k][0]) * qs[j][0]);
           float v = fmaf(y, scale[j], z);
-          if (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);
           if (MASK && !(in[j] >> (16 * b + k) & 1u)) v = -INFINITY;
-          x[b][2 * k + j] = v;
+          x[b][k][j] = v;
         }
     }
     // m is the same in all lanes of a column and nothing moves until some lane sees a score kSlack above it (or
     // a scale above the cap): weights up to 2^kSlack are as good as weights up to 1, and new maxima are common
-    float mx[2], s[kHalves];
+    float mx[J], s[2];
 #pragma unroll
-    for (int j = 0; j < J; ++j) mx[j] = fmaxf(fmaxf(x[0][j], x[0][2 + j]), fmaxf(x[1][j], x[1][2 + j]));
+    for (int j = 0; j < J; ++j) mx[j] = fmaxf(fmaxf(x[0][0][j], x[0][1][j]), fmaxf(x[1][0][j], x[1][1][j]));
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
+    for (int h = 0; h < 2; ++h) {
       s[h] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -288,52 +285,44 @@ struct WarpAttention {
         s[h] = fmaxf(s[h], used ? bf_lo(vm[i >> 1][i & 1][h]) : 0.f);
       }
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[J - 1] > m[J - 1] + kSlack || s[0] > cap[0] || s[kHalves - 1] > cap[kHalves - 1])) {
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[J - 1] > m[J - 1] + kSlack || s[0] > cap[0] || s[1] > cap[1])) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
-        const float nm = fmaxf(m[j], mx[j]);
-        const float al = ex2(m[j] - biased(nm));
-        m[j] = nm;
-        bm[j] = biased(nm);
-        l[j] *= al;
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) zs[j][h] *= al;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          acc[i][j] *= al;
-          acc[i][2 + j] *= al;
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) raise_cap(s[h], h);
+      for (int j = 0; j < J; ++j) raise_max(mx[j], j);
+      raise_cap(s[0], 0);
+      raise_cap(s[1], 1);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      uint32_t pw[2][kHalves];  // weights, turned: tokens of MMA rows 0..7, of rows 8..15
+      uint32_t pw[2][2];  // weights, turned: tokens of MMA rows 0..7, of rows 8..15; per half (QUAD: both in one)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float p0 = ex2(x[b][2 * k] - bm[0]), p1 = J > 1 ? ex2(x[b][2 * k + 1] - bm[1]) : 0.f;
-        l[0] += p0;
-        if (J > 1) l[1] += p1;
+        float w[2][J];
+        float p[J];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          // second tokens enter as -s (15 - c) + (z + 15 s): the codes' sums then stay near zero (below)
+        for (int j = 0; j < J; ++j) {
+          p[j] = ex2(x[b][k][j] - bm[j]);
+          l[j] += p[j];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // second tokens enter as -s (15 - c) + (z + 15 s)
           const float s1 = bf_lo(vm[b][k][h]), sv = s1 * (k ? -r[h] : r[h]);
           const float zv = k ? fmaf(15.f, s1, bf_hi(vm[b][k][h])) : bf_hi(vm[b][k][h]);
-          float w0 = p0 * sv, w1 = J > 1 ? p1 * sv : 0.f;
-          if (MASK) {
-            const bool in0 = in[0] >> (16 * b + k) & 1u, in1 = J > 1 && (in[1] >> (16 * b + k) & 1u);
-            w0 = in0 ? w0 : 0.f;
-            w1 = in1 ? w1 : 0.f;
-            zs[0][h] += in0 ? p0 * zv : 0.f;
-            if (J > 1) zs[1][h] += in1 ? p1 * zv : 0.f;
-          } else {
-            zs[0][h] = fmaf(p0, zv, zs[0][h]);
-            if (J > 1) zs[1][h] = fmaf(p1, zv, zs[1][h]);
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const bool seen = !MASK || (in[j] >> (16 * b + k) & 1u);
+            w[h][j] = seen ? p[j] * sv : 0.f;
+            if (MASK)
+              zs[j][h] += seen ? p[j] * zv : 0.f;
+            else
+              zs[j][h] = fmaf(p[j], zv, zs[j][h]);
           }
-          pw[k][h] = transpose8x8(pack_half2(w0, w1));
+        }
+        if (QUAD) {
+          pw[k][0] = pw[k][1] = transpose8x8(pack_half2(w[0][0], w[1][0]));
+        } else {
+          pw[k][0] = transpose8x8(pack_half2(w[0][0], w[0][J - 1]));
+          pw[k][1] = transpose8x8(pack_half2(w[1][0], w[1][J - 1]));
         }
       }
       const uint2 a0 = lds64(sm + at_v0, 16 * b * kRec), a1 = lds64(sm + at_v1, 16 * b * kRec);
@@ -345,16 +334,15 @@ struct WarpAttention {
         const uint32_t w = __byte_perm(i < 2 ? n0.x : n0.y, i < 2 ? n1.x : n1.y, sel);
         const uint32_t u8 = u >> 8, w8 = w >> 8;
         mma_f16(acc[i], u & kLoMask, u8 & kLoMask, ~w & kLoMask, ~w8 & kLoMask, pw[0][0], pw[1][0]);
-        mma_f16(acc[4 + i], u & kHiMask, u8 & kHiMask, ~w & kHiMask, ~w8 & kHiMask, pw[0][kHalves - 1], pw[1][kHalves - 1]);
+        mma_f16(acc[4 + i], u & kHiMask, u8 & kHiMask, ~w & kHiMask, ~w8 & kHiMask, pw[0][1], pw[1][1]);
       }
     }
   }
 
-  // ---- bf16 rows among the records (PAIR, J = 1: one query row, in columns 0 and 4): tiles of 8 rows of K, then 8
-  // of V, 256 bytes each, 16-byte chunk c of row i at chunk c ^ i.  Scores: MMA rows g and g + 8 are the two halves
-  // of K row g, columns 0 and 1 the halves of q; the score is their diagonal's sum.  Values go into the records'
-  // accumulators: weights carry the factors that those carry, as two bf16 terms (16 bits) in columns 0, 1 (half 0)
-  // and 4, 5 (half 1).
+  // ---- bf16 rows among the records (QUAD, one query row, in column 0): tiles of 8 rows of K, then 8 of V, 256 bytes
+  // each, 16-byte chunk c of row i at chunk c ^ i.  Scores: MMA rows g and g + 8 are the two halves of K row g, columns
+  // 0 and 1 the halves of q; the score is their diagonal's sum.  Values go into the records' accumulators: weights
+  // carry the factors that those carry, as two bf16 terms (16 bits), the second in the unused columns of query 1.
   __device__ __forceinline__ void begin_rows(const __nv_bfloat16* q) {
     const int g = lane() >> 2, t = lane() & 3;
 #pragma unroll
@@ -366,15 +354,24 @@ struct WarpAttention {
         qf[2 * i + 1] = *reinterpret_cast<const uint32_t*>(q + 64 * g + 16 * i + 2 * t + 8);
       }
     }
-    // scales of records may have left a factor that would carry a large row past fp32
-    if (r[0] > pow2i(60)) {
+    const float m0 = __shfl_sync(0xffffffffu, m[0], lane() & 28);
+    if (t != 0) {
+      m[0] = m0;
+      bm[0] = biased(m0);
+      l[0] = zs[0][0] = zs[0][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= pow2i(60) / r[0];
-      cap[0] = pow2i(kTop - 60);
-      r[0] = pow2i(60);
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
     }
+    // scales of records may have left a factor that would carry a large row past fp32
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (r[h] > pow2i(60)) {
+        scale_half(h, pow2i(60) / r[h]);
+        cap[h] = pow2i(kTop - 60);
+        r[h] = pow2i(60);
+      }
   }
   // sm: the tile; in: its live rows (others are zero in memory); bias: this lane's row's (lane < 8) log2 weight
   __device__ __forceinline__ void rows(uint32_t sm, uint32_t in, float bias, float qk_scale) {
@@ -393,26 +390,17 @@ struct WarpAttention {
     }
     float v = __shfl_sync(0xffffffffu, c[0] + c[3], lane() & 28);  // lane t = 0 of the row has it
     const float b = __shfl_sync(0xffffffffu, bias, g);
-    v = (in >> g & 1u) && !(t & 1) ? fmaf(v, qk_scale, b) : -INFINITY;
-    if (__any_sync(0xffffffffu, v > m[0] + kSlack)) {
-      float mx = v;
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      mx = fmaxf(m[0], mx);
-      const float al = ex2(m[0] - biased(mx));
-      m[0] = mx;
-      bm[0] = biased(mx);
-      l[0] *= al;
-      zs[0][0] *= al;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= al;
-    }
+    v = (in >> g & 1u) ? fmaf(v, qk_scale, b) : -INFINITY;
+    if (__any_sync(0xffffffffu, v > m[0] + kSlack)) raise_max(v, 0);
     const float p = ex2(v - bm[0]);
     l[0] += p;
-    const float w = p * (r[0] * pow2i(half() ? -20 : -24)), hi = bf_round(w);
-    const uint32_t pw = transpose8x8((uint32_t)f2bf_bits(hi) | ((uint32_t)f2bf_bits(w - hi) << 16));
+    float w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float full = p * (r[h] * pow2i(h ? -20 : -24)), hi = bf_round(full);
+      w[h] = t == 0 ? hi : t == 1 ? full - hi : 0.f;
+    }
+    const uint32_t pw = transpose8x8((uint32_t)f2bf_bits(w[0]) | ((uint32_t)f2bf_bits(w[1]) << 16));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t r0 = 2 * t, r1 = 2 * t + 1, ch = 8 * h + g;
@@ -423,6 +411,18 @@ struct WarpAttention {
       mma_bf16_k8(acc[4 * h + 3], __byte_perm(a.w, d.w, 0x5410), __byte_perm(a.w, d.w, 0x7632), pw);
     }
   }
+  // after the last rows(): the second terms join column 0
+  __device__ __forceinline__ void end_rows() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float low = __shfl_down_sync(0xffffffffu, acc[4 * h + i][2 * k + h], 1);
+          if ((lane() & 3) == 0) acc[4 * h + i][2 * k + h] += low;
+        }
+  }
 
   // The warp's unnormalised result of each column c < ncol: part[c * kD + d], ml[2 c] = m, ml[2 c + 1] = l.
   __device__ __forceinline__ void finish(float* part, float* ml, int ncol) {
@@ -432,33 +432,30 @@ struct WarpAttention {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) zs[j][h] += __shfl_xor_sync(0xffffffffu, zs[j][h], o);
+        zs[j][0] += __shfl_xor_sync(0xffffffffu, zs[j][0], o);
+        zs[j][1] += __shfl_xor_sync(0xffffffffu, zs[j][1], o);
       }
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int c = acc_col(j);
+      const int c = col(j);
       if (c < ncol) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (PAIR && h != half()) continue;
-          const int k = PAIR ? 0 : h;
           // codes were 2^-24 (half 1: 2^-20) and weights r times too large; 1 / r is a power of two, exact
-          const float f = 1.f / r[k], u = pow2i(h ? 20 : 24), z = zs[j][k];
+          const float f = 1.f / r[h], u = pow2i(h ? 20 : 24), z = zs[j][h];
+          const int k = QUAD ? h : j;
           float o[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // J = 1: the second column holds the rows' second weight term
-            const float* c2 = acc[4 * h + i];
-            o[2 * i] = fmaf((J == 1 ? c2[0] + c2[1] : c2[j]) * u, f, z);
-            o[2 * i + 1] = fmaf((J == 1 ? c2[2] + c2[3] : c2[2 + j]) * u, f, z);
+            o[2 * i] = fmaf(acc[4 * h + i][k] * u, f, z);
+            o[2 * i + 1] = fmaf(acc[4 * h + i][2 + k] * u, f, z);
           }
           float4* dst = reinterpret_cast<float4*>(part + c * kD + 64 * h + 8 * g);
           dst[0] = make_float4(o[0], o[1], o[2], o[3]);
           dst[1] = make_float4(o[4], o[5], o[6], o[7]);
         }
-        if (g == 0 && (!PAIR || half() == 0)) {
+        if (g == 0) {
           ml[2 * c] = m[j];
           ml[2 * c + 1] = l[j];
         }
