@@ -67,7 +67,7 @@ constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kCols = 8;
-constexpr int kRowUnits = 12;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
+constexpr int kRowUnits = 20;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
 constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
 constexpr int kRingBytes = kWarps * kStages * kTileBytes;
 
