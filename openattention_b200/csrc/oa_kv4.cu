@@ -193,6 +193,7 @@ __device__ __forceinline__ void merge_parts(const float* src, int parts, int nco
 // A CTA's way along the line of rows: the row it is at and its tiles of that row.  Counts of units fit 31 bits
 // (checked by the host).
 struct DenseShare {
+  bool by_warp;           // rows go to single warps: nothing below is set
   unsigned b, r;          // request, row within it
   int n, tiles;           // the request's length, a row's tiles
   int tile, share;        // first tile and number of tiles of this CTA's part
@@ -256,6 +257,11 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
     __syncthreads();
   }
   const unsigned total = units * w.per_req;
+  // Many short rows: a warp each, if that is quicker.  In units (a CTA's time for a tile) a warp takes some 6 for a
+  // tile and 24 for a row, a CTA of the line its share of all.
+  const unsigned warps = grid * kWarps, rounds = (w.rows + warps - 1) / warps;
+  s.by_warp = w.rows >= 2 * grid && most < (1 << 16) && rounds * (6u * most + 24u) < total / grid;
+  if (s.by_warp) return true;
   s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * (8u * grid) <= max((kRowUnits + kWarps) * 8u * grid, 9u * total);
   if (s.own) {
     const unsigned row = cta / w.cpr, j = cta - row * w.cpr;
@@ -328,6 +334,79 @@ __device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& 
   return true;
 }
 
+// Rows of a few tiles: each warp takes whole rows, and nothing is merged.
+template <bool QUAD>
+__device__ __forceinline__ void dense_by_warp(const DenseArgs& a, const DenseWork& w, uint32_t ring) {
+  constexpr int J = WarpAttention<QUAD>::J;
+  const int lane = threadIdx.x & 31, G = a.HQ / a.HKV, cols = G * a.T;
+  WarpAttention<QUAD> at;
+  at.lane_addresses();
+  for (unsigned row = blockIdx.x * kWarps + (threadIdx.x >> 5); row < w.rows; row += gridDim.x * kWarps) {
+    const unsigned b = row / w.per_req, r = row - b * w.per_req;
+    const int kvh = r / w.blocks, col0 = (r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
+    const int n = dense_len(a, b), tiles = dense_tiles(n), whole = n - a.T + 1;
+    const unsigned char* src = a.cache + b * a.c_sb + kvh * a.c_sh + 16 * lane;
+    auto fetch = [&](int k, uint32_t slot) {
+#pragma unroll
+      for (int i = 0; i < kTileBytes / 512; ++i)
+        if (16 * lane + 512 * i < (n - k * kTile) * kRec) cp_async16(ring + slot * kTileBytes + 16 * lane + 512 * i, src + 512 * i);
+      src += kTileBytes;
+    };
+    auto split = [&](int c, int& hh, int& tt) {
+      hh = a.T == 1 ? col0 + c : (col0 + c) / a.T;
+      tt = col0 + c - hh * a.T;
+    };
+    int hh, tt;
+    split(at.op_col(), hh, tt);
+    at.load_q(at.op_col() < ncol ? static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + (int64_t)(kvh * G + hh) * a.q.sh + tt * a.q.st
+                                 : nullptr);
+    __syncwarp();  // the last row's tiles are read
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i < tiles) fetch(i, i);
+      cp_async_commit();
+    }
+    at.begin(a.qk_scale);
+    int sees[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      split(at.col(j), hh, tt);
+      sees[j] = whole + tt;
+    }
+    uint32_t slot = 0;
+    for (int k = 0; k < tiles; ++k) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      uint32_t in[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) in[j] = first_bits(sees[j] - k * kTile);
+      if ((k + 1) * kTile <= whole)
+        at.template tile<false>(ring + slot * kTileBytes, in);
+      else
+        at.template tile<true>(ring + slot * kTileBytes, in);
+      __syncwarp();
+      if (k + kStages - 1 < tiles) fetch(k + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+      cp_async_commit();
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+    }
+    at.add_up();
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (at.col(j) >= ncol) continue;
+      split(at.col(j), hh, tt);
+      const int64_t o_at = b * a.o.sb + (int64_t)(kvh * G + hh) * a.o.sh + tt * a.o.st + 8 * (lane >> 2);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float o[8];
+        at.dims(j, h, o);
+        store_out4(const_cast<void*>(a.o.p), a.out_f32, o_at + 64 * h, 0, make_float4(o[0], o[1], o[2], o[3]), at.l[j]);
+        store_out4(const_cast<void*>(a.o.p), a.out_f32, o_at + 64 * h + 4, 0, make_float4(o[4], o[5], o[6], o[7]), at.l[j]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+}
+
 template <bool QUAD>
 __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
   extern __shared__ __align__(16) unsigned char s_ring[];
@@ -339,6 +418,10 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
   {
     DenseShare mine;
     if (!dense_share(a, w, mine)) return;
+    if (mine.by_warp) {
+      dense_by_warp<QUAD>(a, w, smem_u32(s_ring) + warp * (kStages * kTileBytes));
+      return;
+    }
     if (tid == 0) s = mine;
   }
   __syncthreads();
@@ -525,16 +608,17 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
   const int third = lane / 9;  // lanes 27..31 have no part in a record
   const unsigned char* rec = a.cache + kvh * a.c_sh + 16 * (lane - 9 * third);
   const int64_t prow = (a.per_qhead ? r : kvh) * a.kb_sh + 8 * (lane & 15);
+  const unsigned limit = (unsigned)min(a.Lmax, (int64_t)0x7fffffff);
   auto fetch = [&](int j, int v, int stage) {  // starts an item's copies; returns its live entries
-    const uint32_t dst = ring + stage * kTileBytes;
+    const uint32_t dst = ring + stage * kTileBytes + 16 * lane;
     uint32_t in = 0u;
     if (j < tiles) {
-      in = __ballot_sync(0xffffffffu, v >= 0 && (int64_t)v < a.Lmax);
+      in = __ballot_sync(0xffffffffu, (unsigned)v < limit);
+      const uint32_t mine = third < 3 ? in >> third : 0u;  // bit 3 i: entry 3 i + third
 #pragma unroll
       for (int i = 0; i < 11; ++i) {
-        const int e = 3 * i + third;
-        const int64_t at = (int64_t)__shfl_sync(0xffffffffu, v, e & 31) * kRec;
-        if (third < 3 && e < kTile && (in >> (e & 31) & 1u)) cp_async16(dst + 3 * i * kRec + 16 * lane, rec + at);
+        const int at = __shfl_sync(0xffffffffu, v, third + 3 * i);
+        if (mine >> (3 * i) & 1u) cp_async16(dst + 3 * i * kRec, rec + (int64_t)at * kRec);
       }
     } else if (j < items) {
       in = __ballot_sync(0xffffffffu, !(__int_as_float(v) == -INFINITY));
@@ -544,7 +628,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
         const int e = i + (lane >> 4);
         const bool live = in >> e & 1u;
         const int64_t at = live ? prow + (int64_t)(e0 + e) * a.kb_sb : prow;
-        const uint32_t to = dst + e * 256 + (((lane & 15) ^ e) << 4);
+        const uint32_t to = ring + stage * kTileBytes + e * 256 + (((lane & 15) ^ e) << 4);
         cp_async16_or_zero(to, a.kbar + at, live);
         cp_async16_or_zero(to + 2048, a.vbar + at, live);
       }

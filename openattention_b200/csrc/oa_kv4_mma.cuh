@@ -424,9 +424,8 @@ struct WarpAttention {
         }
   }
 
-  // The warp's unnormalised result of each column c < ncol: part[c * kD + d], ml[2 c] = m, ml[2 c + 1] = l.
-  __device__ __forceinline__ void finish(float* part, float* ml, int ncol) {
-    const int g = lane() >> 2;
+  // Every lane's sums over its column's lanes.
+  __device__ __forceinline__ void add_up() {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
 #pragma unroll
@@ -436,21 +435,31 @@ struct WarpAttention {
         zs[j][1] += __shfl_xor_sync(0xffffffffu, zs[j][1], o);
       }
     }
+  }
+  // after add_up(): dims 64 h + 8 (lane / 4) .. + 7 of column j, unnormalised.  Codes were 2^-24 (half 1: 2^-20) and
+  // weights r times too large; 1 / r is a power of two, exact.
+  __device__ __forceinline__ void dims(int j, int h, float (&o)[8]) const {
+    const float f = 1.f / r[h], u = pow2i(h ? 20 : 24), z = zs[j][h];
+    const int k = QUAD ? h : j;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[2 * i] = fmaf(acc[4 * h + i][k] * u, f, z);
+      o[2 * i + 1] = fmaf(acc[4 * h + i][2 + k] * u, f, z);
+    }
+  }
+
+  // The warp's unnormalised result of each column c < ncol: part[c * kD + d], ml[2 c] = m, ml[2 c + 1] = l.
+  __device__ __forceinline__ void finish(float* part, float* ml, int ncol) {
+    const int g = lane() >> 2;
+    add_up();
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int c = col(j);
       if (c < ncol) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          // codes were 2^-24 (half 1: 2^-20) and weights r times too large; 1 / r is a power of two, exact
-          const float f = 1.f / r[h], u = pow2i(h ? 20 : 24), z = zs[j][h];
-          const int k = QUAD ? h : j;
           float o[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[2 * i] = fmaf(acc[4 * h + i][k] * u, f, z);
-            o[2 * i + 1] = fmaf(acc[4 * h + i][2 + k] * u, f, z);
-          }
+          dims(j, h, o);
           float4* dst = reinterpret_cast<float4*>(part + c * kD + 64 * h + 8 * g);
           dst[0] = make_float4(o[0], o[1], o[2], o[3]);
           dst[1] = make_float4(o[4], o[5], o[6], o[7]);

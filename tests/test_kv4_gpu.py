@@ -471,3 +471,20 @@ def test_dense_long_rows_keep_their_precision():
         w = torch.softmax(K @ q[0, h, 0].double() * D ** -0.5, 0)
         err = (got[0, h, 0].double() - w @ V).norm()
         assert err <= 2 * 2.0 ** -11 * ((w[:, None] * s * code).square().sum().sqrt())
+
+
+@pytest.mark.parametrize("B,HQ,HKV,T,top", [(100, 8, 8, 1, 60), (90, 64, 8, 2, 40), (700, 1, 1, 1, 300), (75, 40, 8, 1, 33)])
+def test_dense_many_short_rows(B, HQ, HKV, T, top):
+    """Enough short rows that single warps take them; some requests are empty."""
+    g = _gen(B + HQ)
+    lens = torch.randint(0, top + 1, (B,), generator=g)
+    cache = _records(g, B, HKV, top)
+    for b in range(B):
+        cache[b, :, int(lens[b]):] = 255
+    q = _rows(g, B, HQ, T, D)
+    for out_dtype in (BF, torch.float32):
+        got = kv4.decode_attention(q.cuda(), cache.cuda(), lens.cuda(), out_dtype=out_dtype).cpu()
+        for i in range(0, B * HQ * T, 53):
+            b, h, t = i // (HQ * T), i // T % HQ, i % T
+            m = max(0, int(lens[b]) - T + 1 + t)
+            P.check(got[b, h, t], *P.attend(q[b, h, t], cache[b, h // (HQ // HKV), :m], D ** -0.5))
