@@ -362,8 +362,8 @@ int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream);
 /* Dense attention over the cache: q (B, HQ, T, 128) bf16 rows, out the same shape in bf16 or fp32 (out_dtype).
  * Request b has min(n[b] + offset, Lmax) positions, its T query tokens are the last T of them and token i sees
  * positions <= length - T + i; one that sees none gives zeros.  Query head h reads KV head h / (HQ / HKV).
- * workspace: oa_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, zero before its first use; every call
- * leaves it ready for the next call of the same sizes.  Calls that share one must not overlap on the GPU. */
+ * workspace: at least oa_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, zero before its first use; every
+ * call leaves it ready for the next call of any sizes.  Calls that share one must not overlap on the GPU. */
 typedef struct {
   oa_tensor4 q, cache, out;
   oa_index n;

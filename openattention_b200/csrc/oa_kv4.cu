@@ -74,7 +74,7 @@ constexpr int kRingBytes = kWarps * kStages * kTileBytes;
 struct DensePlan {
   int blocks;    // column blocks of a KV head: ceil(G T / 8)
   int64_t rows;  // B * HKV * blocks
-  int grid;
+  int grid, most_parts;  // most_parts: two for each CTA of the largest grid
 };
 
 DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax) {
@@ -89,6 +89,7 @@ DensePlan dense_plan(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax
   p.rows = B * HKV * p.blocks;
   const int64_t tiles = (Lmax + kTile - 1) / kTile;
   const int64_t parts = std::max<int64_t>(1, (tiles + kWarps - 1) / kWarps);
+  p.most_parts = 4 * sms;
   // two CTAs per SM (their rings fill its shared memory); no more than one per row and 8 tiles
   p.grid = p.rows > 2 * sms ? 2 * sms : (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, p.rows * parts));
   return p;
@@ -188,6 +189,12 @@ __device__ __forceinline__ void merge_parts(const float* src, int parts, int nco
     for (int v = 0; v < shares; ++v) axpy(A, 1.f, reinterpret_cast<const float4*>(s_a)[v * quads + 32 * warp + lane]);
     store_out4(out, out_f32, o_at, lane, A, s_l[warp]);
   }
+}
+
+__device__ __forceinline__ unsigned take_ticket(unsigned* p) {
+  unsigned v;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // A CTA's way along the line of rows: the row it is at and its tiles of that row.  Counts of units fit 31 bits
@@ -535,12 +542,11 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
         parts = cta_of(s, u + s.tiles - 1) - first + 1;
       }
       unsigned* ticket = w.tickets + s.b * w.per_req + s.r;
-      __threadfence();
+      // the barrier orders the CTA's stores before thread 0's release, and its acquire before the CTA's loads
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(ticket, 1u) == parts - 1 ? 1u : 0u;
+      if (tid == 0) s_last = take_ticket(ticket) == parts - 1 ? 1u : 0u;
       __syncthreads();
       if (s_last) {
-        __threadfence();
         merge_parts<QUAD ? 6 : 4>(w.parts + (2 * first + 1) * (int64_t)kPartFloats, (int)parts, ncol, s_part,
                                   const_cast<void*>(a.o.p), a.out_f32, o_at);
         if (tid == 0) *ticket = 0u;
@@ -741,7 +747,9 @@ int launch_list(const ListArgs& a, int64_t rows, int S, const char* fn, cudaStre
   return oa_check_launch(fn);
 }
 
-size_t ticket_bytes(int64_t rows) { return ((size_t)rows * sizeof(unsigned) + 255) & ~size_t(255); }
+// A workspace: the parts of the largest grid, then a ticket per row.  Where the tickets lie does not depend on the
+// call, so calls of any sizes can share a workspace that is large enough for each.
+size_t workspace_bytes(const DensePlan& p) { return (size_t)p.most_parts * kPartFloats * sizeof(float) + (size_t)p.rows * sizeof(unsigned); }
 
 }  // namespace
 }  // namespace oa
@@ -749,7 +757,7 @@ size_t ticket_bytes(int64_t rows) { return ((size_t)rows * sizeof(unsigned) + 25
 extern "C" size_t oa_kv4_attention_workspace_bytes(int64_t B, int64_t HQ, int64_t HKV, int64_t T, int64_t Lmax) {
   if (B <= 0 || T <= 0 || HKV <= 0 || HQ < HKV || Lmax < 0) return 0;
   const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
-  return oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
+  return oa::workspace_bytes(p);
 }
 
 extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream) {
@@ -781,7 +789,7 @@ extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream)
   const int64_t most_units = p.rows * ((Lmax + oa::kTile - 1) / oa::kTile + 1 + oa::kRowUnits);
   OA_REQUIRE(most_units <= 0xffffffffll / 9 && most_units / std::max<int64_t>(p.rows, 1) * 8 * p.grid <= 0xffffffffll,
              "%s: too many records (B * HKV * Lmax) for one call", fn);
-  const size_t need = oa::ticket_bytes(p.rows) + (size_t)p.grid * 2 * oa::kPartFloats * sizeof(float);
+  const size_t need = oa::workspace_bytes(p);
   OA_REQUIRE(workspace && workspace_bytes >= need && oa_aligned16(workspace),
              "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need, workspace_bytes);
   oa::DenseWork w;
@@ -789,8 +797,8 @@ extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream)
   w.per_req = (unsigned)(HKV * p.blocks);
   w.rows = (unsigned)p.rows;
   w.cpr = (unsigned)(p.grid / p.rows);
-  w.tickets = static_cast<unsigned*>(workspace);
-  w.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + oa::ticket_bytes(p.rows));
+  w.parts = static_cast<float*>(workspace);
+  w.tickets = reinterpret_cast<unsigned*>(w.parts + (size_t)p.most_parts * oa::kPartFloats);
   const auto kernel = HQ / HKV * T <= 4 ? &oa::dense_kernel<true> : &oa::dense_kernel<false>;
   const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(kernel), oa::kRingBytes, fn, true);
   if (rc != OA_OK) return rc;

@@ -98,24 +98,31 @@ _ws_cache: dict = {}
 
 
 def attention_workspace(B, HQ, T, cache_len, dev, hkv=HKV):
-    """Scratch of decode_attention for these sizes (uint8, zero-filled; None where it needs none).  Calls that
-    can overlap on the GPU must not share one."""
-    need = _lib.load().oa_kv4_attention_workspace_bytes(B, HQ, hkv, T, cache_len)
-    return torch.zeros(need, dtype=torch.uint8, device=dev) if need else None
+    """Scratch of decode_attention (uint8, zero-filled, 2.4 MB and 4 bytes a row) for these sizes and all that have no
+    more requests, KV heads and blocks of 8 queries of a KV head.  Calls that can overlap on the GPU must not share
+    one."""
+    with torch.cuda.device(dev):
+        need = _lib.load().oa_kv4_attention_workspace_bytes(B, HQ, hkv, T, cache_len)
+    return torch.zeros(max(need, 16), dtype=torch.uint8, device=dev)
 
 
 def _workspace(dev, *sizes):
-    """The kept workspace of these sizes, one for each GPU and stream: calls on one stream run in order and may share
-    it.  A call that is being captured gets its own from the graph's pool, where its zero-fill is replayed too."""
+    """The kept workspace of a GPU and stream, grown on demand: calls on one stream run in order and may share it.  A
+    call that is being captured gets its own from the graph's pool, where its zero-fill is replayed too."""
     capturing = torch.cuda.is_current_stream_capturing()
-    key = (dev, _current_stream(dev), *sizes)
-    ws = None if capturing else _ws_cache.get(key)
-    if ws is None:
-        with torch.cuda.device(dev):
-            need = _lib.load().oa_kv4_attention_workspace_bytes(*sizes)
-        ws = torch.zeros(max(need, 16), dtype=torch.uint8, device=f"cuda:{dev}")
-        if not capturing:
-            _ws_cache[key] = ws
+    key = (dev, _current_stream(dev))
+    kept = None if capturing else _ws_cache.get(key)
+    if kept is not None and sizes in kept[1]:
+        return kept[0]
+    with torch.cuda.device(dev):
+        need = _lib.load().oa_kv4_attention_workspace_bytes(*sizes)
+    if kept is not None and kept[0].numel() >= need:
+        if len(kept[1]) < 4096:
+            kept[1].add(sizes)
+        return kept[0]
+    ws = torch.zeros(max(need, 16), dtype=torch.uint8, device=f"cuda:{dev}")
+    if not capturing:
+        _ws_cache[key] = (ws, {sizes})
     return ws
 
 
@@ -128,8 +135,8 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
     reads KV head h // (HQ // hkv).  A query token before the first position (a length below T, zero or
     negative) gives zeros.  Records at positions >= the length are never used.  sm_scale defaults to 128**-0.5.
 
-    workspace: attention_workspace(...) of the same sizes.  By default one is kept for each device, stream and
-    size; a call that is being captured allocates its own from the graph's pool (graphs may then be replayed
+    workspace: attention_workspace(...) of these sizes or larger ones.  By default one is kept for each device and
+    stream; a call that is being captured allocates its own from the graph's pool (graphs may then be replayed
     side by side), so a decode loop that captures many layers passes one."""
     dev, fc = _device_of("q", q), _cache(cache)
     fq = _rows("q", q, torch.bfloat16, dev)

@@ -488,3 +488,19 @@ def test_dense_many_short_rows(B, HQ, HKV, T, top):
             b, h, t = i // (HQ * T), i // T % HQ, i % T
             m = max(0, int(lens[b]) - T + 1 + t)
             P.check(got[b, h, t], *P.attend(q[b, h, t], cache[b, h // (HQ // HKV), :m], D ** -0.5))
+
+
+def test_dense_calls_of_any_size_share_a_workspace():
+    """Sizes large, small, ragged and large again, through the kept workspace and through one of the caller's."""
+    g = _gen(61)
+    ws = kv4.attention_workspace(40, 32, 2, 700, "cuda")
+    for B, HQ, HKV, T, top in ((40, 32, 8, 2, 700), (1, 4, 2, 1, 2500), (7, 16, 8, 1, 90), (40, 32, 8, 2, 650), (2, 8, 8, 1, 1300)):
+        lens = torch.randint(1, top + 1, (B,), generator=g)
+        cache, q = _records(g, B, HKV, top), _rows(g, B, HQ, T, D)
+        a = kv4.decode_attention(q.cuda(), cache.cuda(), lens.cuda(), workspace=ws)
+        b = kv4.decode_attention(q.cuda(), cache.cuda(), lens.cuda())
+        assert torch.equal(a, b)
+        for i in range(0, B * HQ * T, 1 + B * HQ * T // 9):
+            bb, h, t = i // (HQ * T), i // T % HQ, i % T
+            m = max(0, int(lens[bb]) - T + 1 + t)
+            P.check(a.cpu()[bb, h, t], *P.attend(q[bb, h, t], cache[bb, h // (HQ // HKV), :m], D ** -0.5))
