@@ -42,10 +42,6 @@ struct ListArgs {
   float qk_scale;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& w, float* f) {
-  f[0] = bf_lo(w.x); f[1] = bf_hi(w.x); f[2] = bf_lo(w.y); f[3] = bf_hi(w.y);
-  f[4] = bf_lo(w.z); f[5] = bf_hi(w.z); f[6] = bf_lo(w.w); f[7] = bf_hi(w.w);
-}
 __device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, float A, float L) {
   const float o = L == 0.f ? 0.f : A / L;
   if (a.out_f32)

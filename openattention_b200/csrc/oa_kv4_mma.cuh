@@ -87,11 +87,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t at, int imm) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at + imm));
   return v;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t at, int imm) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + imm));
-  return v;
-}
 
 // Token (0..15 of a 16-token block) of MMA row r (0..7); row r + 8 holds the next token.
 __device__ __forceinline__ int row_token(int r) { return (r & 1) ? 8 + ((r + 3) & 7) : r; }

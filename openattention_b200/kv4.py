@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .geometry import D, HKV
-from .rotary import _call, _CODE, _current_stream, _device_of, _index, _like, _rows, _same_device, _table, _weights
+from .rotary import _call, _CODE, _current_stream, _device_of, _index, _like, _no_grad, _rows, _same_device, _table, _weights
 
 REC = 144
 
@@ -134,6 +134,7 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
     tokens the last T positions; token i sees positions <= length - T + i.  HQ is a multiple of hkv, query head h
     reads KV head h // (HQ // hkv).  A query token before the first position (a length below T, zero or
     negative) gives zeros.  Records at positions >= the length are never used.  sm_scale defaults to 128**-0.5.
+    out must not overlap q or the cache.
 
     workspace: attention_workspace(...) of these sizes or larger ones.  By default one is kept for each device and
     stream; a call that is being captured allocates its own from the graph's pool (graphs may then be replayed
@@ -168,11 +169,11 @@ def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, s
     One softmax over the tokens of sel_idx (BQ, n_sel) and exp_idx (BQ, n_exp) (int32; an index outside [0, Lmax)
     is padding) and nb cluster proxies with logits q . kbar * sm_scale + log_n (log_n = -inf skips one).
     kbar, vbar bf16 (BQ, NB, 128) (for each query row) or (BH, NB, 128) (for each KV row), log_n (BQ, NB) fp32;
-    nb = 0 disables the proxies.  A row with nothing to attend gives zeros."""
+    nb = 0 disables the proxies.  A token that a row lists twice counts twice.  A row with nothing to attend gives
+    zeros.  out must not overlap the inputs."""
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype is not torch.bfloat16 or q.dim() != 2:
         raise RuntimeError("q must be a (rows, 128) bf16 CUDA tensor")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("q requires a gradient: this operator has no backward pass (use torch.no_grad())")
+    _no_grad("q", q)
     fc, dev = _cache(cache, ndim=3), q.get_device()
     _same_device(dev, cache=cache, sel_idx=sel_idx, exp_idx=exp_idx, out=out)
     if sel_idx.dtype is not torch.int32 or sel_idx.dim() != 2 or exp_idx.dtype is not torch.int32 or exp_idx.dim() != 2:
@@ -185,6 +186,8 @@ def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, s
         if kbar is None or vbar is None or log_n is None or kbar.dtype is not torch.bfloat16 or kbar.dim() != 3 or \
                 vbar.dtype is not torch.bfloat16 or vbar.dim() != 3 or log_n.dtype is not torch.float32 or log_n.dim() != 2:
             raise RuntimeError("kbar and vbar must be (rows, NB, 128) bf16 and log_n (rows, NB) fp32")
+        for name, t in (("kbar", kbar), ("vbar", vbar), ("log_n", log_n)):
+            _no_grad(name, t)
         fb = (kbar.data_ptr(), *kbar.shape, *kbar.stride(), vbar.data_ptr(), *vbar.shape, *vbar.stride())
         fl = (log_n.data_ptr(), *log_n.shape, *log_n.stride())
     if out is None:

@@ -113,6 +113,8 @@ class RandomLlama:
         """tokens (B, T) int64.  Fills every layer's K/V cache for positions [0, T), builds the index of
         every layer and request, and returns the greedy next token (B,)."""
         B, T = tokens.shape
+        if B > self.B or not 1 <= T <= self.Lmax:
+            raise RuntimeError(f"tokens must be (up to {self.B}, 1..{self.Lmax}), got {tuple(tokens.shape)}")
         nxt = torch.empty(B, dtype=torch.long, device=self.dev)
         for b in range(B):
             x = self.embed[tokens[b]]                                      # (T, H)
@@ -182,11 +184,19 @@ class RandomLlama:
         C.n_dev = torch.full((1,), n0, dtype=torch.int32, device=self.dev)    # before the step
         C.kv_idx = torch.full((1,), n0 - 1, dtype=torch.int64, device=self.dev)
         C.n0_dev = torch.full((1,), n0, dtype=torch.int32, device=self.dev)
+        self.left = self.Lmax - n0  # positions that steps can still take
         self.n_host = n0 + 1  # ns / nl / k_top of the step (constant over a decode window)
         self.tok = first.to(self.dev).clone()
 
+    def _take_position(self):
+        # the counters are on the device: a step past the caches would go unnoticed there
+        if self.left < 1:
+            raise RuntimeError(f"the caches are full: {self.Lmax} positions")
+        self.left -= 1
+
     @torch.no_grad()
     def step_eager(self) -> torch.Tensor:
+        self._take_position()
         self.tok = self._decode_body(self.tok, self.n_host)
         return self.tok
 
@@ -219,6 +229,7 @@ class RandomLlama:
 
     @torch.no_grad()
     def step_graph(self) -> torch.Tensor:
+        self._take_position()
         self.graph.replay()
         self._tok_in.copy_(self._tok_out)
         return self._tok_out

@@ -27,7 +27,12 @@ def _bad_rows(name, t, dtype, dev):
         raise RuntimeError(f"{name} must be (B, heads, T, 128), got {tuple(t.shape)}")
     if t.get_device() != dev:
         raise RuntimeError(f"{name} must be a tensor on cuda:{dev}, got {t.device}")
-    raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (use torch.no_grad())")
+    _no_grad(name, t)
+
+
+def _no_grad(name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient: this operator has no backward pass (use torch.no_grad())")
 
 
 def _rows(name, t, dtype, dev):
@@ -70,6 +75,7 @@ def _table(cos, sin, dev):
                 not t.is_contiguous() or (t is not cos and t.shape != cos.shape):
             raise RuntimeError(f"{name} must be a contiguous fp32 (positions, rotated dims) table on cuda:{dev}, the "
                                "same shape for both")
+        _no_grad(name, t)
     return cos.data_ptr(), sin.data_ptr(), *cos.shape
 
 
@@ -82,6 +88,7 @@ def _weights(q_weight, k_weight, dtype, dev):
         if not isinstance(w, torch.Tensor) or w.get_device() != dev or w.shape != (D,) or not w.is_contiguous() or \
                 w.dtype not in (dtype, torch.float32) or w.dtype != given[0].dtype:
             raise RuntimeError(f"norm weights must be contiguous ({D},) tensors on cuda:{dev}, both {dtype} or both fp32")
+        _no_grad("a norm weight", w)
     return _lib.ptr(q_weight), _lib.ptr(k_weight), _CODE[given[0].dtype]
 
 

@@ -88,6 +88,8 @@ ROPE = [
     (dict(q_out=_r(1, 4, 3)), "q_out must be"),
     (dict(q_out=_r(1, 1, 2).expand(1, 4, 2, D)), "expanded"),
     (dict(q=_r(1, 4, 2).requires_grad_()), "no backward pass"),
+    (dict(k_weight=torch.zeros(D, requires_grad=True)), "no backward pass"),
+    (dict(cos=torch.zeros(8, 128, requires_grad=True)), "no backward pass"),
 ]
 
 
@@ -151,7 +153,7 @@ def test_decode_attention_refusals(entry, change, match):
     (dict(nb=9), "kbar and vbar must be"), (dict(nb=-1), "bad list sizes"), (dict(vbar=_r(4, 5)), "kbar and vbar"),
     (dict(kbar=_r(3, 6), vbar=_r(3, 6)), "kbar and vbar must be"), (dict(kbar=None, nb=2), "kbar must be|kbar and vbar"),
     (dict(log_n=torch.zeros(4, 4)), "log_n"), (dict(out=torch.zeros(4, 64)), r"\(4, 128\)"),
-    (dict(out=_r(1).expand(4, D)), "overlap")])
+    (dict(out=_r(1).expand(4, D)), "overlap"), (dict(vbar=_r(4, 6).requires_grad_()), "no backward pass")])
 def test_flash_attention_refusals(entry, change, match):
     i = torch.zeros(4, 2, dtype=torch.int32)
     _refused(kv4.flash_attention, dict(q=_r(4), cache=_c(2, 8), sel_idx=i, exp_idx=i, kbar=_r(4, 6), vbar=_r(4, 6),

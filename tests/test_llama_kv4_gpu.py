@@ -82,3 +82,18 @@ def test_prefill_keys_are_the_eager_rotations(monkeypatch):
 
     assert torch.equal(seen["out"][0], eager(seen["q"]))
     assert torch.equal(model.K[0][0, :, :T], eager(seen["k"])[0])
+
+
+@pytest.mark.parametrize("four_bits", [False, True])
+def test_tokens_past_the_caches_are_refused(four_bits):
+    cfg = L.LlamaConfig(layers=1, ffn=256, vocab=512, kv4=four_bits)
+    T = 1030
+    model = L.RandomLlama(cfg, 1, T + 2, "cuda", rho=0.01, seed=9)
+    with pytest.raises(RuntimeError, match="tokens must be"):
+        model.prefill(torch.zeros(1, T + 3, dtype=torch.int64, device="cuda"))
+    model.start_decode(T, model.prefill(torch.arange(T, device="cuda")[None] % cfg.vocab))
+    model.step_eager()
+    model.step_eager()
+    with pytest.raises(RuntimeError, match="caches are full"):
+        model.step_eager()
+    torch.cuda.synchronize()
