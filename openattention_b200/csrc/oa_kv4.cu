@@ -55,6 +55,7 @@ __device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, 
 // CTAs of 8 warps, each warp with its own ring of kStages tiles filled by asynchronous copies (the 4608 bytes
 // of a tile are contiguous).  Lengths live on the device, so each CTA finds its share itself:
 //  - each row its own CTAs, grid / rows of them (no more than one per 8 tiles), where that balances;
+//  - many short rows: a warp each, nothing to merge;
 //  - else the tiles of all rows in one line, cut into equal parts; a CTA then ends one row and begins the next.
 // A row that one CTA covers is written by it.  Otherwise each part leaves (m, l, O) in the workspace and the
 // last CTA to arrive (atomic ticket, no waiting) merges the parts in CTA order, so the result does not depend
@@ -64,6 +65,7 @@ constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kCols = 8;
 constexpr int kRowUnits = 20;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
+constexpr int kLineUnits = kRowUnits + kWarps;  // what a CTA's second row costs it, in tiles
 constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
 constexpr int kRingBytes = kWarps * kStages * kTileBytes;
 
@@ -260,12 +262,14 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
     __syncthreads();
   }
   const unsigned total = units * w.per_req;
-  // Many short rows: a warp each, if that is quicker.  In units (a CTA's time for a tile) a warp takes some 6 for a
-  // tile and 24 for a row, a CTA of the line its share of all.
-  const unsigned warps = grid * kWarps, rounds = (w.rows + warps - 1) / warps;
-  s.by_warp = w.rows >= 2 * grid && most < (1 << 16) && rounds * (6u * most + 24u) < total / grid;
+  // Many short rows: a warp each, if that is quicker.  In units (a CTA's time for a tile when all work, 0.2 us) a warp
+  // alone takes 4.4 for a tile and all warps together 1.2 for a CTA's worth, a further round 10; the line its share and
+  // some 10 more.  (128 requests of 600 tokens: 22.7 us by warps, 33.1 on the line; 64 of 1000: 33.0 and 27.0.)
+  const float warps = (float)(grid * kWarps), work = (float)w.rows * (float)most, rounds = ceilf((float)w.rows / warps);
+  s.by_warp = w.cpr == 0 && most < (1 << 16) &&
+              fmaxf(1.2f * work, 4.4f * rounds * (float)(most * grid)) + 10.f * (rounds - 2.f) * (float)grid < (float)total;
   if (s.by_warp) return true;
-  s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * (8u * grid) <= max((kRowUnits + kWarps) * 8u * grid, 9u * total);
+  s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * grid <= total + kLineUnits * grid;
   if (s.own) {
     const unsigned row = cta / w.cpr, j = cta - row * w.cpr;
     if (row >= w.rows) return false;
@@ -344,7 +348,7 @@ __device__ __forceinline__ void dense_by_warp(const DenseArgs& a, const DenseWor
   const int lane = threadIdx.x & 31, G = a.HQ / a.HKV, cols = G * a.T;
   WarpAttention<QUAD> at;
   at.lane_addresses();
-  for (unsigned row = blockIdx.x * kWarps + (threadIdx.x >> 5); row < w.rows; row += gridDim.x * kWarps) {
+  for (unsigned row = blockIdx.x + (threadIdx.x >> 5) * gridDim.x; row < w.rows; row += gridDim.x * kWarps) {
     const unsigned b = row / w.per_req, r = row - b * w.per_req;
     const int kvh = r / w.blocks, col0 = (r - kvh * w.blocks) * kCols, ncol = min(kCols, cols - col0);
     const int n = dense_len(a, b), tiles = dense_tiles(n), whole = n - a.T + 1;
@@ -863,17 +867,16 @@ extern "C" int oa_kv4_flash(const oa_kv4_flash_args* args, void* stream) {
   a.out_f32 = g.out_dtype == OA_F32;
   a.G = (int)(BQ / BH);
   a.qk_scale = (float)(g.sm_scale * (double)oa::kLog2e);
-  // Warps per row: enough that all rows together fill the GPU's 16 warps per SM, but two items each; up to 8 in a
-  // CTA, beyond that a cluster of CTAs.
-  const int64_t fill = 148 * 16 / BQ, work = ((n_sel + n_exp + oa::kTile - 1) / oa::kTile + (NB + oa::kRowsPerTile - 1) / oa::kRowsPerTile + 1) / 2;
-  const int64_t warps = std::min(fill, work);
+  // Warps per row.  Few rows: clusters of 8-warp CTAs, no more CTAs than SMs and an item for each warp (32 rows of 1350
+  // entries and 192 proxies 14.4 us on one CTA each, 10.3 on clusters of 4, 11.2 of 8; 128 rows 16.4, and 18.4 on
+  // clusters of 2).  Else as many warps as make up 16 on every SM, with two items each (256 rows of 694 entries: 19.7 us
+  // with 8, 20.5 with 4; 1024 rows of 231: 29.1 with 8, 26.5 with 4, 24.6 with 2).
+  const int64_t items = (n_sel + n_exp + oa::kTile - 1) / oa::kTile + (NB + oa::kRowsPerTile - 1) / oa::kRowsPerTile;
+  int S = 1;
+  while (S < 8 && BQ * 2 * S <= 148 && 16 * S <= items) S *= 2;
+  const int64_t warps = std::min(148 * 16 / BQ, (items + 1) / 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (warps >= 16) {
-    const int S = warps >= 64 ? 8 : warps >= 32 ? 4 : 2;
-    OA_REQUIRE(BQ * S <= 0x7fffffff, "%s: too many rows", fn);
-    return oa::launch_list<8>(a, BQ, S, fn, st);
-  }
-  if (warps >= 8) return oa::launch_list<8>(a, BQ, 1, fn, st);
+  if (S > 1 || warps >= 8) return oa::launch_list<8>(a, BQ, S, fn, st);
   if (warps >= 4) return oa::launch_list<4>(a, BQ, 1, fn, st);
   return oa::launch_list<2>(a, BQ, 1, fn, st);
 }
