@@ -164,23 +164,22 @@ __device__ __forceinline__ uint32_t max_bf2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// a / b from r, 1 / b to within an ulp: the product, and one correction by its remainder, where nothing over- or
-// underflows.  Exact where the quotient is a float (a tie between two codes among them), else within an ulp of it.
-__device__ __forceinline__ float divide(float a, float b, float r) {
-  const float q = a * r;
-  return fmaf(fmaf(-q, b, a), r, q);
-}
-
-__device__ __forceinline__ float reciprocal(float x) {  // of a normal number with a normal reciprocal, within an ulp
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return fmaf(fmaf(-x, r, 1.f), r, r);
-}
+// 1 / x in two terms, off by 2^-45 of it: of a normal number with a normal reciprocal
+struct Reciprocal {
+  float hi, lo;
+  explicit __device__ __forceinline__ Reciprocal(float x) {
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(x));
+    lo = fmaf(-x, hi, 1.f) * hi;
+  }
+  // a / x, rounded once as far as 45 bits tell: exact where it is a float (a tie between two codes among them)
+  __device__ __forceinline__ float times(float a) const { return fmaf(a, hi, a * lo); }
+};
 
 // Scale of the group in the low (0) or high (1) halves of the two packed extremes.
 __device__ __forceinline__ float group_scale(uint32_t lo2, uint32_t hi2, int g) {
   const float lo = g ? bf_hi(lo2) : bf_lo(lo2), hi = g ? bf_hi(hi2) : bf_lo(hi2);
-  return bf_round(divide(hi - lo, 15.f, 1.f / 15.f));
+  const float d = hi - lo, q = d * (1.f / 15.f);
+  return bf_round(fmaf(fmaf(-q, 15.f, d), 1.f / 15.f, q));  // a quotient's one correction by its remainder
 }
 // The lane's eight codes as four bytes, and both groups' (scale, offset) words.  kLift: some scale is near fp32's
 // smallest numbers (or zero).
@@ -194,13 +193,13 @@ __device__ __forceinline__ void code_groups(const uint32_t (&v)[4], uint32_t lo2
     const float lo = g ? bf_hi(lo2) : bf_lo(lo2), s = g ? s1 : s0;
     const bool ok = s < INFINITY;  // a NaN, an infinity or a range past fp32 is not
     const float lift = kLift && s < 0x1p-60f ? 0x1p80f : 1.f, ss = kLift ? s * lift : s;
-    const float inv = !kLift || s > 0.f ? reciprocal(ss) : 0.f;
+    const Reciprocal inv(kLift && s == 0.f ? 1.f : ss);  // a scale of 0: all differences are 0
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float d = (g ? bf_hi(v[i]) : bf_lo(v[i])) - lo;
       if (kLift) d *= lift;
-      float q = divide(d, ss, inv);
+      float q = inv.times(d);
       if (kLift) q = fminf(q, 15.f);  // a normal scale is off by 2^-9 at most, its quotients stay under 15.1
       w[i] = __float_as_uint(q + kRound);
     }
