@@ -36,7 +36,7 @@ struct RowArgs {
   float eps;
   int zero_q, zero_k;  // write zeros into padding rows
   int B, T, HQ, HKV;
-  int slots, per;      // slots of a token, slots a warp takes
+  int slots, per;      // slots of a token (append_kernel: pairs of heads), slots a warp takes
 };
 
 // The lane's part of a row: dims 4l .. (a) and 64 + 4l .. (b); p at dim 4l.  Held as loaded, so that several rows'
@@ -181,54 +181,65 @@ __device__ __forceinline__ float group_scale(uint32_t lo2, uint32_t hi2, int g) 
   const float d = hi - lo, q = d * (1.f / 15.f);
   return bf_round(fmaf(fmaf(-q, 15.f, d), 1.f / 15.f, q));  // a quotient's one correction by its remainder
 }
-// The lane's eight codes as four bytes, and both groups' (scale, offset) words.  kLift: some scale is near fp32's
-// smallest numbers (or zero).
-template <bool kLift>
-__device__ __forceinline__ void code_groups(const uint32_t (&v)[4], uint32_t lo2, float s0, float s1, uint32_t& word,
+// The lane's codes, dims (i, 64 + i) in a byte, and both groups' (scale, offset) words.  kLift: some scale is near
+// fp32's smallest numbers (or zero).
+template <bool kLift, int N>
+__device__ __forceinline__ void code_groups(const uint32_t (&v)[N], uint32_t lo2, float s0, float s1, uint32_t (&word)[N / 4],
                                             uint32_t (&out)[2]) {
   constexpr float kRound = 12582912.f;  // 0x4b400000: a code is the sum's lowest byte
-  word = 0u;
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) word[j] = 0u;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     const float lo = g ? bf_hi(lo2) : bf_lo(lo2), s = g ? s1 : s0;
     const bool ok = s < INFINITY;  // a NaN, an infinity or a range past fp32 is not
     const float lift = kLift && s < 0x1p-60f ? 0x1p80f : 1.f, ss = kLift ? s * lift : s;
     const Reciprocal inv(kLift && s == 0.f ? 1.f : ss);  // a scale of 0: all differences are 0
-    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float d = (g ? bf_hi(v[i]) : bf_lo(v[i])) - lo;
-      if (kLift) d *= lift;
-      float q = inv.times(d);
-      if (kLift) q = fminf(q, 15.f);  // a normal scale is off by 2^-9 at most, its quotients stay under 15.1
-      w[i] = __float_as_uint(q + kRound);
+    for (int j = 0; j < N / 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float d = (g ? bf_hi(v[4 * j + i]) : bf_lo(v[4 * j + i])) - lo;
+        if (kLift) d *= lift;
+        float q = inv.times(d);
+        if (kLift) q = fminf(q, 15.f);  // a normal scale is off by 2^-9 at most, its quotients stay under 15.1
+        w[i] = __float_as_uint(q + kRound);
+      }
+      const uint32_t codes4 = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+      word[j] |= ok ? codes4 << (4 * g) : 0u;
     }
-    const uint32_t codes4 = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
-    word |= ok ? codes4 << (4 * g) : 0u;
     out[g] = ok ? pack2(s, lo) : 0x00007fc0u;
   }
 }
 
-// The half-warp's row, as bf16x2 of dims (4l + i, 64 + 4l + i), into one side of a record.  The halves of the head lie
-// side by side, so one bf16x2 minimum and maximum serve both groups; NaN and infinities show in them.  Adding
-// 3 * 2^22 to a quotient rounds it to the nearest whole number, ties to even, in the low bits.  Scales near fp32's
-// smallest are lifted by 2^80 first.  Called by whole warps.
-__device__ __forceinline__ void quantise_row(const uint32_t (&v)[4], unsigned char* codes, int meta, int hl) {
-  uint32_t lo2 = min_bf2(min_bf2(v[0], v[1]), min_bf2(v[2], v[3]));
-  uint32_t hi2 = max_bf2(max_bf2(v[0], v[1]), max_bf2(v[2], v[3]));
+// A row that 64 / N lanes hold, lane l as bf16x2 of dims (N l + i, 64 + N l + i), into one side of a record.  The halves
+// of the head lie side by side, so one bf16x2 minimum and maximum serve both groups; NaN and infinities show in them.
+// Adding 3 * 2^22 to a quotient rounds it to the nearest whole number, ties to even, in the low bits.  Scales near
+// fp32's smallest are lifted by 2^80 first.  Called by whole warps; live: the row is stored.
+template <int N>
+__device__ __forceinline__ void quantise_row(const uint32_t (&v)[N], unsigned char* codes, int meta, int l, bool live) {
+  uint32_t lo2 = v[0], hi2 = v[0];
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) {
+  for (int i = 1; i < N; ++i) {
+    lo2 = min_bf2(lo2, v[i]);
+    hi2 = max_bf2(hi2, v[i]);
+  }
+#pragma unroll
+  for (int o = 32 / N; o >= 1; o >>= 1) {
     lo2 = min_bf2(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
     hi2 = max_bf2(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
   }
-  uint32_t word, out[2];
+  uint32_t word[N / 4], out[2];
   const float s0 = group_scale(lo2, hi2, 0), s1 = group_scale(lo2, hi2, 1);
   if (__any_sync(0xffffffffu, fminf(s0, s1) < 0x1p-60f))
     code_groups<true>(v, lo2, s0, s1, word, out);
   else
     code_groups<false>(v, lo2, s0, s1, word, out);
-  *reinterpret_cast<uint32_t*>(codes + 4 * hl) = word;
-  if (hl == 0) *reinterpret_cast<uint2*>(codes + meta) = make_uint2(out[0], out[1]);
+  if (!live) return;
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) reinterpret_cast<uint32_t*>(codes + N * l)[j] = word[j];
+  if (l == 0) *reinterpret_cast<uint2*>(codes + meta) = make_uint2(out[0], out[1]);
 }
 
 // One half-warp's rows h0, h0 + step, ... below h1 of one token, kSlots at a time: normalised, rotated, stored.  Rows
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
   const unsigned b = a.T == 1 ? token : token / a.T, t = token - b * a.T;
   const int64_t pos = per_request(a.start, b) + a.offset + t;
   bool live = a.lens.p == nullptr || (int64_t)t < per_request(a.lens, b);
-  if (a.cos) live = live && pos >= 0 && pos < a.P;
+  live = live && pos >= 0 && pos < a.P;
   const int s0 = blockIdx.y * a.per, s1 = min(s0 + a.per, a.slots);
   const E* q = static_cast<const E*>(a.q.p) + b * a.q.sb + t * a.q.st + 4 * hl;
   E* qo = static_cast<E*>(const_cast<void*>(a.qo.p)) + b * a.qo.sb + t * a.qo.st + 4 * hl;
@@ -286,10 +297,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
     return;
   }
   float cs[8], sn[8];
-  if (a.cos) {
-    load_table(a.cos + pos * a.R, a.R, hl, cs);
-    load_table(a.sin + pos * a.R, a.R, hl, sn);
-  }
+  load_table(a.cos + pos * a.R, a.R, hl, cs);
+  load_table(a.sin + pos * a.R, a.R, hl, sn);
   if (CACHE && k0 < k1 && pos >= 0 && pos < a.Lmax) {
     const Rows& r = half ? a.v : a.k;
     const E* p = static_cast<const E*>(r.p) + b * r.sb + t * r.st + 4 * hl + k0 * r.sh;
@@ -301,15 +310,14 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
     auto write = [&](const Quads<E>& raw) {  // one head's K and V row into its record
       uint32_t v[4];
       raw.pairs(v);
-      if (a.cos) {  // the V rows of the warp go through the shuffles with the K rows and come out as they were
-        float x[8];
-        raw.get(x);
-        if (a.wk) norm_row(x, wf, a.eps);
-        rotate_row<FULL>(x, cs, sn, a.R, hl);
+      // the V rows of the warp go through the shuffles with the K rows and come out as they were
+      float x[8];
+      raw.get(x);
+      if (a.wk) norm_row(x, wf, a.eps);
+      rotate_row<FULL>(x, cs, sn, a.R, hl);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = half ? v[i] : pack2(x[i], x[4 + i]);  // the cache holds bf16 rows
-      }
-      quantise_row(v, codes, meta, hl);
+      for (int i = 0; i < 4; ++i) v[i] = half ? v[i] : pack2(x[i], x[4 + i]);  // the cache holds bf16 rows
+      quantise_row(v, codes, meta, hl, true);
       codes += a.c_sh;
     };
     int h = k0;
@@ -332,6 +340,48 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const RowArgs a) {
     rotate_rows<E, FULL, kSlots>(k, a.k.sh, ko, a.ko.sh, k0, k1, half, a.wk, a, cs, sn, hl);
   }
   if (q0 < q1) rotate_rows<E, FULL, kSlots>(q, a.q.sh, qo, a.qo.sh, q0, q1, half, a.wq, a, cs, sn, hl);
+}
+
+// Rows into the cache as they are.  Eight lanes to a row, lane l dims 8l .. 8l + 7 and 64 + 8l .. + 7 (a row's minimum and
+// maximum are then three exchanges, and what a group costs once is shared by two heads' rows); a warp takes the K and V
+// rows of two heads at a time, kPairs of them in flight.
+template <int kPairs>
+__global__ void __launch_bounds__(kRowThreads) append_kernel(const RowArgs a) {
+  const int lane = threadIdx.x & 31, l = lane & 7, side = lane >> 3 & 1, sub = lane >> 4;
+  const unsigned token = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  if (token >= (unsigned)a.B * a.T) return;
+  const unsigned b = a.T == 1 ? token : token / a.T, t = token - b * a.T;
+  const int64_t pos = per_request(a.start, b) + a.offset + t;
+  if (pos < 0 || pos >= a.Lmax || (a.lens.p && (int64_t)t >= per_request(a.lens, b))) return;
+  const Rows& r = side ? a.v : a.k;
+  const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(r.p) + b * r.sb + t * r.st + 8 * l;
+  const int64_t sh = r.sh;
+  unsigned char* rec = a.cache + b * a.c_sb + pos * kRec + (side ? kRecV : 0);
+  const int meta = side ? kRecMeta + 8 - kRecV : kRecMeta;
+  const int h1 = min(a.HKV, 2 * (blockIdx.y + 1) * a.per);
+  for (int h0 = 2 * blockIdx.y * a.per; h0 < h1; h0 += 2 * kPairs) {
+    uint4 x[kPairs][2];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {  // heads behind the last are read as the first, and dropped
+      const int h = h0 + 2 * j + sub;
+      const uint4* from = reinterpret_cast<const uint4*>(p + (h < h1 ? h : h0) * sh);
+      x[j][0] = __ldg(from);
+      x[j][1] = __ldg(from + 8);
+    }
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      if (h0 + 2 * j >= h1) break;
+      const int h = h0 + 2 * j + sub;
+      const uint32_t lo[4] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w}, hi[4] = {x[j][1].x, x[j][1].y, x[j][1].z, x[j][1].w};
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __byte_perm(lo[i], hi[i], 0x5410);
+        v[2 * i + 1] = __byte_perm(lo[i], hi[i], 0x7632);
+      }
+      quantise_row(v, rec + h * a.c_sh, meta, l, h < h1);
+    }
+  }
 }
 
 // Records back to rows: a half-warp per record, lane l the code words l (dims 4l.. and 64 + 4l..), kRecords in flight.
@@ -400,16 +450,23 @@ __global__ void __launch_bounds__(kRowThreads) unpack_kernel(const UnpackArgs a)
 }
 
 // ---------------------------------------------------------------- host side
+// What a launch over tokens and slots of a token needs: a warp takes as many slots (keeping the token's table entries)
+// as still leave 24 warps to each of 148 SMs.
+int plan_rows(RowArgs& a, int slots, const char* fn, dim3* grid) {
+  const int64_t tokens = (int64_t)a.B * a.T;
+  OA_REQUIRE(tokens <= 0x7fffffff, "%s: too many rows", fn);
+  a.slots = slots;
+  a.per = (int)std::min<int64_t>(slots, std::max<int64_t>(1, tokens * slots / (148 * 24)));
+  while ((slots + a.per - 1) / a.per > 65535) a.per *= 2;
+  *grid = dim3((unsigned)((tokens + kRowThreads / 32 - 1) / (kRowThreads / 32)), (slots + a.per - 1) / a.per);
+  return OA_OK;
+}
 template <typename E, bool CACHE, bool FULL>
 int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
-  a.slots = (CACHE ? a.HKV : (a.HKV + 1) / 2) + (a.HQ + 1) / 2;
-  const int64_t tokens = (int64_t)a.B * a.T;
-  if (tokens == 0 || a.slots == 0) return OA_OK;
-  OA_REQUIRE(tokens <= 0x7fffffff, "%s: too many rows", fn);
-  // a warp keeps a token's table entries for as many slots as still leave 24 warps to each of 148 SMs
-  a.per = (int)std::min<int64_t>(a.slots, std::max<int64_t>(1, tokens * a.slots / (148 * 24)));
-  while ((a.slots + a.per - 1) / a.per > 65535) a.per *= 2;
-  const dim3 grid((unsigned)((tokens + kRowThreads / 32 - 1) / (kRowThreads / 32)), (a.slots + a.per - 1) / a.per);
+  const int slots = (CACHE ? a.HKV : (a.HKV + 1) / 2) + (a.HQ + 1) / 2;
+  if (a.B == 0 || a.T == 0 || slots == 0) return OA_OK;
+  dim3 grid;
+  OA_TRY(plan_rows(a, slots, fn, &grid));
   if (a.per >= 4)
     rows_kernel<E, CACHE, FULL, 4><<<grid, kRowThreads, 0, st>>>(a);
   else
@@ -418,7 +475,17 @@ int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
 }
 template <typename E, bool CACHE>
 int launch_rows(RowArgs& a, const char* fn, cudaStream_t st) {
-  return a.cos == nullptr || a.R == kD ? launch_rows<E, CACHE, true>(a, fn, st) : launch_rows<E, CACHE, false>(a, fn, st);
+  return a.R == kD ? launch_rows<E, CACHE, true>(a, fn, st) : launch_rows<E, CACHE, false>(a, fn, st);
+}
+int launch_append(RowArgs& a, const char* fn, cudaStream_t st) {
+  if (a.B == 0 || a.T == 0 || a.HKV == 0) return OA_OK;
+  dim3 grid;
+  OA_TRY(plan_rows(a, (a.HKV + 1) / 2, fn, &grid));
+  if (a.per >= 4)
+    append_kernel<4><<<grid, kRowThreads, 0, st>>>(a);
+  else
+    append_kernel<1><<<grid, kRowThreads, 0, st>>>(a);
+  return oa_check_launch(fn);
 }
 
 // The parts of a block that oa_qk_norm_rope and oa_kv4_append share.
@@ -491,7 +558,8 @@ extern "C" int oa_kv4_append(const oa_kv4_append_args* args, void* stream) {
   OA_TRY(oa_take_index(fn, "lens", g.lens, B, false, &a.lens));
   a.offset = g.offset;
   a.B = (int)B; a.T = (int)T; a.HQ = (int)HQ; a.HKV = (int)HKV;
-  return oa::launch_rows<__nv_bfloat16, true>(a, fn, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a.cos ? oa::launch_rows<__nv_bfloat16, true>(a, fn, st) : oa::launch_append(a, fn, st);
 }
 
 extern "C" int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream) {
