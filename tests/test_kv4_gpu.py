@@ -504,3 +504,60 @@ def test_dense_calls_of_any_size_share_a_workspace():
             bb, h, t = i // (HQ * T), i // T % HQ, i % T
             m = max(0, int(lens[bb]) - T + 1 + t)
             P.check(a.cpu()[bb, h, t], *P.attend(q[bb, h, t], cache[bb, h // (HQ // HKV), :m], D ** -0.5))
+
+
+def test_append_long_odd_heads():
+    """A prompt long enough that a warp takes several heads of a token, an odd number of them."""
+    g = _gen(62)
+    B, T, hkv = 2, 2500, 7
+    x = _rows(g, B, T, 2 * hkv, D).transpose(1, 2)
+    k, v = x[:, :hkv], x[:, hkv:]
+    cache = torch.randint(0, 256, (B, hkv, T + 9, REC), generator=g).to(torch.uint8)
+    want = cache.clone()
+    want[:, :, 4:4 + T] = P.pack(k, v)
+    dev, y = cache.cuda(), x.cuda()
+    kv4.append(dev, y[:, :hkv], y[:, hkv:], torch.tensor([5], device="cuda"), offset=-1)
+    assert torch.equal(dev.cpu(), want)
+
+
+@pytest.mark.parametrize("R", [128, 80])
+def test_rope_append_long_odd_heads(R):
+    """As above for the rotation: one launch equals rotation and append, and both the definition."""
+    g = _gen(63)
+    B, T, HQ, HKV = 1, 1700, 9, 3
+    cos, sin = P.table(T + 3, R)
+    x = _rows(g, B, T, HQ + 2 * HKV, D)
+    y = x.cuda().transpose(1, 2)
+    q, k, v = y[:, :HQ], y[:, HQ:HQ + HKV], y[:, HQ + HKV:]
+    w = torch.randn(D, generator=g) + 1
+    start = torch.tensor([3], dtype=torch.int32, device="cuda")
+    one, two = kv4.new_cache(B, T + 3, "cuda", hkv=HKV), kv4.new_cache(B, T + 3, "cuda", hkv=HKV)
+    args = dict(q_weight=w.cuda(), k_weight=w.cuda())
+    q1 = kv4.rope_append(one, q, k, v, cos.cuda(), sin.cuda(), start, **args)
+    q2, k2 = rotary.qk_norm_rope(q, k, cos.cuda(), sin.cuda(), start, **args)
+    kv4.append(two, k2, v, start)
+    assert torch.equal(q1, q2) and torch.equal(one, two)
+    for got, h0, h1 in ((q2, 0, HQ), (k2, HQ, HQ + HKV)):
+        P.check(got, *P.rope(x.transpose(1, 2)[:, h0:h1], cos, sin, [3], [T], w))
+
+
+@pytest.mark.parametrize("B,HKV,lens", [
+    (310, 1, [700, 0, 3, 64, 1, 33, 250, 90, 5, 12]),   # more rows than CTAs, too uneven for a warp each: shares of a line
+    (16, 8, [5000, 1, 0, 33, 900, 64, 2, 400]),         # rows with CTAs to spare, too uneven to have their own
+    (40, 8, [1100, 1300, 1200])])                       # even ones on the line
+def test_dense_rows_that_share_ctas(B, HKV, lens):
+    g = _gen(64 + B)
+    lens = [lens[b % len(lens)] if b % 7 else lens[0] for b in range(B)]
+    cache = _records(g, B, HKV, max(lens))
+    q = _rows(g, B, HKV, 1, D)
+    got = kv4.decode_attention(q.cuda(), cache.cuda(), torch.tensor(lens, device="cuda"), out_dtype=torch.float32)
+    step = 1 if HKV == 1 else 5
+    want, slack = _dense_want(q[:, ::step], cache[:, ::step], lens, D ** -0.5)
+    P.check(got[:, ::step], want, slack)
+
+
+@pytest.mark.parametrize("BQ,n_exp", [(30, 1300), (60, 1300), (8, 2000), (100, 700)])
+def test_lists_of_few_rows(BQ, n_exp):
+    """Rows that clusters of 4, 2, 8 and no cluster share."""
+    x = _list_case(_gen(BQ + n_exp), BQ, 2, 900, 5, n_exp, 7, True)
+    P.check(kv4.flash_attention(*(t.cuda() for t in x), out_dtype=torch.float32), *_list_want(x, 7))
