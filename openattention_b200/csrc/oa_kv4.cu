@@ -60,11 +60,18 @@ __device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, 
 // A row that one CTA covers is written by it.  Otherwise each part leaves (m, l, O) in the workspace and the
 // last CTA to arrive (atomic ticket, no waiting) merges the parts in CTA order, so the result does not depend
 // on which CTA is last.
+// What bounds it: memory, once rows are long.  32 requests x 32768 tokens, 32 heads over 8: 190 us, 6.35 TB/s of records
+// (97% of a copy's rate), and 212-219 us in long runs, which the power limit slows.  The line reaches that where 256
+// rows with a CTA each take 207 us; the 8-column tile takes 222 us there.  Two query tokens (8 columns) are bound by
+// issue: 8 requests x 32768, 65-70 us, floor 46.  One request x 32768: 17 us, floor 6: a launch, the first loads and
+// the merge.  64 requests of 1 to 8191 tokens, two query tokens: 70 us, floor 38: what rows cost besides their tiles.
 constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kCols = 8;
-constexpr int kRowUnits = 20;  // what a row costs a CTA besides its tiles, in tiles (query, merge, idle pipeline)
+// What a row costs a CTA besides its tiles (query, merge, idle pipeline), in tiles.  64 ragged requests take 114, 83, 70,
+// 70 us with 6, 12, 20, 32.
+constexpr int kRowUnits = 20;
 constexpr int kLineUnits = kRowUnits + kWarps;  // what a CTA's second row costs it, in tiles
 constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
 constexpr int kRingBytes = kWarps * kStages * kTileBytes;
@@ -269,6 +276,7 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
   s.by_warp = w.cpr == 0 && most < (1 << 16) &&
               fmaxf(1.2f * work, 4.4f * rounds * (float)(most * grid)) + 10.f * (rounds - 2.f) * (float)grid < (float)total;
   if (s.by_warp) return true;
+  // (32 requests of 1000 tokens: 13.4 us with their own CTAs, 18.5 on the line; 16 of 32768: 110 and 101)
   s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * grid <= total + kLineUnits * grid;
   if (s.own) {
     const unsigned row = cta / w.cpr, j = cta - row * w.cpr;
@@ -568,7 +576,9 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
 // proxies are masked by a bit and not fetched.  A list belongs to one query row: one of the MMA's query columns is
 // used, which is still less work than unpacking codes to fp32 for plain FMAs (a tile of 32 takes some 350
 // instructions, against about 770 on the same pipes).  The warps' states are merged in shared memory, then over the
-// cluster.
+// cluster.  1024 rows of 231 entries and 64 proxies: 24.6 us for 63 MB.  Latency bounds that (a launch, indices, then records:
+// DRAM at 47%, issue at 41%); longer lists add 3.75 TB/s of records, which is 5 TB/s of DRAM accesses: a scattered record
+// of 144 bytes takes three or four of 64.
 constexpr int kRowsPerTile = 8;
 
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
@@ -799,6 +809,7 @@ extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream)
   w.cpr = (unsigned)(p.grid / p.rows);
   w.parts = static_cast<float*>(workspace);
   w.tickets = reinterpret_cast<unsigned*>(w.parts + (size_t)p.most_parts * oa::kPartFloats);
+  // up to four queries of a KV head fit the tile that holds each one's halves side by side (oa_kv4_mma.cuh)
   const auto kernel = HQ / HKV * T <= 4 ? &oa::dense_kernel<true> : &oa::dense_kernel<false>;
   const int rc = oa_smem_opt_in(reinterpret_cast<const void*>(kernel), oa::kRingBytes, fn, true);
   if (rc != OA_OK) return rc;

@@ -65,7 +65,8 @@ static inline int oa_take_rows(const char* fn, const char* name, const oa_tensor
   int64_t st[3];
   for (int i = 0; i < 3; ++i) {
     st[i] = t.size[i] > 1 ? t.stride[i] : 0;
-    OA_REQUIRE(!writes || empty || t.size[i] <= 1 || st[i] != 0, "%s: %s must not be an expanded tensor", fn, name);
+    OA_REQUIRE(!writes || empty || t.size[i] <= 1 || st[i] >= oa::kD || st[i] <= -oa::kD,
+               "%s: %s must not be an expanded tensor: its rows would overlap", fn, name);
     OA_REQUIRE(st[i] * esize % 16 == 0 || empty, "%s: %s rows must start on 16-byte boundaries (strides)", fn, name);
   }
   OA_REQUIRE(oa_aligned16(t.p), "%s: %s rows must start on 16-byte boundaries (base address)", fn, name);
@@ -99,7 +100,9 @@ static inline int oa_take_cache(const char* fn, const oa_tensor4& t, bool writes
   *sb = t.size[0] > 1 ? t.stride[0] : 0;
   *sh = t.size[1] > 1 ? t.stride[1] : 0;
   OA_REQUIRE(empty || (*sb % 16 == 0 && *sh % 16 == 0), "%s: cache strides must be multiples of 16 bytes", fn);
-  OA_REQUIRE(!writes || empty || ((t.size[0] <= 1 || *sb != 0) && (t.size[1] <= 1 || *sh != 0)),
+  const int64_t run = t.size[2] * oa::kRec;
+  OA_REQUIRE(!writes || empty ||
+                 ((t.size[0] <= 1 || *sb >= run || *sb <= -run) && (t.size[1] <= 1 || *sh >= run || *sh <= -run)),
              "%s: the cache must not be an expanded tensor: its requests would share records", fn);
   return OA_OK;
 }

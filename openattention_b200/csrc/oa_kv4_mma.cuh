@@ -24,7 +24,7 @@
 // accumulator's lanes the same way as in O^T = V^T (16 dims) x P (columns): running maxima and sums need no exchange,
 // only P turns (movmatrix).  The contraction's order is free, so a lane's operand words are its 16 contiguous bytes
 // of a K row and 8 bytes of a V row.  Rows of an MMA are assigned to tokens so that both loads touch every bank once
-// although records lie 36 words apart.  A tile costs about 370 instructions, of which 176 unpack codes.
+// although records lie 36 words apart.  176 of a tile's instructions unpack codes.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -94,7 +94,8 @@ __device__ __forceinline__ int row_token(int r) { return (r & 1) ? 8 + ((r + 3) 
 // QUAD: at most four columns.  The MMA's eight columns are each query's two halves, side by side in a lane, which
 // therefore serves one query: column 2c takes half 0 only (its q operand is zero in the other half's steps), 2c + 1
 // half 1, in scores and in weights.  Else eight columns, two queries to a lane, and the halves take sums and weights
-// of their own.
+// of their own.  (32 requests x 32768 tokens with four queries a KV head: 190 us, 222 with eight columns; 40 x 3000: 37.0
+// and 39.6; a tile takes 480 instructions, 600 with eight columns.)
 template <bool QUAD>
 struct WarpAttention {
   static constexpr int J = QUAD ? 1 : 2;  // columns (queries) of a lane

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .geometry import D, HKV
-from .rotary import _call, _CODE, _current_stream, _device_of, _index, _like, _no_grad, _rows, _same_device, _table, _weights
+from .rotary import _call, _CODE, _current_device, _current_stream, _device_of, _index, _like, _no_grad, _rows, _same_device, _table, _weights
 
 REC = 144
 
@@ -109,7 +109,11 @@ def attention_workspace(B, HQ, T, cache_len, dev, hkv=HKV):
 def _workspace(dev, *sizes):
     """The kept workspace of a GPU and stream, grown on demand: calls on one stream run in order and may share it.  A
     call that is being captured gets its own from the graph's pool, where its zero-fill is replayed too."""
-    capturing = torch.cuda.is_current_stream_capturing()
+    if dev == _current_device():
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(dev):
+            capturing = torch.cuda.is_current_stream_capturing()
     key = (dev, _current_stream(dev))
     kept = None if capturing else _ws_cache.get(key)
     if kept is not None and sizes in kept[1]:

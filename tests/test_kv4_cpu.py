@@ -87,6 +87,7 @@ ROPE = [
     (dict(q_out=_r(1, 4, 2, dtype=torch.float32)), "q_out must be torch.bfloat16"),
     (dict(q_out=_r(1, 4, 3)), "q_out must be"),
     (dict(q_out=_r(1, 1, 2).expand(1, 4, 2, D)), "expanded"),
+    (dict(q_out=_r(5 * 4 * 2).view(-1).as_strided((1, 4, 2, D), (2048, 256, 64, 1))), "overlap"),
     (dict(q=_r(1, 4, 2).requires_grad_()), "no backward pass"),
     (dict(k_weight=torch.zeros(D, requires_grad=True)), "no backward pass"),
     (dict(cos=torch.zeros(8, 128, requires_grad=True)), "no backward pass"),
@@ -104,6 +105,7 @@ def test_rope_refusals(entry, change, match):
     (dict(cache=torch.zeros(1, 2, 8, 160, dtype=torch.uint8)[..., :REC]), "contiguous records"),
     (dict(cache=_c(2, 8)), "cache must be"), (dict(cache=torch.zeros(1, 2, 8, 128, dtype=torch.uint8)), "cache must be"),
     (dict(cache=_c(1, 1, 8).expand(1, 2, 8, REC)), "expanded"), (dict(cache=_c(1, 3, 8)), "k must be"),
+    (dict(cache=_c(1, 2, 8).as_strided((1, 2, 8, REC), (2 * 8 * REC, 4 * REC, REC, 1))), "share records"),
     (dict(cache=torch.zeros(2 * 8 * REC + 8, dtype=torch.uint8)[8:].view(1, 2, 8, REC)), "16-byte"),
     (dict(v=_r(1, 2, 3)), "v must be"), (dict(start=_i(4)), "start must hold"), (dict(start=None), "start must be given"),
     (dict(lens=torch.zeros(1)), "lens must be")])
