@@ -22,7 +22,8 @@ import torch
 
 from . import _lib
 from .geometry import D, HKV
-from .rotary import _call, _CODE, _current_device, _current_stream, _device_of, _index, _like, _no_grad, _rows, _same_device, _table, _weights
+from .rotary import (_call, _CODE, _current_device, _current_stream, _device_of, _index, _like, _no_grad, _own_rows, _rows,
+                     _same_device, _table, _weights)
 
 REC = 144
 
@@ -65,9 +66,12 @@ def rope_append(cache, q, k, v, cos, sin, start, *, offset=0, lens=None, q_weigh
     zero = q_out is None
     if zero:
         q_out = _like(q)
+        fo = _own_rows(q_out, fq[1:5])
+    else:
+        fo = _rows("q_out", q_out, bf, dev)
     qp, kp, wd = _weights(q_weight, k_weight, bf, dev)
-    _call(dev, "oa_kv4_append", *fq, *_rows("k", k, bf, dev), *_rows("v", v, bf, dev), *_rows("q_out", q_out, bf, dev), *fc,
-          *_table(cos, sin, dev), *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, wd, zero, eps)
+    _call(dev, "oa_kv4_append", *fq, *_rows("k", k, bf, dev), *_rows("v", v, bf, dev), *fo, *fc, *_table(cos, sin, dev),
+          *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, wd, zero, eps)
     return q_out
 
 
@@ -76,21 +80,27 @@ def unpack(cache, start, T, *, offset=0, lens=None, out_dtype=torch.bfloat16, k_
     i < T.  Rows i >= lens[b] and positions outside the cache are zero in outputs that this call allocates and
     left as they were in k_out / v_out."""
     fc, dev = _cache(cache), cache.get_device()
-    shape = (*cache.shape[:2], T, D)
-    if k_out is not None or v_out is not None:
+    zk, zv = k_out is None, v_out is None
+    if not (zk and zv):
         _same_device(dev, k_out=k_out, v_out=v_out)
-        out_dtype = (v_out if k_out is None else k_out).dtype
+        out_dtype = (v_out if zk else k_out).dtype
     if T < 0 or out_dtype not in _CODE:
         raise RuntimeError(f"T must be >= 0 and the outputs bf16 or fp32, got {T}, {out_dtype}")
-    zk, zv = k_out is None, v_out is None
+    shape = (fc[1], fc[2], T, D)
     if zk:
-        k_out = torch.empty(shape, dtype=out_dtype, device=cache.device)
+        k_out = cache.new_empty(shape, dtype=out_dtype)
+        fk = _own_rows(k_out, shape)
+    else:
+        fk = _rows("k_out", k_out, out_dtype, dev)
+        if k_out.shape != shape:
+            raise RuntimeError(f"k_out must be {shape}, got {tuple(k_out.shape)}")
     if zv:
         v_out = _like(k_out)
-    if not zk and k_out.shape != shape:
-        raise RuntimeError(f"k_out must be {shape}, got {tuple(k_out.shape)}")
-    _call(dev, "oa_kv4_unpack", *fc, *_rows("k_out", k_out, out_dtype, dev), *_rows("v_out", v_out, out_dtype, dev),
-          *_index("start", start, dev), *_index("lens", lens, dev), offset, _CODE[out_dtype], zk, zv)
+        fv = _own_rows(v_out, shape)
+    else:
+        fv = _rows("v_out", v_out, out_dtype, dev)
+    _call(dev, "oa_kv4_unpack", *fc, *fk, *fv, *_index("start", start, dev), *_index("lens", lens, dev), offset,
+          _CODE[out_dtype], zk, zv)
     return k_out, v_out
 
 
@@ -145,19 +155,23 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
     side by side), so a decode loop that captures many layers passes one."""
     dev, fc = _device_of("q", q), _cache(cache)
     fq = _rows("q", q, torch.bfloat16, dev)
+    _same_device(dev, cache=cache, workspace=workspace, out=out)
+    dt = torch.bfloat16 if out_dtype is None else out_dtype
+    if out is not None and out_dtype is None:
+        dt = out.dtype
+    if dt not in _CODE or (out is not None and dt != out.dtype):
+        raise RuntimeError(f"the output must be bf16 or fp32 and out of type out_dtype, got {dt}"
+                           f"{'' if out is None else f' and out {out.dtype}'}")
     if out is None:
-        out = _like(q) if out_dtype is None else torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    elif not isinstance(out, torch.Tensor):
-        raise RuntimeError("out must be a CUDA tensor")
-    _same_device(dev, cache=cache, workspace=workspace)
-    dt = out.dtype
-    if dt not in _CODE or (out_dtype is not None and out_dtype != dt):
-        raise RuntimeError(f"the output must be bf16 or fp32 and out of type out_dtype, got {dt}, out_dtype {out_dtype}")
+        out = _like(q) if out_dtype is None else q.new_empty(fq[1:5], dtype=dt)
+        fo = _own_rows(out, fq[1:5])
+    else:
+        fo = _rows("out", out, dt, dev)
     if workspace is None:
         workspace = _workspace(dev, *fq[1:3], fc[2], fq[3], fc[3])
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise RuntimeError("workspace must be a contiguous uint8 tensor")
-    _call(dev, "oa_kv4_attention", *fq, *fc, *_rows("out", out, dt, dev), *_index("n", n, dev), workspace.data_ptr(),
+    _call(dev, "oa_kv4_attention", *fq, *fc, *fo, *_index("n", n, dev), workspace.data_ptr(),
           workspace.numel(), offset, _CODE[dt], D ** -0.5 if sm_scale is None else sm_scale)
     return out
 

@@ -69,13 +69,25 @@ def _index(name, t, dev):
     return t.data_ptr(), t.shape[0], t.stride(0), t.dtype is torch.int64
 
 
-def _table(cos, sin, dev):
+def _bad_table(cos, sin, dev):
     for name, t in (("cos", cos), ("sin", sin)):
         if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != dev or t.dim() != 2 or \
                 not t.is_contiguous() or (t is not cos and t.shape != cos.shape):
             raise RuntimeError(f"{name} must be a contiguous fp32 (positions, rotated dims) table on cuda:{dev}, the "
                                "same shape for both")
         _no_grad(name, t)
+
+
+def _table(cos, sin, dev):
+    try:
+        shape = cos.shape
+        if sin.shape == shape and cos.dtype is sin.dtype is torch.float32 and cos.get_device() == sin.get_device() == dev and \
+                cos.is_contiguous() and sin.is_contiguous() and not (cos.requires_grad or sin.requires_grad):
+            rows, width = shape
+            return cos.data_ptr(), sin.data_ptr(), rows, width
+    except (AttributeError, ValueError):
+        pass
+    _bad_table(cos, sin, dev)
     return cos.data_ptr(), sin.data_ptr(), *cos.shape
 
 
@@ -94,6 +106,12 @@ def _weights(q_weight, k_weight, dtype, dev):
 
 def _like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _own_rows(t, sizes):
+    """_rows of a contiguous tensor that the call itself allocated; sizes: (B, heads, T, 128)."""
+    _, H, T, _ = sizes
+    return t.data_ptr(), *sizes, H * T * D, T * D, D, 1
 
 
 _entries: dict = {}
@@ -134,10 +152,15 @@ def qk_norm_rope(q, k, cos, sin, start, *, offset=0, lens=None, q_weight=None, k
     zq, zk = q_out is None, k_out is None
     if zq:
         q_out = _like(q)
+        fqo = _own_rows(q_out, fq[1:5])
+    else:
+        fqo = _rows("q_out", q_out, dt, dev)
     if zk:
         k_out = _like(k)
+        fko = _own_rows(k_out, fk[1:5])
+    else:
+        fko = _rows("k_out", k_out, dt, dev)
     qp, kp, wd = _weights(q_weight, k_weight, dt, dev)
-    _call(dev, "oa_qk_norm_rope", *fq, *fk, *_rows("q_out", q_out, dt, dev), *_rows("k_out", k_out, dt, dev),
-          *_table(cos, sin, dev), *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, _CODE[dt], wd,
+    _call(dev, "oa_qk_norm_rope", *fq, *fk, *fqo, *fko, *_table(cos, sin, dev), *_index("start", start, dev), *_index("lens", lens, dev), qp, kp, offset, _CODE[dt], wd,
           zq, zk, eps)
     return q_out, k_out
