@@ -561,3 +561,58 @@ def test_lists_of_few_rows(BQ, n_exp):
     """Rows that clusters of 4, 2, 8 and no cluster share."""
     x = _list_case(_gen(BQ + n_exp), BQ, 2, 900, 5, n_exp, 7, True)
     P.check(kv4.flash_attention(*(t.cuda() for t in x), out_dtype=torch.float32), *_list_want(x, 7))
+
+
+@pytest.mark.parametrize("B,HQ,HKV,T,lens", [
+    (3, 4, 2, 2, [1, 33, 700]), (2, 2, 2, 3, [2, 65]), (1, 8, 2, 1, [5]), (4, 3, 3, 4, [4, 3, 0, 40]),
+    (600, 1, 1, 4, [50, 3, 0, 64, 33, 1, 2, 17, 96])])
+def test_dense_few_columns_of_several_tokens(B, HQ, HKV, T, lens):
+    """At most four columns a KV head, from heads and query tokens; the last with a warp to a row."""
+    g = _gen(65 + B)
+    lens = [lens[b % len(lens)] for b in range(B)]
+    cache = _records(g, B, HKV, max(lens))
+    for b, n in enumerate(lens):
+        cache[b, :, n:] = 255
+    q = _rows(g, B, HQ, T, D)
+    got = kv4.decode_attention(q.cuda(), cache.cuda(), torch.tensor(lens, device="cuda"), out_dtype=torch.float32)
+    P.check(got, *_dense_want(q, cache, lens, D ** -0.5))
+
+
+def test_prompt_write_read_and_lists_in_a_graph():
+    """Rotation, cache write, read-back and list attention captured before any of them ran eagerly on these tensors, and
+    replayed with new inputs and positions, twice over one graph's outputs."""
+    g = _gen(66)
+    B, HQ, HKV, T, Lmax = 2, 8, 2, 21, 64
+    cos, sin = (t.cuda() for t in P.table(Lmax, 128))
+    x = torch.zeros(B, T, HQ + 2 * HKV, D, dtype=BF, device="cuda")
+    start = torch.zeros(B, dtype=torch.int32, device="cuda")
+    sel = torch.full((B * HQ, 5), -1, dtype=torch.int32, device="cuda")
+    exp = torch.full((B * HQ, 40), -1, dtype=torch.int32, device="cuda")
+    kb, vb, ln = (torch.zeros(B * HQ, 6, D, dtype=BF, device="cuda"), torch.zeros(B * HQ, 6, D, dtype=BF, device="cuda"),
+                  torch.zeros(B * HQ, 6, device="cuda"))
+    cache = kv4.new_cache(B, Lmax, "cuda", hkv=HKV)
+
+    def run(cache):
+        y = x.transpose(1, 2)
+        q, k = rotary.qk_norm_rope(y[:, :HQ], y[:, HQ:HQ + HKV], cos, sin, start)
+        kv4.append(cache, k, y[:, HQ + HKV:], start)
+        k2, v2 = kv4.unpack(cache, start, T)
+        o = kv4.flash_attention(q[:, :, -1].reshape(B * HQ, D), cache.view(B * HKV, Lmax, REC), sel, exp, kb, vb, ln)
+        return q, k2, v2, o
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(cache)
+    other = kv4.new_cache(B, Lmax, "cuda", hkv=HKV)
+    for i in range(3):
+        x.copy_(_rows(g, B, T, HQ + 2 * HKV, D))
+        start.copy_(torch.tensor([3 * i, 40 - i]))
+        sel.copy_(torch.randint(-1, Lmax, sel.shape, generator=g))
+        exp.copy_(torch.randint(-1, Lmax, exp.shape, generator=g))
+        kb.copy_(_rows(g, B * HQ, 6, D))
+        vb.copy_(_rows(g, B * HQ, 6, D))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(other)
+        assert torch.equal(cache, other) and all(torch.equal(a, b) for a, b in zip(outs, want))
