@@ -155,7 +155,8 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
     side by side), so a decode loop that captures many layers passes one."""
     dev, fc = _device_of("q", q), _cache(cache)
     fq = _rows("q", q, torch.bfloat16, dev)
-    _same_device(dev, cache=cache, workspace=workspace, out=out)
+    if cache.get_device() != dev or workspace is not None or out is not None:
+        _same_device(dev, cache=cache, workspace=workspace, out=out)
     dt = torch.bfloat16 if out_dtype is None else out_dtype
     if out is not None and out_dtype is None:
         dt = out.dtype
@@ -179,6 +180,13 @@ def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, ou
 _NO_PROXIES, _NO_LOG = (0,) * 14, (0,) * 5
 
 
+def _list(t, dev):
+    """The block's fields of an index list; None: not one on GPU `dev`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != dev:
+        return None
+    return t.data_ptr(), *t.shape, *t.stride()
+
+
 def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, sm_scale=None, out_dtype=None,
                     out=None):
     """flash.ours_flash / flash.decode_expand_attention over a 4-bit cache: q (BQ, 128) bf16, cache (BH, Lmax, 144)
@@ -193,27 +201,30 @@ def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, s
         raise RuntimeError("q must be a (rows, 128) bf16 CUDA tensor")
     _no_grad("q", q)
     fc, dev = _cache(cache, ndim=3), q.get_device()
-    _same_device(dev, cache=cache, sel_idx=sel_idx, exp_idx=exp_idx, out=out)
-    if sel_idx.dtype is not torch.int32 or sel_idx.dim() != 2 or exp_idx.dtype is not torch.int32 or exp_idx.dim() != 2:
-        raise RuntimeError(f"sel_idx and exp_idx must be (rows, n) int32 tensors, got {tuple(sel_idx.shape)} {sel_idx.dtype} "
-                           f"and {tuple(exp_idx.shape)} {exp_idx.dtype}")
+    fs, fe = _list(sel_idx, dev), _list(exp_idx, dev)
+    if fs is None or fe is None or cache.get_device() != dev or out is not None:
+        _same_device(dev, cache=cache, sel_idx=sel_idx, exp_idx=exp_idx, out=out)
+    if fs is None or fe is None:
+        got = " and ".join(f"{tuple(t.shape)} {t.dtype}" if isinstance(t, torch.Tensor) else type(t).__name__
+                           for t in (sel_idx, exp_idx))
+        raise RuntimeError(f"sel_idx and exp_idx must be (rows, n) int32 tensors, got {got}")
     NB = (0 if kbar is None else kbar.shape[1]) if nb is None else int(nb)
     fb, fl = _NO_PROXIES, _NO_LOG
     if NB > 0:
-        _same_device(dev, kbar=kbar, vbar=vbar, log_n=log_n)
         if kbar is None or vbar is None or log_n is None or kbar.dtype is not torch.bfloat16 or kbar.dim() != 3 or \
                 vbar.dtype is not torch.bfloat16 or vbar.dim() != 3 or log_n.dtype is not torch.float32 or log_n.dim() != 2:
             raise RuntimeError("kbar and vbar must be (rows, NB, 128) bf16 and log_n (rows, NB) fp32")
+        if not kbar.get_device() == vbar.get_device() == log_n.get_device() == dev:
+            _same_device(dev, kbar=kbar, vbar=vbar, log_n=log_n)
         for name, t in (("kbar", kbar), ("vbar", vbar), ("log_n", log_n)):
             _no_grad(name, t)
         fb = (kbar.data_ptr(), *kbar.shape, *kbar.stride(), vbar.data_ptr(), *vbar.shape, *vbar.stride())
         fl = (log_n.data_ptr(), *log_n.shape, *log_n.stride())
     if out is None:
-        out = _like(q) if out_dtype is None else torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        out = _like(q) if out_dtype is None else q.new_empty(q.shape, dtype=out_dtype)
     dt = out.dtype
     if dt not in _CODE or out.dim() != 2 or (out_dtype is not None and out_dtype != dt):
         raise RuntimeError(f"out must be (rows, 128) bf16 or fp32 of type out_dtype, got {tuple(out.shape)} {dt}")
-    _call(dev, "oa_kv4_flash", q.data_ptr(), *q.shape, *q.stride(), *fc, sel_idx.data_ptr(), *sel_idx.shape,
-          *sel_idx.stride(), exp_idx.data_ptr(), *exp_idx.shape, *exp_idx.stride(), *fb, *fl, out.data_ptr(), *out.shape,
-          *out.stride(), _CODE[dt], NB, D ** -0.5 if sm_scale is None else sm_scale)
+    _call(dev, "oa_kv4_flash", q.data_ptr(), *q.shape, *q.stride(), *fc, *fs, *fe, *fb, *fl, out.data_ptr(),
+          *out.shape, *out.stride(), _CODE[dt], NB, D ** -0.5 if sm_scale is None else sm_scale)
     return out

@@ -150,7 +150,7 @@ def test_decode_attention_refusals(entry, change, match):
 @pytest.mark.parametrize("change,match", [
     (dict(q=_r(4, dtype=torch.float32)), "q must be"), (dict(q=torch.zeros(4, 64, dtype=BF)), r"\(4, 128\)"),
     (dict(cache=_c(3, 8)), "multiple of the cache's"), (dict(cache=_c(1, 2, 8)), "cache must be"),
-    (dict(sel_idx=torch.zeros(4, 2, dtype=torch.int64)), "sel_idx"), (dict(exp_idx=torch.zeros(3, 2, dtype=torch.int32)), "exp_idx"),
+    (dict(sel_idx=torch.zeros(4, 2, dtype=torch.int64)), "sel_idx"), (dict(exp_idx=None), "exp_idx"), (dict(exp_idx=torch.zeros(3, 2, dtype=torch.int32)), "exp_idx"),
     (dict(exp_idx=torch.zeros(4, 4, dtype=torch.int32)[:, ::2]), "contiguous"),
     (dict(nb=9), "kbar and vbar must be"), (dict(nb=-1), "bad list sizes"), (dict(vbar=_r(4, 5)), "kbar and vbar"),
     (dict(kbar=_r(3, 6), vbar=_r(3, 6)), "kbar and vbar must be"), (dict(kbar=None, nb=2), "kbar must be|kbar and vbar"),
