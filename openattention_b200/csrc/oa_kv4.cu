@@ -69,10 +69,11 @@ constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
 constexpr int kCols = 8;
-// What a row costs a CTA besides its tiles (query, merge, idle pipeline), in tiles.  64 ragged requests take 114, 83, 70,
-// 70 us with 6, 12, 20, 32.
-constexpr int kRowUnits = 20;
-constexpr int kLineUnits = kRowUnits + kWarps;  // what a CTA's second row costs it, in tiles
+// What a row costs a CTA besides its tiles (query, merge, idle pipeline), in tiles of four columns and of eight.  64
+// ragged requests with two query tokens take 114, 83, 70 us with 6, 12, 20; over 24 uneven batches 20 to 23 are best for
+// four columns, 27 for eight (2% quicker than 20).
+constexpr int kRowUnits4 = 20, kRowUnits8 = 27;
+constexpr int kLineUnits = 35;  // what a second row costs a CTA of the line, in tiles
 constexpr int kPartFloats = kCols * kD + 2 * kCols;  // one part: O of 8 columns, then their (m, l)
 constexpr int kRingBytes = kWarps * kStages * kTileBytes;
 
@@ -225,6 +226,7 @@ __device__ __forceinline__ unsigned cta_begin(const DenseShare& s, unsigned cta)
 }
 
 // False: nothing for this CTA.  Every thread of the CTA finds the same.
+template <int kRowUnits>
 __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
   __shared__ unsigned s_pre[kDenseThreads];  // units of a row of each request before thread i's requests
   __shared__ unsigned s_sum[kWarps];
@@ -276,7 +278,8 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
   s.by_warp = w.cpr == 0 && most < (1 << 16) &&
               fmaxf(1.2f * work, 4.4f * rounds * (float)(most * grid)) + 10.f * (rounds - 2.f) * (float)grid < (float)total;
   if (s.by_warp) return true;
-  // (32 requests of 1000 tokens: 13.4 us with their own CTAs, 18.5 on the line; 16 of 32768: 110 and 101)
+  // (32 requests of 1000 tokens: 13.4 us with their own CTAs, 18.5 on the line; 24 of 2000: 20.5 and 23.4; 16 of 32768:
+  // 110 and 101)
   s.own = w.cpr >= 1 && (kRowUnits + (most + w.cpr - 1) / w.cpr) * grid <= total + kLineUnits * grid;
   if (s.own) {
     const unsigned row = cta / w.cpr, j = cta - row * w.cpr;
@@ -330,6 +333,7 @@ __device__ __forceinline__ bool dense_share(const DenseArgs& a, const DenseWork&
 }
 
 // The next row on the line, if any of its tiles are this CTA's.
+template <int kRowUnits>
 __device__ __forceinline__ bool dense_next(const DenseArgs& a, const DenseWork& w, DenseShare& s) {
   const int step = s.tiles + kRowUnits - s.off;
   s.line += step;
@@ -425,6 +429,7 @@ __device__ __forceinline__ void dense_by_warp(const DenseArgs& a, const DenseWor
 template <bool QUAD>
 __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs a, const DenseWork w) {
   extern __shared__ __align__(16) unsigned char s_ring[];
+  constexpr int kRowUnits = QUAD ? kRowUnits4 : kRowUnits8;
   __shared__ unsigned s_last;
   __shared__ DenseShare s;  // the same for all threads: kept here, out of the loop's registers
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -432,7 +437,7 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
   const unsigned cta = blockIdx.x;
   {
     DenseShare mine;
-    if (!dense_share(a, w, mine)) return;
+    if (!dense_share<kRowUnits>(a, w, mine)) return;
     if (mine.by_warp) {
       dense_by_warp<QUAD>(a, w, smem_u32(s_ring) + warp * (kStages * kTileBytes));
       return;
@@ -562,7 +567,7 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
     }
     if (s.own) return;
     __syncthreads();
-    if (tid == 0) s_last = dense_next(a, w, s) ? 1u : 0u;
+    if (tid == 0) s_last = dense_next<kRowUnits>(a, w, s) ? 1u : 0u;
     __syncthreads();  // s_part is the ring again
     if (!s_last) return;
   }
@@ -796,7 +801,7 @@ extern "C" int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream)
   const size_t workspace_bytes = (size_t)std::max<int64_t>(g.workspace_bytes, 0);
   const oa::DensePlan p = oa::dense_plan(B, HQ, HKV, T, Lmax);
   // units on the line (and 9 of them per row of the grid's widest product) are counted in 32 bits
-  const int64_t most_units = p.rows * ((Lmax + oa::kTile - 1) / oa::kTile + 1 + oa::kRowUnits);
+  const int64_t most_units = p.rows * ((Lmax + oa::kTile - 1) / oa::kTile + 1 + oa::kRowUnits8);
   OA_REQUIRE(most_units <= 0xffffffffll / 9 && most_units / std::max<int64_t>(p.rows, 1) * 8 * p.grid <= 0xffffffffll,
              "%s: too many records (B * HKV * Lmax) for one call", fn);
   const size_t need = oa::workspace_bytes(p);
