@@ -64,7 +64,7 @@ __device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, 
 // (97% of a copy's rate), and 212-219 us in long runs, which the power limit slows.  The line reaches that where 256
 // rows with a CTA each take 207 us; the 8-column tile takes 222 us there.  Two query tokens (8 columns) are bound by
 // issue: 8 requests x 32768, 65-70 us, floor 46.  One request x 32768: 17 us, floor 6: a launch, the first loads and
-// the merge.  64 requests of 1 to 8191 tokens, two query tokens: 70 us, floor 38: what rows cost besides their tiles.
+// the merge.  64 requests of 1 to 8191 tokens, two query tokens: 66 us, floor 38: what rows cost besides their tiles.
 constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
