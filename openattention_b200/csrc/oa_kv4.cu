@@ -166,7 +166,6 @@ __device__ __forceinline__ void merge_parts(const float* src, int parts, int nco
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    M = biased(M);
     for (int v = lane; v < parts; v += 32) {
       const float f = ex2(s_f[v * kCols + warp] - M);
       L = fmaf(f, __ldcg(at(v) + kCols * kD + 2 * warp + 1), L);
@@ -531,11 +530,10 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
         f[v] = s_part[v * kPartFloats + kCols * kD + 2 * warp];
         M = fmaxf(M, f[v]);
       }
-      const float base_m = biased(M);
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int v = 0; v < kWarps; ++v) {
-        const float e = ex2(f[v] - base_m);
+        const float e = ex2(f[v] - M);
         L = fmaf(e, s_part[v * kPartFloats + kCols * kD + 2 * warp + 1], L);
         axpy(A, e, reinterpret_cast<const float4*>(s_part + v * kPartFloats)[32 * warp + lane]);
       }
@@ -708,7 +706,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
   for (int i = 0; i < W; ++i) M = fmaxf(M, st[i * kNext + kD]);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    f[i] = ex2(st[i * kNext + kD] - biased(M));
+    f[i] = ex2(st[i * kNext + kD] - M);
     L = fmaf(f[i], st[i * kNext + kD + 1], L);
   }
   for (int d = tid; d < kD; d += 32 * W) {
@@ -731,11 +729,11 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
     for (int k = 0; k < S; ++k) M = fmaxf(M, ld_cluster(cluster_addr(s_cta + kD, k)));
     L = 0.f;
     for (int k = 0; k < S; ++k)
-      L = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - biased(M)), ld_cluster(cluster_addr(s_cta + kD + 1, k)), L);
+      L = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - M), ld_cluster(cluster_addr(s_cta + kD + 1, k)), L);
     for (int d = tid; d < kD; d += 32 * W) {
       float A = 0.f;
       for (int k = 0; k < S; ++k)
-        A = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - biased(M)), ld_cluster(cluster_addr(s_cta + d, k)), A);
+        A = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - M), ld_cluster(cluster_addr(s_cta + d, k)), A);
       store_list(a, r, d, A, L);
     }
   }

@@ -12,8 +12,11 @@
 // largest.  (e4m3 operands would hold a code in a byte, but mma.sync takes them apart into fp16 here: slower.)
 //
 // Values.  The scale goes into the weight: o = sum_t (p_t s_t) c_t + sum_t p_t z_t, the second sum in fp32 outside the
-// tensor cores.  p s is scaled by a power of two per half, chosen so that the largest scale seen gives [2^6, 2^7): it
-// is rounded to fp16 (11 bits) over 20 octaves below the largest, beneath them it is off by 2^-32 of the largest.
+// tensor cores.  p s is scaled by a power of two r per column and half and rounded to fp16: 11 bits over 20 octaves below
+// the largest p s seen, beneath them off by 2^-31 of that.  r is chosen from weight times scale, not from the scale alone:
+// a record of huge scale and no weight (or whose weight the running maximum took away later) must not push what the
+// others give beneath fp16.  Running maxima are whole numbers (of log2 units, rounded up), so that weights, sums
+// and r move by exact powers of two and what a larger maximum takes from the weights r can give back.
 //
 // Tensor cores truncate their running sums.  Codes are all positive, so sums of p s c would grow with the context
 // and with them the truncation, while the offsets' part cancels most of them (1.1e-2 of the result was seen at
@@ -34,8 +37,13 @@ namespace oa {
 
 constexpr int kTile = 32;                   // records per tile
 constexpr int kTileBytes = kTile * kRec;
-constexpr float kSlack = 8.f;  // log2
-constexpr int kTop = 7;        // scales times r stay at most 2^kTop, weights at most 2^(kTop + kSlack) < fp16's 65504
+constexpr float kSlack = 5.f;        // log2
+constexpr int kTop = 7;              // p s r stays under 2^kTop where r is chosen
+constexpr float kCap = 32768.f;      // p s r above it (fp16 ends at 65504) has r chosen anew
+constexpr uint32_t kWide = 0x4480u;  // 2^10 = kCap / 2^kSlack in bf16
+// Where nothing was seen: under every score, and finite, so that its difference from itself is 0 and from -inf is -inf.
+constexpr float kNoMax = -3.402823466e38f;
+constexpr int kRowTop = 60;      // log2 of the largest r beside bf16 rows
 constexpr uint32_t kLoMask = 0x000f000fu, kHiMask = 0x00f000f0u;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -73,8 +81,22 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, results under 2^-126 ar
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float lg2(float x) {  // log2, of a subnormal too
+  float r;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {  // the number, of a number and a NaN
+  uint32_t v;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+  return v;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t v;
+  asm("mul.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(a), "r"(b));
+  return v;
+}
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-__device__ __forceinline__ float biased(float m) { return m == -INFINITY ? 0.f : m; }
 
 // shared-space loads
 __device__ __forceinline__ uint4 lds128(uint32_t at, int imm) {
@@ -103,9 +125,9 @@ struct WarpAttention {
   float scale[J];           // per column: sm_scale log2(e) 2^(24 - exponent of q)
   float qs[J][2];           // sm_scale log2(e) times the sum of q over each half
   float acc[8][4];          // O^T: half h, tile i -> acc[4 h + i], QUAD: MMA column h of the lane's two counts
-  float m[J], bm[J], l[J];  // running maximum (log2 units; bm: 0 while it is -inf), this lane's share of the sum
+  float m[J], l[J];         // running maximum (log2 units; kNoMax: none yet), this lane's share of the sum
   float zs[J][2];           // this lane's share of sum p z, per half
-  float r[2], cap[2];       // power-of-two factor of p s per half, and the largest scale it holds
+  uint32_t r2[J];           // power-of-two factor of p s per column: bf16 of half 0 | of half 1 << 16
   uint32_t at_k, at_m, at_v0, at_v1;  // this lane's addresses in a tile
 
   static __device__ __forceinline__ int lane() { return threadIdx.x & 31; }
@@ -174,57 +196,46 @@ struct WarpAttention {
       scale[j] = __shfl_sync(0xffffffffu, sc, src);
       qs[j][0] = __shfl_sync(0xffffffffu, s[0], src) * qk_scale;
       qs[j][1] = __shfl_sync(0xffffffffu, s[1], src) * qk_scale;
-      m[j] = -INFINITY;
-      bm[j] = l[j] = zs[j][0] = zs[j][1] = 0.f;
+      m[j] = kNoMax;
+      l[j] = zs[j][0] = zs[j][1] = 0.f;
+      r2[j] = 0x7e807e80u;  // 2^126
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      r[h] = pow2i(126);
-      cap[h] = pow2i(kTop - 126);
-    }
   }
 
-  // A scale above the cap: choose the factor anew for the largest scale of this tile.
-  __device__ __forceinline__ void raise_cap(float s, int h) {
+  __device__ __forceinline__ float r(int j, int h) const { return h ? bf_hi(r2[j]) : bf_lo(r2[j]); }
+  // The largest of a column's lanes.
+  static __device__ __forceinline__ float column_max(float x) {
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
-    if (!(s > cap[h])) return;
-    const int es = max(kTop - 127, (__float_as_int(s) >> 23) - 127);
-    const float next = pow2i(kTop - 1 - es);
-    // next / r as a power of two; one under 2^-126 drops what is there, which is that much smaller
-    const int d = (__float_as_int(next) >> 23) - (__float_as_int(r[h]) >> 23);
-    scale_half(h, d < -126 ? 0.f : pow2i(d));
-    r[h] = next;
-    cap[h] = pow2i(kTop) / next;
+    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
   }
-  __device__ __forceinline__ void scale_half(int h, float f) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (!QUAD || (j & 1) == h) acc[4 * h + i][j] *= f;
-  }
-  // A score above the running maximum of column j: new maximum, and everything of the column scaled to it.  mx: the
-  // lane's largest.
-  __device__ __forceinline__ void raise_max(float mx, int j) {
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float nm = fmaxf(m[j], mx);
-    const float al = ex2(m[j] - biased(nm));
+  // Column j's running maximum takes in mx (the lane's largest score): by how many octaves its weights fall.  Sums of
+  // weights follow; the accumulators' part is set_factor's.
+  __device__ __forceinline__ int raise_max(float mx, int j) {
+    const float nm = fmaxf(m[j], ceilf(column_max(mx)));
+    const int d = nm > m[j] ? (int)fminf(nm - m[j], 300.f) : 0;
+    const float al = d > 126 ? 0.f : pow2i(-d);
     m[j] = nm;
-    bm[j] = biased(nm);
     l[j] *= al;
     zs[j][0] *= al;
     zs[j][1] *= al;
+    return d;
+  }
+  // Column j, half h: its factor becomes 2^e (e <= 126) after weights fell by d octaves, but rises by no more than d:
+  // what is in the accumulators never grows.
+  __device__ __forceinline__ void set_factor(int j, int h, int e, int d) {
+    const int now = (int)(h ? r2[j] >> 23 : r2[j] >> 7 & 0xffu) - 127 + d, to = min(now, max(-126, e));
+    const float f = to - now < -126 ? 0.f : pow2i(to - now);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (QUAD || (k & 1) == j) acc[i][k] *= al;
+        if ((k & 1) == (QUAD ? h : j)) acc[4 * h + i][k] *= f;
+    r2[j] = __byte_perm(r2[j], (to + 127) << 7, h ? 0x5410 : 0x3254);
   }
 
   // One tile of 32 records at shared address `sm`.  MASK: the lane's column j sees only the tokens whose bit is set in
@@ -267,25 +278,51 @@ struct WarpAttention {
           x[b][k][j] = v;
         }
     }
-    // m is the same in all lanes of a column and nothing moves until some lane sees a score kSlack above it (or
-    // a scale above the cap): weights up to 2^kSlack are as good as weights up to 1, and new maxima are common
-    float mx[J], s[2];
+    // m is the same in all lanes of a column and nothing moves until some lane sees a score kSlack above it (weights
+    // up to 2^kSlack are as good as weights up to 1, and new maxima are common) or a weight that fp16 may not hold.
+    // That takes a scale above kCap / 2^kSlack / r; where there is one, the lane's largest weight times its largest
+    // scale is a closer bound.
+    float mx[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) mx[j] = fmaxf(fmaxf(x[0][0][j], x[0][1][j]), fmaxf(x[1][0][j], x[1][1][j]));
+    uint32_t s2 = 0u;  // the lane's largest scales, one bf16 for each half
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s[h] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool used = !MASK || ((in[0] | in[J - 1]) >> (16 * (i >> 1) + (i & 1)) & 1u);
-        s[h] = fmaxf(s[h], used ? bf_lo(vm[i >> 1][i & 1][h]) : 0.f);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const bool used = !MASK || ((in[0] | in[J - 1]) >> (16 * (i >> 1) + (i & 1)) & 1u);
+      const uint32_t v = __byte_perm(vm[i >> 1][i & 1][0], vm[i >> 1][i & 1][1], 0x5410);
+      s2 = max_bf16x2(s2, used ? v : 0u);
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[J - 1] > m[J - 1] + kSlack || s[0] > cap[0] || s[1] > cap[1])) {
+    const uint32_t sr = mul_bf16x2(s2, J == 1 ? r2[0] : max_bf16x2(r2[0], r2[J - 1]));
+    bool above = false;
 #pragma unroll
-      for (int j = 0; j < J; ++j) raise_max(mx[j], j);
-      raise_cap(s[0], 0);
-      raise_cap(s[1], 1);
+    for (int j = 0; j < J; ++j) above = above || mx[j] > m[j] + kSlack;
+    if (__any_sync(0xffffffffu, above || sr >= kWide << 16 || sr << 16 >= kWide << 16)) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const float e = ex2(mx[j] - m[j]);
+        above = above || fmaxf(e * bf_lo(s2) * r(j, 0), e * bf_hi(s2) * r(j, 1)) > kCap;
+      }
+      if (__any_sync(0xffffffffu, above)) {
+        float lg[2][4];  // log2 of the scales
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lg[h][i] = lg2(bf_lo(vm[i >> 1][i & 1][h]));
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          float top[2];  // log2 of the tile's largest p s; -inf where the column does not see, a NaN drops
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            top[h] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[h] = fmaxf(top[h], x[i >> 1][i & 1][j] + lg[h][i]);
+            top[h] = column_max(top[h]);
+          }
+          const int d = raise_max(mx[j], j);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) set_factor(j, h, kTop - 1 - max(kTop - 1 - 126, __float2int_rd(top[h] - m[j])), d);
+        }
+      }
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -296,18 +333,18 @@ struct WarpAttention {
         float p[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          p[j] = ex2(x[b][k][j] - bm[j]);
+          p[j] = ex2(x[b][k][j] - m[j]);
           l[j] += p[j];
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           // second tokens enter as -s (15 - c) + (z + 15 s)
-          const float s1 = bf_lo(vm[b][k][h]), sv = s1 * (k ? -r[h] : r[h]);
+          const float s1 = bf_lo(vm[b][k][h]);
           const float zv = k ? fmaf(15.f, s1, bf_hi(vm[b][k][h])) : bf_hi(vm[b][k][h]);
 #pragma unroll
           for (int j = 0; j < J; ++j) {
             const bool seen = !MASK || (in[j] >> (16 * b + k) & 1u);
-            w[h][j] = seen ? p[j] * sv : 0.f;
+            w[h][j] = seen ? p[j] * s1 * (k ? -r(j, h) : r(j, h)) : 0.f;  // in this order: s r may pass fp32
             if (MASK)
               zs[j][h] += seen ? p[j] * zv : 0.f;
             else
@@ -353,21 +390,17 @@ struct WarpAttention {
     const float m0 = __shfl_sync(0xffffffffu, m[0], lane() & 28);
     if (t != 0) {
       m[0] = m0;
-      bm[0] = biased(m0);
       l[0] = zs[0][0] = zs[0][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
     }
-    // scales of records may have left a factor that would carry a large row past fp32
+    // one factor for a row's two terms; scales of records may have left one that would carry a large row past fp32
+    r2[0] = __shfl_sync(0xffffffffu, r2[0], lane() & 28);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      if (r[h] > pow2i(60)) {
-        scale_half(h, pow2i(60) / r[h]);
-        cap[h] = pow2i(kTop - 60);
-        r[h] = pow2i(60);
-      }
+      set_factor(0, h, kRowTop, 0);
   }
   // sm: the tile; in: its live rows (others are zero in memory); bias: this lane's row's (lane < 8) log2 weight
   __device__ __forceinline__ void rows(uint32_t sm, uint32_t in, float bias, float qk_scale) {
@@ -387,13 +420,17 @@ struct WarpAttention {
     float v = __shfl_sync(0xffffffffu, c[0] + c[3], lane() & 28);  // lane t = 0 of the row has it
     const float b = __shfl_sync(0xffffffffu, bias, g);
     v = (in >> g & 1u) ? fmaf(v, qk_scale, b) : -INFINITY;
-    if (__any_sync(0xffffffffu, v > m[0] + kSlack)) raise_max(v, 0);
-    const float p = ex2(v - bm[0]);
+    if (__any_sync(0xffffffffu, v > m[0] + kSlack)) {
+      const int d = raise_max(v, 0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) set_factor(0, h, kRowTop, d);
+    }
+    const float p = ex2(v - m[0]);
     l[0] += p;
     float w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float full = p * (r[h] * pow2i(h ? -20 : -24)), hi = bf_round(full);
+      const float full = p * (r(0, h) * pow2i(h ? -20 : -24)), hi = bf_round(full);
       w[h] = t == 0 ? hi : t == 1 ? full - hi : 0.f;
     }
     const uint32_t pw = transpose8x8((uint32_t)f2bf_bits(w[0]) | ((uint32_t)f2bf_bits(w[1]) << 16));
@@ -435,7 +472,7 @@ struct WarpAttention {
   // after add_up(): dims 64 h + 8 (lane / 4) .. + 7 of column j, unnormalised.  Codes were 2^-24 (half 1: 2^-20) and
   // weights r times too large; 1 / r is a power of two, exact.
   __device__ __forceinline__ void dims(int j, int h, float (&o)[8]) const {
-    const float f = 1.f / r[h], u = pow2i(h ? 20 : 24), z = zs[j][h];
+    const float f = 1.f / r(j, h), u = pow2i(h ? 20 : 24), z = zs[j][h];
     const int k = QUAD ? h : j;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -1,0 +1,66 @@
+"""Attention over the 4-bit cache where rows differ by many powers of two: a record whose V scale is far above the
+others' and whose weight makes up for it, against the definition in 64 bits (kv4_plain.py derives the tolerances)."""
+import math
+
+import pytest
+import torch
+
+import kv4_plain as P
+from openattention_b200 import kv4
+
+pytestmark = pytest.mark.gpu
+D, REC = 128, 144
+BF = torch.bfloat16
+
+
+def _far_apart(seed, heads, n, power, early):
+    """q (heads, 128) and records (n, 144).  The record at `at` has V values 2^power times the others'.
+
+    early: it is the first, its logit like its neighbours', and the second half of the tokens stand 60 (nats) above it:
+    by then its weight is 2^-86.  Else its own logit lies about 40 below the others'."""
+    g = torch.Generator().manual_seed(seed)
+    u = torch.randint(0, 2, (D,), generator=g) * 2.0 - 1
+    q = u + torch.randn(heads, D, generator=g) * 0.25
+    k, v = torch.randn(n, D, generator=g), torch.randn(n, D, generator=g)
+    at = 0 if early else n // 3
+    if early:
+        k[n // 2:] += u * 60 / (D * D ** -0.5)
+    else:
+        k[at] = -u * 40 / (D * D ** -0.5) + torch.randn(D, generator=g) * 0.1
+    v[at] *= 2.0 ** power
+    return q.to(BF), P.pack(k.to(BF), v.to(BF))
+
+
+FAR = [(26, False), (40, False), (26, True), (70, True)]
+
+
+@pytest.mark.parametrize("power,early", FAR)
+@pytest.mark.parametrize("B,HKV,G,T,n", [
+    (1, 1, 4, 1, 4096),      # a tile or two a warp, many parts
+    (16, 8, 2, 1, 4000),     # several tiles a warp
+    (16, 8, 8, 1, 4000), (16, 8, 3, 2, 4000),  # eight columns
+    (100, 4, 4, 1, 330), (100, 4, 7, 1, 330)])  # a warp a row
+def test_dense_values_far_apart(B, HKV, G, T, n, power, early):
+    q, rec = _far_apart(71 + G, HKV * G * T, n, power, early)
+    q = q.view(1, HKV * G, T, D)
+    got = kv4.decode_attention(q.cuda().expand(B, -1, -1, -1), rec.cuda().expand(B, HKV, n, REC),
+                               torch.tensor([n], device="cuda"), out_dtype=torch.float32).cpu()
+    assert torch.equal(got, got[:1].expand_as(got))
+    for h in range(0, HKV * G, 1 + HKV * G // 6):
+        for t in range(T):
+            P.check(got[0, h, t], *P.attend(q[0, h, t], rec[:n - T + 1 + t], D ** -0.5), f"head {h}, token {t}")
+
+
+@pytest.mark.parametrize("power,early", FAR)
+@pytest.mark.parametrize("rows,n,NB", [(2, 2000, 0), (40, 1300, 7), (200, 700, 9), (1100, 231, 64)])
+def test_lists_values_far_apart(rows, n, NB, power, early):
+    q, rec = _far_apart(72 + rows, rows, n, power, early)
+    g = torch.Generator().manual_seed(73)
+    kbar, vbar = torch.randn(rows, NB, D, generator=g).to(BF), torch.randn(rows, NB, D, generator=g).to(BF)
+    # with `early`, proxies stand where the late tokens do
+    log_n = torch.rand(rows, NB, generator=g) * 3 + (60 if early else 0)
+    idx = torch.arange(n, dtype=torch.int32).expand(rows, n).contiguous()
+    got = kv4.flash_attention(q.cuda(), rec.cuda()[None], idx[:, :5].contiguous().cuda(), idx[:, 5:].contiguous().cuda(),
+                              kbar.cuda(), vbar.cuda(), log_n.cuda(), out_dtype=torch.float32).cpu()
+    for r in range(0, rows, 1 + rows // 9):
+        P.check(got[r], *P.attend(q[r], rec, D ** -0.5, kbar[r], vbar[r], log_n[r]), f"row {r}")
