@@ -43,7 +43,7 @@ constexpr float kCap = 32768.f;      // p s r above it (fp16 ends at 65504) has 
 constexpr uint32_t kWide = 0x4480u;  // 2^10 = kCap / 2^kSlack in bf16
 // Where nothing was seen: under every score, and finite, so that its difference from itself is 0 and from -inf is -inf.
 constexpr float kNoMax = -3.402823466e38f;
-constexpr int kRowTop = 60;      // log2 of the largest r beside bf16 rows
+constexpr int kRowTop = 20;  // log2 of the largest r beside bf16 rows: their weights, r 2^-24 and r 2^-20 of p, stay at most p
 constexpr uint32_t kLoMask = 0x000f000fu, kHiMask = 0x00f000f0u;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -396,7 +396,7 @@ struct WarpAttention {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
     }
-    // one factor for a row's two terms; scales of records may have left one that would carry a large row past fp32
+    // one factor for a row's two terms, and none that would carry a large row past fp32
     r2[0] = __shfl_sync(0xffffffffu, r2[0], lane() & 28);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -470,14 +470,16 @@ struct WarpAttention {
     }
   }
   // after add_up(): dims 64 h + 8 (lane / 4) .. + 7 of column j, unnormalised.  Codes were 2^-24 (half 1: 2^-20) and
-  // weights r times too large; 1 / r is a power of two, exact.
+  // weights r times too large; 1 / r is a power of two, exact.  No step on the way is
+  // larger than the result: both factors in one for r >= 1, else first u, which leaves r times the result.
   __device__ __forceinline__ void dims(int j, int h, float (&o)[8]) const {
     const float f = 1.f / r(j, h), u = pow2i(h ? 20 : 24), z = zs[j][h];
+    const float first = f > 1.f ? u : 1.f, then = f > 1.f ? f : u * f;
     const int k = QUAD ? h : j;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      o[2 * i] = fmaf(acc[4 * h + i][k] * u, f, z);
-      o[2 * i + 1] = fmaf(acc[4 * h + i][2 + k] * u, f, z);
+      o[2 * i] = fmaf(acc[4 * h + i][k] * first, then, z);
+      o[2 * i + 1] = fmaf(acc[4 * h + i][2 + k] * first, then, z);
     }
   }
 

@@ -64,3 +64,24 @@ def test_lists_values_far_apart(rows, n, NB, power, early):
                               kbar.cuda(), vbar.cuda(), log_n.cuda(), out_dtype=torch.float32).cpu()
     for r in range(0, rows, 1 + rows // 9):
         P.check(got[r], *P.attend(q[r], rec, D ** -0.5, kbar[r], vbar[r], log_n[r]), f"row {r}")
+
+
+@pytest.mark.parametrize("vs,ps", [(1.0, 1e25), (1.0, 1e30), (1e30, 1e30), (1.0, 1e35), (1e30, 1.0), (1e-30, 1.0), (1.0, 1e-30),
+                                   (1e-30, 1e-30)])
+@pytest.mark.parametrize("n,NB", [(300, 20), (0, 9), (70, 3)])
+def test_lists_large_and_small_value_rows(n, NB, vs, ps):
+    """Values of the records and of the proxies far from 1, and from each other."""
+    g = torch.Generator().manual_seed(74)
+    rows = 6
+    rec = P.pack(torch.randn(400, D, generator=g).to(BF), (torch.randn(400, D, generator=g) * vs).to(BF))
+    q, kbar = torch.randn(rows, D, generator=g).to(BF), torch.randn(rows, NB, D, generator=g).to(BF)
+    vbar = (torch.randn(rows, NB, D, generator=g) * ps).to(BF)
+    log_n = torch.rand(rows, NB, generator=g) * 3
+    log_n[:2] = -math.inf                # rows without proxies
+    idx = torch.arange(n, dtype=torch.int32).expand(rows, n).contiguous()
+    none = torch.zeros(rows, 0, dtype=torch.int32)
+    for out_dtype in (BF, torch.float32):
+        got = kv4.flash_attention(q.cuda(), rec.cuda()[None], none.cuda(), idx.cuda(), kbar.cuda(), vbar.cuda(), log_n.cuda(),
+                                  out_dtype=out_dtype).cpu()
+        for r in range(rows):
+            P.check(got[r], *P.attend(q[r], rec[:n], D ** -0.5, kbar[r], vbar[r], log_n[r]), f"row {r}")
