@@ -287,8 +287,9 @@ int oa_cluster_sums(const void* K, const void* V, int64_t hkv, int64_t Lmax, int
  *
  * These entries take their arguments in one block of 8-byte fields (a decode loop that crosses a foreign-function
  * boundary per call pays for each argument there).  An oa_tensor is an address with sizes and strides in elements;
- * the entries check sizes against each other, that last dims are contiguous and that rows start on 16-byte
- * boundaries (base and strides; the stride of a dim of one element is ignored).
+ * the entries check sizes against each other, that last dims are contiguous, that rows start on 16-byte
+ * boundaries (base and strides; the stride of a dim of one element is ignored) and that rows and records that are
+ * written lie apart (from the smallest stride on, each steps over what the smaller ones span).
  *
  * Row i of request b stands at position p = start[b] + offset + i.  Per-request numbers (oa_index: start, lens, n)
  * are device int32 or int64, one for each request or one for all.  lens (p NULL: all T rows): rows i >= lens[b] are

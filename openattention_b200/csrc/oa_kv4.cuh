@@ -47,6 +47,27 @@ struct Rows {
     if (rc_ != OA_OK) return rc_; \
   } while (0)
 
+// Whether runs of `run` elements, one for each index of dims with these sizes and strides, lie apart.  From the smallest
+// stride on, each must step over everything the smaller ones span: so it is for every view that slicing, permuting
+// and splitting of dims can make of a dense tensor.
+template <int N>
+static inline bool oa_apart(const int64_t* size, const int64_t* stride, int64_t run) {
+  __int128 step[N], span = run;
+  int n = 0, order[N];
+  for (int i = 0; i < N; ++i) {
+    if (size[i] <= 1) continue;
+    step[i] = stride[i] < 0 ? -(__int128)stride[i] : (__int128)stride[i];
+    int at = n++;
+    for (; at > 0 && step[order[at - 1]] > step[i]; --at) order[at] = order[at - 1];
+    order[at] = i;
+  }
+  for (int i = 0; i < n; ++i) {
+    if (step[order[i]] < span) return false;
+    span += (size[order[i]] - 1) * step[order[i]];
+  }
+  return true;
+}
+
 // Rows (B, H, T, 128) of element size `esize` into out (strides of single-element dims cleared: any number may
 // stand there); H, T < 0: any.  Empty rows have no address.  `writes`: rows must not share memory.
 static inline int oa_take_rows(const char* fn, const char* name, const oa_tensor4& t, int esize, int64_t B, int64_t H,
@@ -65,10 +86,10 @@ static inline int oa_take_rows(const char* fn, const char* name, const oa_tensor
   int64_t st[3];
   for (int i = 0; i < 3; ++i) {
     st[i] = t.size[i] > 1 ? t.stride[i] : 0;
-    OA_REQUIRE(!writes || empty || t.size[i] <= 1 || st[i] >= oa::kD || st[i] <= -oa::kD,
-               "%s: %s must not be an expanded tensor: its rows would overlap", fn, name);
     OA_REQUIRE(st[i] * esize % 16 == 0 || empty, "%s: %s rows must start on 16-byte boundaries (strides)", fn, name);
   }
+  OA_REQUIRE(!writes || empty || oa_apart<3>(t.size, st, oa::kD),
+             "%s: %s must not be an expanded tensor or one of interleaved strides: its rows would overlap", fn, name);
   OA_REQUIRE(oa_aligned16(t.p), "%s: %s rows must start on 16-byte boundaries (base address)", fn, name);
   *out = oa::Rows{t.p, st[0], st[1], st[2]};
   return OA_OK;
@@ -100,9 +121,8 @@ static inline int oa_take_cache(const char* fn, const oa_tensor4& t, bool writes
   *sb = t.size[0] > 1 ? t.stride[0] : 0;
   *sh = t.size[1] > 1 ? t.stride[1] : 0;
   OA_REQUIRE(empty || (*sb % 16 == 0 && *sh % 16 == 0), "%s: cache strides must be multiples of 16 bytes", fn);
-  const int64_t run = t.size[2] * oa::kRec;
-  OA_REQUIRE(!writes || empty ||
-                 ((t.size[0] <= 1 || *sb >= run || *sb <= -run) && (t.size[1] <= 1 || *sh >= run || *sh <= -run)),
-             "%s: the cache must not be an expanded tensor: its requests would share records", fn);
+  const int64_t st[2] = {*sb, *sh};
+  OA_REQUIRE(!writes || empty || oa_apart<2>(t.size, st, t.size[2] * oa::kRec),
+             "%s: the cache must not be an expanded tensor or one of interleaved strides: its requests would share records", fn);
   return OA_OK;
 }
