@@ -44,15 +44,16 @@ struct RowArgs {
 };
 
 // The lane's part of a row: dims 4l .. (a) and 64 + 4l .. (b); p at dim 4l.  Held as loaded, so that several rows'
-// loads are in flight before the first is used.
+// loads are in flight before the first is used.  Plain loads: rows may be rotated where they stand, and the read-only
+// path is for memory that no one writes during the launch.
 template <typename E>
 struct Quads;
 template <>
 struct Quads<__nv_bfloat16> {
   uint2 a, b;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) {
-    a = __ldg(reinterpret_cast<const uint2*>(p));
-    b = __ldg(reinterpret_cast<const uint2*>(p + 64));
+    a = *reinterpret_cast<const uint2*>(p);
+    b = *reinterpret_cast<const uint2*>(p + 64);
   }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     x[0] = bf_lo(a.x); x[1] = bf_hi(a.x); x[2] = bf_lo(a.y); x[3] = bf_hi(a.y);
@@ -70,8 +71,8 @@ template <>
 struct Quads<float> {
   float4 a, b;
   __device__ __forceinline__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const float4*>(p));
-    b = __ldg(reinterpret_cast<const float4*>(p + 64));
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 64);
   }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
