@@ -13,9 +13,9 @@ from .geometry import D
 
 _CODE = {torch.bfloat16: _lib.OA_BF16, torch.float32: _lib.OA_F32}
 
-
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# None on a torch without CUDA, where every call is refused (its tensors are not on a GPU) before it gets here
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _bad_rows(name, t, dtype, dev):
