@@ -208,7 +208,7 @@ __device__ __forceinline__ void code_groups(const uint32_t (&v)[N], uint32_t lo2
         float d = (g ? bf_hi(v[4 * j + i]) : bf_lo(v[4 * j + i])) - lo;
         if (kLift) d *= lift;
         float q = inv.times(d);
-        if (kLift) q = fminf(q, 15.f);  // a normal scale is off by 2^-9 at most, its quotients stay under 15.1
+        if (kLift) q = fminf(q, 15.f);  // a normal scale is off by 2^-8 at most, its quotients stay under 15.06
         w[i] = __float_as_uint(q + kRound);
       }
       const uint32_t codes4 = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
