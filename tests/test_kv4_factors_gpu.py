@@ -85,3 +85,25 @@ def test_lists_large_and_small_value_rows(n, NB, vs, ps):
                                   out_dtype=out_dtype).cpu()
         for r in range(rows):
             P.check(got[r], *P.attend(q[r], rec[:n], D ** -0.5, kbar[r], vbar[r], log_n[r]), f"row {r}")
+
+
+@pytest.mark.parametrize("G", [2, 8])
+@pytest.mark.parametrize("half,power", [(0, -30), (1, -26)])
+def test_query_elements_far_apart(G, half, power):
+    """A query element of 1 meets codes of 0 only; what decides are the others, 2^-30 of it (dims 0..63) or 2^-26 (64..127),
+    which the fp16 operand still holds in full."""
+    g = torch.Generator().manual_seed(75)
+    n, H = 500, 4
+    q = torch.zeros(1, H * G, 1, D)
+    q[..., 64 * half:64 * half + 64] = (1 + torch.rand(1, H * G, 1, 64, generator=g)) * 2.0 ** power * (
+        torch.randint(0, 2, (1, H * G, 1, 64), generator=g) * 2 - 1)
+    q[..., 0] = 1.0
+    k = torch.zeros(1, H, n, D)
+    k[..., 64 * half:64 * half + 64] = torch.rand(1, H, n, 64, generator=g) * 2
+    k[..., 64 * half + 63] = 0.0          # the group's minimum, so its offset, is 0
+    k[..., 0] = 0.0
+    q, cache = q.to(BF), P.pack(k.to(BF), torch.randn(1, H, n, D, generator=g).to(BF))
+    scale = 0.25 * 2.0 ** -power
+    got = kv4.decode_attention(q.cuda(), cache.cuda(), torch.tensor([n], device="cuda"), sm_scale=scale, out_dtype=torch.float32)
+    for h in range(H * G):
+        P.check(got[0, h, 0], *P.attend(q[0, h, 0], cache[0, h // G], scale), f"head {h}")
