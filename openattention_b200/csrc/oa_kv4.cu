@@ -600,12 +600,20 @@ __device__ __forceinline__ void cluster_sync() {
 
 template <int W>
 constexpr size_t list_smem() { return (size_t)W * kStages * kTileBytes; }
+// Only CTAs of 8 warps form clusters, and leave their state where the others can read it.  What the rule for W counts on,
+// 16 warps on an SM (of 228 KB, 1 KB of it taken for each CTA), leaves two warps' CTAs no room for that.
+template <int W>
+constexpr int kClusterFloats = W == 8 ? kD + 2 : 1;
+template <int W>
+constexpr bool kSixteenWarps = 16 / W * (list_smem<W>() + kClusterFloats<W> * sizeof(float) + 1024) <= 228 * 1024;
+static_assert(kSixteenWarps<2> && kSixteenWarps<4> && kSixteenWarps<8>, "16 warps of list_kernel must fit an SM's shared memory");
 
 template <int W>
-__global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, int S) {
+__global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, int S) {  // S: CTAs of a row (W < 8: one)
   extern __shared__ __align__(16) unsigned char s_dyn[];  // [warp][stage][item]; a warp's state when it is done
-  __shared__ float s_cta[kD + 2];
+  __shared__ float s_cta[kClusterFloats<W>];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (W < 8) S = 1;
   const int rank = S > 1 ? blockIdx.x % S : 0;
   const int64_t r = blockIdx.x / S, kvh = r / a.G;
   const int nw = W * S, total = a.n_sel + a.n_exp;
@@ -713,31 +721,36 @@ __global__ void __launch_bounds__(32 * W, 16 / W) list_kernel(const ListArgs a, 
     float A = 0.f;
 #pragma unroll
     for (int i = 0; i < W; ++i) A = fmaf(f[i], st[i * kNext + d], A);
-    if (S == 1)
-      store_list(a, r, d, A, L);
-    else
-      s_cta[d] = A;
-  }
-  if (S == 1) return;
-  if (tid == 0) {
-    s_cta[kD] = M;
-    s_cta[kD + 1] = L;
-  }
-  cluster_sync();
-  if (rank == 0) {
-    M = -INFINITY;
-    for (int k = 0; k < S; ++k) M = fmaxf(M, ld_cluster(cluster_addr(s_cta + kD, k)));
-    L = 0.f;
-    for (int k = 0; k < S; ++k)
-      L = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - M), ld_cluster(cluster_addr(s_cta + kD + 1, k)), L);
-    for (int d = tid; d < kD; d += 32 * W) {
-      float A = 0.f;
-      for (int k = 0; k < S; ++k)
-        A = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - M), ld_cluster(cluster_addr(s_cta + d, k)), A);
-      store_list(a, r, d, A, L);
+    if constexpr (W == 8) {
+      if (S > 1) {
+        s_cta[d] = A;
+        continue;
+      }
     }
+    store_list(a, r, d, A, L);
   }
-  cluster_sync();  // no CTA leaves while its state is read
+  if constexpr (W == 8) {
+    if (S == 1) return;
+    if (tid == 0) {
+      s_cta[kD] = M;
+      s_cta[kD + 1] = L;
+    }
+    cluster_sync();
+    if (rank == 0) {
+      M = -INFINITY;
+      for (int k = 0; k < S; ++k) M = fmaxf(M, ld_cluster(cluster_addr(s_cta + kD, k)));
+      L = 0.f;
+      for (int k = 0; k < S; ++k)
+        L = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - M), ld_cluster(cluster_addr(s_cta + kD + 1, k)), L);
+      for (int d = tid; d < kD; d += 32 * W) {
+        float A = 0.f;
+        for (int k = 0; k < S; ++k)
+          A = fmaf(ex2(ld_cluster(cluster_addr(s_cta + kD, k)) - M), ld_cluster(cluster_addr(s_cta + d, k)), A);
+        store_list(a, r, d, A, L);
+      }
+    }
+    cluster_sync();  // no CTA leaves while its state is read
+  }
 }
 
 template <int W>
