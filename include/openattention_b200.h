@@ -361,6 +361,8 @@ typedef struct {
 int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream);
 
 /* Dense attention over the cache: q (B, HQ, T, 128) bf16 rows, out the same shape in bf16 or fp32 (out_dtype).
+ * Weight times V scale is rounded to fp16 (11 bits; 2^-11 of the sum of weight * scale * code), whatever the output's type.
+ * Elements of a query more than 2^26 below its largest are rounded; the largest may not pass 2^105.
  * Request b has min(n[b] + offset, Lmax) positions, its T query tokens are the last T of them and token i sees
  * positions <= length - T + i; one that sees none gives zeros.  Query head h reads KV head h / (HQ / HKV).
  * workspace: at least oa_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned, zero before its first use; every
@@ -377,7 +379,7 @@ int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream);
 
 /* OpenAttention.flash over the cache (BH, Lmax, 144): q (BQ, 128) bf16, sel and exp_idx (BQ, n) int32 contiguous,
  * proxies kbar, vbar (BQ, >= NB, 128) (for each query row) or (BH, >= NB, 128) (for each KV row) bf16, log_n
- * (BQ, >= NB) fp32, out (BQ, 128) in out_dtype; semantics of oa_flash_qhead_proxies / oa_flash_kvhead_proxies.
+ * (BQ, >= NB) fp32, out (BQ, 128) in out_dtype; roundings as in oa_kv4_attention, proxies' weights 16 bits; semantics of oa_flash_qhead_proxies / oa_flash_kvhead_proxies.
  * NB = 0 disables the proxies. */
 typedef struct {
   oa_tensor2 q;

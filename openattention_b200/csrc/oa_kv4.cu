@@ -60,11 +60,13 @@ __device__ __forceinline__ void store_list(const ListArgs& a, int64_t r, int d, 
 // A row that one CTA covers is written by it.  Otherwise each part leaves (m, l, O) in the workspace and the
 // last CTA to arrive (atomic ticket, no waiting) merges the parts in CTA order, so the result does not depend
 // on which CTA is last.
-// What bounds it: memory, once rows are long.  32 requests x 32768 tokens, 32 heads over 8: 190 us, 6.35 TB/s of records
-// (97% of a copy's rate), and 212-219 us in long runs, which the power limit slows.  The line reaches that where 256
-// rows with a CTA each take 207 us; the 8-column tile takes 222 us there.  Two query tokens (8 columns) are bound by
-// issue: 8 requests x 32768, 65-70 us, floor 46.  One request x 32768: 17 us, floor 6: a launch, the first loads and
-// the merge.  64 requests of 1 to 8191 tokens, two query tokens: 66 us, floor 38: what rows cost besides their tiles.
+// What bounds it: memory, once rows are long.  32 requests x 32768 tokens, 32 heads over 8: 188 us, 6.4 TB/s of records
+// (98% of a copy's rate), and 212-232 us in long runs, which the power limit slows.  The line reaches that where 256
+// rows with a CTA each take 207 us; the 8-column tile takes 222 us there.  Two query tokens (8 columns): 8 requests x
+// 32768, 65 us, floor 46, with issue active 45% of the time; the first stall is instruction fetch (the tile stands
+// four times in the kernel: masked and not, for single warps and for CTAs).  One request x 32768: 15 us, floor 6: a
+// launch, the first loads and the merge through global memory.  64 requests of 1 to 8191 tokens, two query tokens: 62
+// us, floor 38: what rows cost besides their tiles.
 constexpr int kWarps = 8;
 constexpr int kDenseThreads = 32 * kWarps;
 constexpr int kStages = 3;
@@ -140,7 +142,8 @@ __device__ __forceinline__ void store_out4(void* out, int out_f32, int64_t at, i
 // The parts of one row, part v at src (v = 0) or src + (2 v - 1) kPartFloats.  Every thread sums four dims of one
 // column over its share of the parts, kAhead loads in flight; the first ones are issued before the weights
 // 2^(m_v - M) are known.  The shares are added in a fixed order.  o_at: the output row of column `warp`.
-// Inlined, and kAhead no larger: a call, or more loads held, spills the caller's main loop.
+// Inlined, and kAhead no larger: a call, or more loads held, spills more than the caller's main loop spills as it is (4
+// bytes with four columns, 72 with eight).
 template <int kAhead>
 __device__ __forceinline__ void merge_parts(const float* src, int parts, int ncol, float* sh, void* out, int out_f32,
                                          int64_t o_at) {
@@ -580,7 +583,7 @@ __global__ void __launch_bounds__(kDenseThreads, 2) dense_kernel(const DenseArgs
 // used, which is still less work than unpacking codes to fp32 for plain FMAs (a tile of 32 takes some 350
 // instructions, against about 770 on the same pipes).  The warps' states are merged in shared memory, then over the
 // cluster.  1024 rows of 231 entries and 64 proxies: 24.6 us for 63 MB.  Latency bounds that (a launch, indices, then records:
-// DRAM at 47%, issue at 41%); longer lists add 3.75 TB/s of records, which is 5 TB/s of DRAM accesses: a scattered record
+// DRAM at 46%, issue at 42%); longer lists add 3.75 TB/s of records, which is 5 TB/s of DRAM accesses: a scattered record
 // of 144 bytes takes three or four of 64.
 constexpr int kRowsPerTile = 8;
 

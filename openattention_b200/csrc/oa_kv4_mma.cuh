@@ -8,8 +8,9 @@
 // multiply the bare codes, the scales and offsets enter after, in fp32, once per token and half.  Codes cost one AND
 // each pair: a nibble left in place in a 16-bit word is an fp16 subnormal, code * 2^-24 (low nibble) or 16 code * 2^-24
 // (high nibble), exact.  Low and high nibbles are the two halves, so the factor 16 belongs to a whole half.  q is
-// scaled by a power of two per column (largest element in [2^13, 2^14)), exact unless an element is 2^-37 of the
-// largest.  (e4m3 operands would hold a code in a byte, but mma.sync takes them apart into fp16 here: slower.)
+// scaled by a power of two per column (largest element in [2^13, 2^14), half 1 by 2^-4 more), which holds elements
+// down to 2^-30 (half 0) and 2^-26 (half 1) of the largest in full; below, they are off by 2^-25, that is by 2^-38 and
+// 2^-34 of the largest at most.  (e4m3 operands would hold a code in a byte, but mma.sync takes them apart into fp16 here: slower.)
 //
 // Values.  The scale goes into the weight: o = sum_t (p_t s_t) c_t + sum_t p_t z_t, the second sum in fp32 outside the
 // tensor cores.  p s is scaled by a power of two r per column and half and rounded to fp16: 11 bits over 20 octaves below
@@ -117,7 +118,7 @@ __device__ __forceinline__ int row_token(int r) { return (r & 1) ? 8 + ((r + 3) 
 // therefore serves one query: column 2c takes half 0 only (its q operand is zero in the other half's steps), 2c + 1
 // half 1, in scores and in weights.  Else eight columns, two queries to a lane, and the halves take sums and weights
 // of their own.  (32 requests x 32768 tokens with four queries a KV head: 190 us, 222 with eight columns; 40 x 3000: 37.0
-// and 39.6; a tile takes 480 instructions, 600 with eight columns.)
+// and 39.6; a tile takes 475 instructions, 630 with eight columns.)
 template <bool QUAD>
 struct WarpAttention {
   static constexpr int J = QUAD ? 1 : 2;  // columns (queries) of a lane
@@ -281,7 +282,8 @@ struct WarpAttention {
     // m is the same in all lanes of a column and nothing moves until some lane sees a score kSlack above it (weights
     // up to 2^kSlack are as good as weights up to 1, and new maxima are common) or a weight that fp16 may not hold.
     // That takes a scale above kCap / 2^kSlack / r; where there is one, the lane's largest weight times its largest
-    // scale is a closer bound.
+    // scale is a closer bound.  (32 requests x 32768 tokens 188 us, and 195 where every tile has such scales: an early
+    // token that takes most of the weight and whose values are 2^-10 of the others'.)
     float mx[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) mx[j] = fmaxf(fmaxf(x[0][0][j], x[0][1][j]), fmaxf(x[1][0][j], x[1][1][j]));

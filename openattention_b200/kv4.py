@@ -13,6 +13,13 @@ j + 64 in its high one; a value is scale * code + offset.  The offset is the gro
 bf16((max - min) / 15), the code min(rint((x - offset) / scale), 15), so a value is off by at most about half a
 scale.  A group that holds an infinity or a NaN reads back as NaN.
 
+Attention multiplies the codes on the tensor cores.  There the product of a token's weight and its V scale is rounded
+to fp16, 11 bits, in fp32 outputs too: a result is off by up to 2^-11 of the sum of weight * scale * code over its
+tokens (5e-4 of it is typical for unit normal values), and fp32 outputs save the last rounding only.  Softmax maxima and
+sums, offsets and proxies stay in fp32 (proxies' weights 16 bits).  The sum of weight * value is formed before it is
+divided by the weights' sum, so values whose sum passes fp32 overflow.  Elements of one query more than 2^26 below its
+largest are rounded, and the largest may not pass 2^105.
+
 Positions are device arrays (int32 or int64, one for each request or one for all), so every call can be captured
 in a CUDA graph and replayed as they advance.  Forward only; everything runs on the current CUDA stream.
 """
@@ -142,7 +149,7 @@ def _workspace(dev, *sizes):
 
 def decode_attention(q, cache, n, *, offset=0, sm_scale=None, out_dtype=None, out=None, workspace=None):
     """q (B, HQ, T, 128) bf16 over the cache (B, hkv, Lmax, 144) -> (B, HQ, T, 128) in out_dtype (bf16, the
-    default, or fp32).
+    default, or fp32; either holds about 11 bits of the codes' part, see above).
 
     n (B,) or (1,) int32 or int64 on the device: request b's length is min(n[b] + offset, Lmax), its T query
     tokens the last T positions; token i sees positions <= length - T + i.  HQ is a multiple of hkv, query head h
@@ -190,7 +197,7 @@ def _list(t, dev):
 def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, sm_scale=None, out_dtype=None,
                     out=None):
     """flash.ours_flash / flash.decode_expand_attention over a 4-bit cache: q (BQ, 128) bf16, cache (BH, Lmax, 144)
-    -> (BQ, 128).  Row r reads KV row r // (BQ // BH).
+    -> (BQ, 128) in out_dtype (bf16 or fp32, with about 11 bits of the codes' part, see above).  Row r reads KV row r // (BQ // BH).
 
     One softmax over the tokens of sel_idx (BQ, n_sel) and exp_idx (BQ, n_exp) (int32; an index outside [0, Lmax)
     is padding) and nb cluster proxies with logits q . kbar * sm_scale + log_n (log_n = -inf skips one).
