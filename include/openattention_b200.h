@@ -361,7 +361,7 @@ typedef struct {
 int oa_kv4_unpack(const oa_kv4_unpack_args* args, void* stream);
 
 /* Dense attention over the cache: q (B, HQ, T, 128) bf16 rows, out the same shape in bf16 or fp32 (out_dtype).
- * Weight times V scale is rounded to fp16 (11 bits; 2^-11 of the sum of weight * scale * code), whatever the output's type.
+ * Weight times V scale is rounded to fp16 (11 bits; 2^-11 of the sum of weight * 15 * scale), whatever the output's type.
  * Elements of a query more than 2^26 below its largest are rounded; the largest may not pass 2^105.
  * Request b has min(n[b] + offset, Lmax) positions, its T query tokens are the last T of them and token i sees
  * positions <= length - T + i; one that sees none gives zeros.  Query head h reads KV head h / (HQ / HKV).

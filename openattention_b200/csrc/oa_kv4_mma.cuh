@@ -16,8 +16,9 @@
 // tensor cores.  p s is scaled by a power of two r per column and half and rounded to fp16: 11 bits over 20 octaves below
 // the largest p s seen, beneath them off by 2^-31 of that.  r is chosen from weight times scale, not from the scale alone:
 // a record of huge scale and no weight (or whose weight the running maximum took away later) must not push what the
-// others give beneath fp16.  Running maxima are whole numbers (of log2 units, rounded up), so that weights, sums
-// and r move by exact powers of two and what a larger maximum takes from the weights r can give back.
+// others give beneath fp16.  A column's running maximum is its first tile's, so that a row's only token weighs exactly 1,
+// and from there moves by whole octaves (up to the next), so that weights, sums and r move by powers of two and what a
+// larger maximum takes from the weights r can give back.
 //
 // Tensor cores truncate their running sums.  Codes are all positive, so sums of p s c would grow with the context
 // and with them the truncation, while the offsets' part cancels most of them (1.1e-2 of the result was seen at
@@ -217,10 +218,10 @@ struct WarpAttention {
   // Column j's running maximum takes in mx (the lane's largest score): by how many octaves its weights fall.  Sums of
   // weights follow; the accumulators' part is set_factor's.
   __device__ __forceinline__ int raise_max(float mx, int j) {
-    const float nm = fmaxf(m[j], ceilf(column_max(mx)));
-    const int d = nm > m[j] ? (int)fminf(nm - m[j], 300.f) : 0;
+    const float to = column_max(mx), up = ceilf(to - m[j]);
+    const int d = up > 0.f ? (int)fminf(up, 300.f) : 0;
     const float al = d > 126 ? 0.f : pow2i(-d);
-    m[j] = nm;
+    if (d > 0) m[j] = d == 300 ? to : m[j] + up;  // none before, or nothing left of it
     l[j] *= al;
     zs[j][0] *= al;
     zs[j][1] *= al;

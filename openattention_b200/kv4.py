@@ -14,7 +14,7 @@ bf16((max - min) / 15), the code min(rint((x - offset) / scale), 15), so a value
 scale.  A group that holds an infinity or a NaN reads back as NaN.
 
 Attention multiplies the codes on the tensor cores.  There the product of a token's weight and its V scale is rounded
-to fp16, 11 bits, in fp32 outputs too: a result is off by up to 2^-11 of the sum of weight * scale * code over its
+to fp16, 11 bits, in fp32 outputs too: a result is off by up to 2^-11 of the sum of weight * 15 * scale over its
 tokens (5e-4 of it is typical for unit normal values), and fp32 outputs save the last rounding only.  Softmax maxima and
 sums, offsets and proxies stay in fp32 (proxies' weights 16 bits).  The sum of weight * value is formed before it is
 divided by the weights' sum, so values whose sum passes fp32 overflow.  Elements of one query more than 2^26 below its

@@ -107,3 +107,25 @@ def test_query_elements_far_apart(G, half, power):
     got = kv4.decode_attention(q.cuda(), cache.cuda(), torch.tensor([n], device="cuda"), sm_scale=scale, out_dtype=torch.float32)
     for h in range(H * G):
         P.check(got[0, h, 0], *P.attend(q[0, h, 0], cache[0, h // G], scale), f"head {h}")
+
+
+@pytest.mark.parametrize("scale", [D ** -0.5, 3.7, -0.01])
+@pytest.mark.parametrize("G,T", [(1, 1), (4, 1), (8, 1), (3, 2)])
+def test_one_token_gives_its_values(G, T, scale):
+    """A softmax over one token, or over copies of one, is the token's values: the weight is 1 and its product with a bf16
+    scale holds in fp16, so only fp32 roundings remain (of scale * code + offset, in up to four steps, and the division)."""
+    g = torch.Generator().manual_seed(76)
+    B, H, n = 3, 4, 9
+    rec = P.pack(*(torch.randn(B, H, 1, D, generator=g).to(BF) for _ in range(2)))
+    q = torch.randn(B, H * G, T, D, generator=g).to(BF)
+    code, s, z = (t.repeat_interleave(G, 1) for t in P.parts(rec, 1))  # (B, H * G, 1, 128)
+    want, slack = s * code + z, 8 * 2.0 ** -24 * (15 * s + z.abs())
+    for m in (1, n):
+        lens = torch.full((B,), m + T - 1, dtype=torch.int32, device="cuda")
+        got = kv4.decode_attention(q.cuda(), rec.cuda().expand(B, H, 1, REC).repeat(1, 1, n + T, 1), lens, sm_scale=scale,
+                                   out_dtype=torch.float32)
+        P.check(got[:, :, :1], want, slack, f"{m} tokens")
+        i = torch.zeros(B * H * G, m, dtype=torch.int32, device="cuda")
+        got = kv4.flash_attention(q[:, :, 0].reshape(-1, D).cuda(), rec.view(B * H, 1, REC).cuda(), i[:, :0], i, None, None, None,
+                                  sm_scale=scale, out_dtype=torch.float32)
+        P.check(got.view(B, H * G, 1, D), want, slack, f"list of {m}")
