@@ -379,8 +379,8 @@ int oa_kv4_attention(const oa_kv4_attention_args* args, void* stream);
 
 /* OpenAttention.flash over the cache (BH, Lmax, 144): q (BQ, 128) bf16, sel and exp_idx (BQ, n) int32 contiguous,
  * proxies kbar, vbar (BQ, >= NB, 128) (for each query row) or (BH, >= NB, 128) (for each KV row) bf16, log_n
- * (BQ, >= NB) fp32, out (BQ, 128) in out_dtype; roundings as in oa_kv4_attention, proxies' weights 16 bits; semantics of oa_flash_qhead_proxies / oa_flash_kvhead_proxies.
- * NB = 0 disables the proxies. */
+ * (BQ, >= NB) fp32, out (BQ, 128) in out_dtype; roundings as in oa_kv4_attention, proxies' weights 16 bits;
+ * semantics of oa_flash_qhead_proxies / oa_flash_kvhead_proxies.  NB = 0 disables the proxies. */
 typedef struct {
   oa_tensor2 q;
   oa_tensor3 cache;

@@ -10,7 +10,8 @@
 // (high nibble), exact.  Low and high nibbles are the two halves, so the factor 16 belongs to a whole half.  q is
 // scaled by a power of two per column (largest element in [2^13, 2^14), half 1 by 2^-4 more), which holds elements
 // down to 2^-30 (half 0) and 2^-26 (half 1) of the largest in full; below, they are off by 2^-25, that is by 2^-38 and
-// 2^-34 of the largest at most.  (e4m3 operands would hold a code in a byte, but mma.sync takes them apart into fp16 here: slower.)
+// 2^-34 of the largest at most.  (e4m3 operands would hold a code in a byte, but mma.sync takes them apart into fp16
+// here: slower.)
 //
 // Values.  The scale goes into the weight: o = sum_t (p_t s_t) c_t + sum_t p_t z_t, the second sum in fp32 outside the
 // tensor cores.  p s is scaled by a power of two r per column and half and rounded to fp16: 11 bits over 20 octaves below
@@ -473,8 +474,8 @@ struct WarpAttention {
     }
   }
   // after add_up(): dims 64 h + 8 (lane / 4) .. + 7 of column j, unnormalised.  Codes were 2^-24 (half 1: 2^-20) and
-  // weights r times too large; 1 / r is a power of two, exact.  No step on the way is
-  // larger than the result: both factors in one for r >= 1, else first u, which leaves r times the result.
+  // weights r times too large; 1 / r is a power of two, exact.  No step on the way is larger than the result: both
+  // factors in one for r >= 1, else first u, which leaves r times the result.
   __device__ __forceinline__ void dims(int j, int h, float (&o)[8]) const {
     const float f = 1.f / r(j, h), u = pow2i(h ? 20 : 24), z = zs[j][h];
     const float first = f > 1.f ? u : 1.f, then = f > 1.f ? f : u * f;

@@ -13,9 +13,9 @@
 // token's rows two at a time ("slots": two query rows, or the K and the V row of one head, whose record it writes
 // whole), kSlots loads in flight; cos and sin stay in registers for all of them.
 //
-// What bounds it: memory, for long prompts.  32768 tokens of 32 + 8 heads in bf16: 109 us, 6.5 TB/s (with the norm 119); rope_append
-// 129 us, floor 113.  Four loads in flight against one: 112 and 142 us; a warp for a whole token
-// against one for every slot: 112 and 242.  A decode step's rows take a launch's time.
+// What bounds it: memory, for long prompts.  32768 tokens of 32 + 8 heads in bf16: 109 us, 6.5 TB/s (with the norm 119);
+// rope_append 129 us, floor 113.  Four loads in flight against one: 112 and 142 us; a warp for a whole token against
+// one for every slot: 112 and 242.  A decode step's rows take a launch's time.
 #include "oa_kv4.cuh"
 
 namespace oa {

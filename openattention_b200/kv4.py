@@ -197,7 +197,8 @@ def _list(t, dev):
 def flash_attention(q, cache, sel_idx, exp_idx, kbar, vbar, log_n, nb=None, *, sm_scale=None, out_dtype=None,
                     out=None):
     """flash.ours_flash / flash.decode_expand_attention over a 4-bit cache: q (BQ, 128) bf16, cache (BH, Lmax, 144)
-    -> (BQ, 128) in out_dtype (bf16 or fp32, with about 11 bits of the codes' part, see above).  Row r reads KV row r // (BQ // BH).
+    -> (BQ, 128) in out_dtype (bf16 or fp32, with about 11 bits of the codes' part, see above).  Row r reads KV row
+    r // (BQ // BH).
 
     One softmax over the tokens of sel_idx (BQ, n_sel) and exp_idx (BQ, n_exp) (int32; an index outside [0, Lmax)
     is padding) and nb cluster proxies with logits q . kbar * sm_scale + log_n (log_n = -inf skips one).
